@@ -23,6 +23,8 @@ OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_POW = 0, 1, 2, 3, 4
 OP_RELU, OP_GELU, OP_ERF, OP_SQRT, OP_COPY = 16, 17, 18, 19, 20
 REDUCE_MEAN, REDUCE_SUM, REDUCE_MAX, REDUCE_MIN = 0, 1, 2, 3
 OP_LOG, OP_TANH, OP_SIGMOID, OP_SOFTPLUS, OP_RECIPROCAL, OP_EXP, OP_NEG, OP_ABS = 21, 22, 23, 24, 25, 26, 27, 28
+#: what QuantizedLinear's `activation` may say
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 PROGRAM_REG, PROGRAM_TENSOR, PROGRAM_VECTOR, PROGRAM_IMMEDIATE = 0, 1, 2, 3
 PROGRAM_MAX_INSTR, PROGRAM_MAX_TENSORS, PROGRAM_MAX_VECTORS, PROGRAM_MAX_IMM = 16, 4, 4, 8
 
@@ -91,6 +93,12 @@ SIGNATURES: typing.Dict[str, typing.Tuple[typing.Any, typing.List[typing.Any]]] 
     "mi355x_eltwise_program_f32": (_int, [ctypes.POINTER(ctypes.c_void_p), _int, ctypes.POINTER(ctypes.c_void_p), _int, _vp,
                                           _i64, _i64, ctypes.POINTER(ctypes.c_uint32), _int,
                                           ctypes.POINTER(ctypes.c_float), _int, _vp]),
+    "mi355x_skip_rms_norm": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _f32, _vp]),
+    "mi355x_quantized_linear": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp]),
+    "mi355x_rotary_positions": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _c_i64_p, _int, _int, _int, _vp]),
+    "mi355x_differential_attention_splits": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "mi355x_differential_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                             _f32, _f32, _int, _i64, _int, _vp]),
     "mi355x_program_function": (_int, [ctypes.c_char_p]),
     "mi355x_program_run": (_i64, [_vp, _i64, _i64, _vp, _i64, _vp, _vp]),
 }

@@ -64,7 +64,9 @@ constexpr Function kFunctions[] = {
     MI355X_FUNCTION(mi355x_attention_f32), MI355X_FUNCTION(mi355x_attention_masked_f32), MI355X_FUNCTION(mi355x_layernorm_f32), MI355X_FUNCTION(mi355x_layernorm_parts_f32), MI355X_FUNCTION(mi355x_gemm_parts_f32), MI355X_FUNCTION(mi355x_gemm_softmax_f32),
     MI355X_FUNCTION(mi355x_reduce_mean_f32), MI355X_FUNCTION(mi355x_reduce_f32), MI355X_FUNCTION(mi355x_reduce_nd_f32),
     MI355X_FUNCTION(mi355x_maxpool2d_f32), MI355X_FUNCTION(mi355x_batchnorm_f32), MI355X_FUNCTION(mi355x_eltwise_f32),
-    MI355X_FUNCTION(mi355x_eltwise_program_f32), MI355X_FUNCTION(mi355x_permute_b32), MI355X_FUNCTION(mi355x_cast)};
+    MI355X_FUNCTION(mi355x_eltwise_program_f32), MI355X_FUNCTION(mi355x_permute_b32), MI355X_FUNCTION(mi355x_cast),
+    MI355X_FUNCTION(mi355x_skip_rms_norm), MI355X_FUNCTION(mi355x_quantized_linear), MI355X_FUNCTION(mi355x_rotary_positions),
+    MI355X_FUNCTION(mi355x_differential_attention)};
 #undef MI355X_FUNCTION
 constexpr int kNumFunctions = sizeof(kFunctions) / sizeof(kFunctions[0]);
 

@@ -44,6 +44,8 @@ def clean_onnx_name(name: str) -> str:
 
 
 def onnx_tensor_type_to_typeclass(elem_type: int) -> dace.typeclass:
+    if elem_type == TensorProto.BFLOAT16:
+        return dace.bfloat16
     try:
         return dace.typeclass_of(proto.tensor_dtype_to_np_dtype(elem_type))
     except KeyError:
@@ -321,7 +323,7 @@ class ONNXModel:
             if tensor.name in params:
                 weight = params[tensor.name].detach()
         if weight is None:
-            weight, owner = torch.from_numpy(np.array(tensor.array, copy=True).reshape(tensor.dims)), None
+            weight, owner = dace.from_numpy(np.array(tensor.array, copy=True).reshape(tensor.dims), dtype), None
         else:
             owner = weight
         weight = weight.to(self.device).contiguous()
@@ -495,7 +497,7 @@ class ONNXModel:
                 if not v.is_contiguous():
                     v = v.contiguous()
             else:
-                v = torch.from_numpy(np.ascontiguousarray(np.asarray(v, dtype=desc.dtype.np_dtype))).to(self.device)
+                v = dace.from_numpy(np.asarray(v, dtype=desc.dtype.np_dtype), desc.dtype).to(self.device)
             call[clean_onnx_name(n)] = v
         outputs = collections.OrderedDict()
         packed = self._packed_now() if self._packed else []
@@ -533,7 +535,7 @@ class ONNXModel:
                                                                           device=self.device)
             weights = self._own_weights()
             compiled(**call, **out_kwargs, **(self._weight_args(weights, packed) if packed else weights))
-        results = [t if use_torch else t.cpu().numpy() for t in outputs.values()]
+        results = [t if use_torch else dace.to_numpy(t) for t in outputs.values()]
         return results[0] if len(results) == 1 else tuple(results)
 
 

@@ -45,7 +45,7 @@ from ... import _lib
 from ...sdfg import SDFG, SDFGState, Ptr, Stream, I64Array, U32Array, F32Array, PtrArray, AliasNode
 from ...util.utils import in_desc_with_name, out_desc_with_name, prod
 from ..forward_implementation_abc import ONNXForward
-from .utils import op_implementation, kernel_call_for_node
+from .utils import op_implementation, kernel_call_for_node, empty_sdfg_for_node
 
 IMPLEMENTATION_NAME = "mi355x"
 MAX_ELTWISE_DIMS = 8
@@ -848,6 +848,190 @@ class MI355XLayerNormalization(ONNXForward):
         beta = "B" if _has_input(node, state, "B") else None
         return kernel_call_for_node(node, state, "mi355x_layernorm_f32", [
             Ptr("X"), Ptr("Scale"), Ptr(beta), Ptr("Y"), rows, cols, float(node.epsilon), Stream()])
+
+
+# ------------------------------------------------------------------------------------
+# quantised and differential transformers (no node of the reference's)
+
+# ONNX TensorProto data types of the arrays that these kernels compute with in float32
+_MIXED_TYPES = {"float32": 1, "float16": 10, "bfloat16": 16}
+
+
+def _mixed_type(*descs):
+    """The element type that all of ``descs`` have, None if they differ or it is none of those."""
+    names = {d.dtype.name for d in descs}
+    return _MIXED_TYPES.get(names.pop()) if len(names) == 1 else None
+
+
+def _descs(node, state, sdfg, inputs=(), outputs=()):
+    """The descriptors of the connected ones among the connectors, None for the others."""
+    return [in_desc_with_name(node, state, sdfg, c) if _has_input(node, state, c) else None for c in inputs] + \
+        [out_desc_with_name(node, state, sdfg, c) if _has_output(node, state, c) else None for c in outputs]
+
+
+@op_implementation(op="SkipRMSNormalization", name=IMPLEMENTATION_NAME)
+class MI355XSkipRMSNormalization(ONNXForward):
+    """Sum with the residual, root-mean-square norm and its quantisation to eight bits in one pass over memory."""
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        X, gain, skip, Y, Sum, Q, scale = _descs(node, state, sdfg, ("X", "Scale", "skip"), ("Y", "Sum", "Q", "q_scale"))
+        like_x = [d for d in (X, skip, Y, Sum) if d is not None]
+        kind = _mixed_type(gain, *like_x)
+        shape, axis = tuple(X.shape), int(node.axis)
+        if kind is None or not _contig(*(d for d in (gain, Q, scale, *like_x) if d is not None)) or not -len(shape) <= axis < len(shape):
+            return None
+        rows, cols = prod(shape[:axis % len(shape)]), prod(shape[axis % len(shape):])
+        if gain.total_size != cols or any(tuple(d.shape) != shape for d in like_x) or (rows and not cols):
+            return None
+        if (Q is None) != (scale is None) or (Y is None and Sum is None and Q is None) or not 0 <= float(node.epsilon) < float("inf"):
+            return None
+        if Q is not None and (Q.dtype != dace.int8 or tuple(Q.shape) != shape or not _is_f32(scale) or scale.total_size != rows):
+            return None
+        return rows, cols, kind
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XSkipRMSNormalization._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        rows, cols, kind = MI355XSkipRMSNormalization._plan(node, state, sdfg)
+        optional = lambda name, has: Ptr(name if has(node, state, name) else None)  # noqa: E731
+        return kernel_call_for_node(node, state, "mi355x_skip_rms_norm", [
+            Ptr("X"), optional("skip", _has_input), Ptr("Scale"), *(optional(c, _has_output) for c in ("Y", "Sum", "Q", "q_scale")),
+            rows, cols, kind, float(node.epsilon), Stream()])
+
+
+@op_implementation(op="QuantizedLinear", name=IMPLEMENTATION_NAME)
+class MI355XQuantizedLinear(ONNXForward):
+    """int8 rows times int8 weights on the matrix unit, with scales, bias, activation and residual where the sums are."""
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        X, W, xs, ws, bias, residual, Y = _descs(node, state, sdfg, ("X", "W", "x_scale", "w_scale", "B", "residual"), ("Y", ))
+        kind = _mixed_type(*(d for d in (bias, residual, Y) if d is not None))
+        if kind is None or kind != int(node.to) or node.activation not in _lib.ACTIVATIONS:
+            return None
+        if X.dtype != dace.int8 or W.dtype != dace.int8 or not _is_f32(xs, ws) or len(X.shape) < 1 or len(W.shape) != 2 or X.shape[-1] != W.shape[1]:
+            return None
+        lead, N, K = tuple(X.shape[:-1]), W.shape[0], W.shape[1]
+        if not _contig(*(d for d in (X, W, xs, ws, bias, residual, Y) if d is not None)) or K >= 1 << 17:
+            return None
+        if any(d is not None and tuple(d.shape) != lead + (N, ) for d in (residual, Y)) or (bias is not None and tuple(bias.shape) != (N, )):
+            return None
+        M = prod(lead)
+        if xs.total_size != 1 and tuple(xs.shape) not in (lead, lead + (1, )) or ws.total_size != 1 and tuple(ws.shape) != (N, ):
+            return None
+        return M, N, K, xs.total_size, ws.total_size, kind
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XQuantizedLinear._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        M, N, K, x_scales, w_scales, kind = MI355XQuantizedLinear._plan(node, state, sdfg)
+        optional = lambda name: Ptr(name if _has_input(node, state, name) else None)  # noqa: E731
+        return kernel_call_for_node(node, state, "mi355x_quantized_linear", [
+            Ptr("X"), Ptr("W"), Ptr("x_scale"), Ptr("w_scale"), optional("B"), optional("residual"), Ptr("Y"), M, N, K, x_scales, w_scales,
+            _lib.ACTIVATIONS[node.activation], kind, Stream()])
+
+
+@op_implementation(op="RotaryPositions", name=IMPLEMENTATION_NAME)
+class MI355XRotaryPositions(ONNXForward):
+    """Queries and keys of a layer turned in one launch, the angles of a token computed once for all heads."""
+
+    MAX_AXES = 8
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        Q, positions, frequencies, K, Q_out, K_out = _descs(node, state, sdfg, ("Q", "positions", "frequencies", "K"), ("Q_out", "K_out"))
+        if (K is None) != (K_out is None):
+            return None
+        heads = [d for d in (Q, K, Q_out, K_out) if d is not None]
+        kind = _mixed_type(*heads)
+        if kind is None or not _contig(positions, frequencies, *heads) or any(len(d.shape) != 4 for d in heads) or not _is_f32(frequencies):
+            return None
+        B, S, H, D = Q.shape
+        if tuple(Q_out.shape) != (B, S, H, D) or K is not None and (tuple(K_out.shape) != tuple(K.shape) or (K.shape[0], K.shape[1], K.shape[3]) != (B, S, D)):
+            return None
+        if positions.dtype not in (dace.int32, dace.int64) or len(positions.shape) != 3 or tuple(positions.shape[1:]) != (B, S) or len(frequencies.shape) != 1:
+            return None
+        axes, pairs = positions.shape[0], frequencies.shape[0]
+        sections = [int(n) for n in node.sections] if node.sections is not None else [pairs] + [0] * (axes - 1)
+        if not 1 <= axes <= MI355XRotaryPositions.MAX_AXES or len(sections) != axes or min(sections) < 0 or sum(sections) != pairs or 2 * pairs > D:
+            return None
+        if pairs > 2048 or D > 1 << 16 or max(H, K.shape[2] if K is not None else 0) > 1 << 12:
+            return None
+        return B * S, H, K.shape[2] if K is not None else 0, D, 2 * pairs, axes, sections, positions.dtype.bytes, kind
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XRotaryPositions._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        tokens, heads, kv_heads, size, rotated, axes, sections, position_bytes, kind = MI355XRotaryPositions._plan(node, state, sdfg)
+        K, K_out = (Ptr(c if _has_input(node, state, "K") else None) for c in ("K", "K_out"))
+        return kernel_call_for_node(node, state, "mi355x_rotary_positions", [
+            Ptr("Q"), K, Ptr("positions"), Ptr("frequencies"), Ptr("Q_out"), K_out, tokens, heads, kv_heads, size, rotated, axes,
+            I64Array(sections), int(bool(node.interleaved)), position_bytes, kind, Stream()])
+
+
+@op_implementation(op="DifferentialAttention", name=IMPLEMENTATION_NAME)
+class MI355XDifferentialAttention(ONNXForward):
+    """Both softmax maps of every head, their difference and its product with the values in one launch; with few queries the keys
+    are dealt to several workgroups and a second launch joins their sums, which stand in a transient of the graph."""
+
+    HEAD_SIZES = (32, 64, 128)
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        vectors = ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")
+        Q, K, V, lengths, *learned, O = _descs(node, state, sdfg, ("Q", "K", "V", "lengths") + vectors, ("O", ))
+        kind = _mixed_type(Q, K, V, O)
+        if kind is None or any(len(d.shape) != 4 for d in (Q, K, V, O)) or not _contig(Q, K, V, O, *learned):
+            return None
+        (B, Sq, H2, D), (Sk, G2) = Q.shape, K.shape[1:3]
+        H, G = H2 // 2, G2 // 2
+        if H2 % 2 or G2 % 2 or not G or H % G or D not in MI355XDifferentialAttention.HEAD_SIZES:
+            return None
+        if tuple(K.shape) != (B, Sk, G2, D) or tuple(V.shape) != (B, Sk, G, 2 * D) or tuple(O.shape) != (B, Sq, H, 2 * D):
+            return None
+        if not _is_f32(*learned) or any(len(d.shape) != 1 or d.shape != learned[0].shape for d in learned):
+            return None
+        if lengths is not None and (lengths.dtype != dace.int32 or tuple(lengths.shape) != (B, ) or not _contig(lengths)):
+            return None
+        scale = float(D) ** -0.5 if node.scale is None else float(node.scale)
+        if not 0 < scale < float("inf"):
+            return None
+        return B, Sq, Sk, H, G, D, learned[0].shape[0], scale, kind
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XDifferentialAttention._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        B, Sq, Sk, H, G, D, vector, scale, kind = MI355XDifferentialAttention._plan(node, state, sdfg)
+        splits = _lib.library().mi355x_differential_attention_splits(B, Sq, Sk, H, G, D, kind)
+        lengths = "lengths" if _has_input(node, state, "lengths") else None
+        call = kernel_call_for_node(node, state, "mi355x_differential_attention", [
+            *(Ptr(c) for c in ("Q", "K", "V", "lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")), Ptr(lengths), Ptr("O"),
+            Ptr("_scratch" if splits > 1 else None), B, Sq, Sk, H, G, D, vector, float(node.lambda_init), scale, int(bool(node.causal)), splits, kind, Stream()])
+        if splits == 1:
+            return call
+        nsdfg, nstate, inputs, outputs = empty_sdfg_for_node(sdfg, state, node)
+        nsdfg.add_transient("_scratch", [splits * B * Sq * H * (4 * D + 4)], dace.float32)
+        call.add_out_connector("_scratch")
+        nstate.add_node(call)
+        for side, array in inputs.items():
+            nstate.add_edge(array, None, call, side, nsdfg.make_array_memlet(side))
+        for side, array in outputs.items():
+            nstate.add_edge(call, side, array, None, nsdfg.make_array_memlet(side))
+        nstate.add_edge(call, "_scratch", nstate.add_write("_scratch"), None, nsdfg.make_array_memlet("_scratch"))
+        return nsdfg
 
 
 # ------------------------------------------------------------------------------------

@@ -23,6 +23,7 @@ import numpy as np
 class TensorProto:
     # element types (onnx.TensorProto.DataType)
     UNDEFINED, FLOAT, UINT8, INT8, UINT16, INT16, INT32, INT64, STRING, BOOL, FLOAT16, DOUBLE = range(12)
+    BFLOAT16 = 16   # (numpy has no such type: `array` holds its values in float32)
 
     def __init__(self, name="", dims=(), data_type=FLOAT, array: typing.Optional[np.ndarray] = None):
         self.name = name
@@ -38,6 +39,18 @@ _NP_OF = {
     TensorProto.DOUBLE: np.float64,
 }
 _ONNX_OF = {np.dtype(v): k for k, v in _NP_OF.items()}
+_NP_OF[TensorProto.BFLOAT16] = np.float32
+
+
+def _bfloat16_bits(values: np.ndarray) -> np.ndarray:
+    """float32 values rounded to the nearest bfloat16, as their 16 bits."""
+    bits = np.ascontiguousarray(values, dtype=np.float32).view(np.uint32)
+    rounded = ((bits.astype(np.uint64) + 0x7FFF + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(values), ((bits >> 16) | 0x40).astype(np.uint16), rounded)
+
+
+def _bfloat16_values(bits: np.ndarray) -> np.ndarray:
+    return (np.asarray(bits).astype(np.uint32) << 16).view(np.float32)
 
 
 def tensor_dtype_to_np_dtype(data_type: int):
@@ -125,6 +138,11 @@ class helper:
         return NodeProto(op_type, inputs, outputs, name, attrs, domain)
 
     @staticmethod
+    def make_tensor(name, data_type, dims, vals) -> TensorProto:
+        array = np.asarray(vals).astype(tensor_dtype_to_np_dtype(data_type)).reshape(dims)
+        return TensorProto(name, dims, data_type, _bfloat16_values(_bfloat16_bits(array)) if data_type == TensorProto.BFLOAT16 else array)
+
+    @staticmethod
     def make_tensor_value_info(name, elem_type, shape) -> ValueInfoProto:
         return ValueInfoProto(name, elem_type, shape)
 
@@ -199,6 +217,8 @@ def _ser_tensor(t: TensorProto) -> bytes:
     if t.name:
         out += _f_bytes(8, t.name)
     arr = np.ascontiguousarray(t.array).astype(tensor_dtype_to_np_dtype(t.data_type), copy=False)
+    if t.data_type == TensorProto.BFLOAT16:
+        arr = _bfloat16_bits(arr)
     out += _f_bytes(9, arr.astype(arr.dtype.newbyteorder("<"), copy=False).tobytes())
     return out
 
@@ -344,7 +364,9 @@ def _parse_tensor(b: bytes) -> TensorProto:
         elif f in (5, 7, 11):
             typed[f].extend(_packed_varints(v) if wt == _BYTES else [_signed(v)])
     dtype = tensor_dtype_to_np_dtype(t.data_type)
-    if raw is not None:
+    if t.data_type == TensorProto.BFLOAT16:
+        arr = _bfloat16_values(np.frombuffer(raw, dtype="<u2") if raw is not None else np.array(typed[5], dtype=np.uint16))
+    elif raw is not None:
         arr = np.frombuffer(raw, dtype=dtype.newbyteorder("<")).astype(dtype)
     else:
         src = {TensorProto.FLOAT: 4, TensorProto.DOUBLE: 10, TensorProto.INT64: 7}.get(t.data_type, 5)

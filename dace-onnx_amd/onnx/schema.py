@@ -74,6 +74,8 @@ _A = ONNXAttributeType
 _FLOATS = [dace.float16, dace.float32, dace.float64]
 _NUMERIC = _FLOATS + [dace.int32, dace.int64, dace.uint8, dace.int8, dace.int16]
 _ANY = _NUMERIC + [dace.bool_]
+_HELD = _ANY + [dace.bfloat16]   # of nodes that move values without looking at them
+_MIXED = [dace.float32, dace.float16, dace.bfloat16]   # of nodes that compute in float32 whatever their arrays hold
 
 
 def _unary(name, version, in_name, out_name, types=_FLOATS, attributes=(), doc=""):
@@ -132,12 +134,48 @@ SCHEMAS: typing.List[ONNXSchema] = [
     _unary("Abs", 6, "X", "Y", types=_NUMERIC),
     ONNXSchema("Reshape", 5, [ONNXParameter("data", "T"), ONNXParameter("shape", "tensor(int64)")],
                [ONNXParameter("reshaped", "T")], (),
-               [ONNXTypeConstraint("T", _ANY), ONNXTypeConstraint("tensor(int64)", [dace.int64])]),
+               [ONNXTypeConstraint("T", _HELD), ONNXTypeConstraint("tensor(int64)", [dace.int64])]),
     _unary("Transpose", 1, "data", "transposed", types=_ANY, attributes=[ONNXAttribute("perm", _A.Ints)]),
-    _unary("Flatten", 11, "input", "output", types=_ANY, attributes=[ONNXAttribute("axis", _A.Int, 1)]),
-    _unary("Identity", 1, "input", "output", types=_ANY),
-    _unary("Squeeze", 11, "data", "squeezed", types=_ANY, attributes=[ONNXAttribute("axes", _A.Ints)]),
-    _unary("Unsqueeze", 11, "data", "expanded", types=_ANY, attributes=[ONNXAttribute("axes", _A.Ints, required=True)]),
+    _unary("Flatten", 11, "input", "output", types=_HELD, attributes=[ONNXAttribute("axis", _A.Int, 1)]),
+    _unary("Identity", 1, "input", "output", types=_HELD),
+    _unary("Squeeze", 11, "data", "squeezed", types=_HELD, attributes=[ONNXAttribute("axes", _A.Ints)]),
+    _unary("Unsqueeze", 11, "data", "expanded", types=_HELD, attributes=[ONNXAttribute("axes", _A.Ints, required=True)]),
+    # The four below are not ONNX operators: those of transformers whose products are quantised or whose attention is a difference.
+    ONNXSchema("SkipRMSNormalization", 1,
+               [ONNXParameter("X", "T"), ONNXParameter("Scale", "T"), ONNXParameter("skip", "T", _O)],
+               [ONNXParameter("Y", "T", _O), ONNXParameter("Sum", "T", _O), ONNXParameter("Q", "Q", _O), ONNXParameter("q_scale", "U", _O)],
+               [ONNXAttribute("axis", _A.Int, -1), ONNXAttribute("epsilon", _A.Float, 1e-5)],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("Q", [dace.int8]), ONNXTypeConstraint("U", [dace.float32])],
+               "Sum = X + skip; Y = Sum / sqrt(mean(Sum^2) + epsilon) * Scale over the trailing dimensions from `axis` on; Q = round(Y / q_scale) "
+               "with q_scale = max |Y| / 127 of each row. Any of the outputs may be left out, Q and q_scale together. A row with a value that is "
+               "not finite has a q_scale that is not a number."),
+    ONNXSchema("QuantizedLinear", 1,
+               [ONNXParameter("X", "Q"), ONNXParameter("W", "Q"), ONNXParameter("x_scale", "U"), ONNXParameter("w_scale", "U"),
+                ONNXParameter("B", "T", _O), ONNXParameter("residual", "T", _O)],
+               [ONNXParameter("Y", "T")],
+               [ONNXAttribute("activation", _A.String, "none"), ONNXAttribute("to", _A.Int, 1)],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("Q", [dace.int8]), ONNXTypeConstraint("U", [dace.float32])],
+               "Y = activation(x_scale * w_scale * (X W^T) + B) + residual: rows X [..., K], weights W [N, K], a scale for each row (or one) and "
+               "for each column (or one); activation `none`, `relu`, `gelu` (with erf) or `silu`; `to` is Y's element type."),
+    ONNXSchema("RotaryPositions", 1,
+               [ONNXParameter("Q", "T"), ONNXParameter("positions", "I"), ONNXParameter("frequencies", "U"), ONNXParameter("K", "T", _O)],
+               [ONNXParameter("Q_out", "T"), ONNXParameter("K_out", "T", _O)],
+               [ONNXAttribute("sections", _A.Ints), ONNXAttribute("interleaved", _A.Int, 0)],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("I", [dace.int64, dace.int32]), ONNXTypeConstraint("U", [dace.float32])],
+               "Pair i of each head of Q [B, S, H, D] (and K) turned by positions[axis, b, s] * frequencies[i]; `sections` says how many pairs, in "
+               "order, belong to each axis (all to the first if it is left out). Pairs are i and i + R / 2 of the first R = 2 len(frequencies) "
+               "values, neighbours if `interleaved`; values from R on are copied."),
+    ONNXSchema("DifferentialAttention", 1,
+               [ONNXParameter("Q", "T"), ONNXParameter("K", "T"), ONNXParameter("V", "T"), ONNXParameter("lambda_q1", "U"),
+                ONNXParameter("lambda_k1", "U"), ONNXParameter("lambda_q2", "U"), ONNXParameter("lambda_k2", "U"),
+                ONNXParameter("lengths", "I", _O)],
+               [ONNXParameter("O", "T")],
+               [ONNXAttribute("lambda_init", _A.Float, 0.8), ONNXAttribute("scale", _A.Float), ONNXAttribute("causal", _A.Int, 0)],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("U", [dace.float32]), ONNXTypeConstraint("I", [dace.int32])],
+               "O = (softmax(scale Q1 K1^T) - l softmax(scale Q2 K2^T)) V with l = exp(q1 . k1) - exp(q2 . k2) + lambda_init; Q [B, Sq, 2 H, d] and "
+               "K [B, Sk, 2 G, d] hold the two maps of a head next to each other, V is [B, Sk, G, 2 d], O [B, Sq, H, 2 d]; H / G heads "
+               "share keys and values. Keys from lengths[b] on do not exist; if `causal`, query i sees the keys up to i + lengths[b] - Sq. A row "
+               "without keys is 0. `scale` is 1 / sqrt(d) if it is left out."),
     # Pad only ever runs folded into the Conv that reads it (transformation/fusion.py, the reference's PadConvFusion)
     ONNXSchema("Pad", 11,
                [ONNXParameter("data", "T"), ONNXParameter("pads", "tensor(int64)"), ONNXParameter("constant_value", "T", _O)],

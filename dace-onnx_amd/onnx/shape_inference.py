@@ -61,6 +61,22 @@ def _infer_node(node, shapes, types, constants):
         return [(ins[0], tys[0])]
     if op == "LayerNormalization":
         return [(ins[0], tys[0])]
+    if op == "SkipRMSNormalization":
+        axis = a.get("axis", -1)
+        if not -len(ins[0]) <= axis < len(ins[0]):
+            raise ShapeInferenceError(f"{op} '{node.name}': axis {axis} of a rank-{len(ins[0])} input")
+        return [(ins[0], tys[0]), (ins[0], tys[0]), (ins[0], TensorProto.INT8), (tuple(ins[0][:axis % len(ins[0])]), TensorProto.FLOAT)]
+    if op == "QuantizedLinear":
+        if len(ins[0]) < 1 or len(ins[1]) != 2 or ins[0][-1] != ins[1][1]:
+            raise ShapeInferenceError(f"{op} '{node.name}': rows of {ins[0]} and weights of {ins[1]} (expected [N, K])")
+        return [(tuple(ins[0][:-1]) + (ins[1][0], ), int(a.get("to", TensorProto.FLOAT)))]
+    if op == "RotaryPositions":
+        return [(ins[0], tys[0])] + ([(ins[3], tys[3])] if len(ins) > 3 and ins[3] is not None else [])
+    if op == "DifferentialAttention":
+        Q, V = ins[0], ins[2]
+        if len(Q) != 4 or len(V) != 4 or Q[2] % 2:
+            raise ShapeInferenceError(f"{op} '{node.name}': queries of {Q} and values of {V} (expected [B, S, 2 H, d] and [B, S, H, 2 d])")
+        return [((Q[0], Q[1], Q[2] // 2, V[3]), tys[0])]
     if op == "MatMul" or op == "MatMulInteger":
         A, B = ins[0], ins[1]
         if len(A) < 2 or len(B) < 2:
@@ -211,6 +227,8 @@ def infer_shapes(model: ModelProto) -> ModelProto:
     for node in g.node:
         results = _infer_node(node, shapes, types, constants)
         for out_name, (shape, ty) in zip(node.output, results):
+            if out_name == "":
+                continue   # omitted optional output
             if out_name in shapes and tuple(shapes[out_name]) != tuple(shape):
                 raise ShapeInferenceError(
                     f"{node.op_type} '{node.name}': inferred shape {shape} for '{out_name}' "

@@ -46,11 +46,11 @@ log = logging.getLogger(__name__)
 class typeclass:
     """Element type, the subset of ``dace.typeclass`` the ONNX path touches."""
 
-    def __init__(self, name: str, np_dtype, ctype: str):
+    def __init__(self, name: str, np_dtype, ctype: str, size=None):
         self.name = name
         self.type = np.dtype(np_dtype).type
-        self.np_dtype = np.dtype(np_dtype)
-        self.bytes = self.np_dtype.itemsize
+        self.np_dtype = np.dtype(np_dtype)   #: what its values are held in on the host
+        self.bytes = size or self.np_dtype.itemsize
         self.ctype = ctype
 
     @property
@@ -86,9 +86,10 @@ int16 = typeclass("int16", np.int16, "int16_t")
 int32 = typeclass("int32", np.int32, "int32_t")
 int64 = typeclass("int64", np.int64, "int64_t")
 bool_ = typeclass("bool_", np.bool_, "bool")
+bfloat16 = typeclass("bfloat16", np.float32, "uint16_t", 2)   # (numpy has no such type: float32 there)
 
-_ALL_TYPES = [float16, float32, float64, int8, uint8, int16, int32, int64, bool_]
-_BY_NP = {t.np_dtype: t for t in _ALL_TYPES}
+_BY_NP = {t.np_dtype: t for t in (float16, float32, float64, int8, uint8, int16, int32, int64, bool_)}
+_ALL_TYPES = [*_BY_NP.values(), bfloat16]
 
 
 def typeclass_of(dtype) -> typeclass:
@@ -104,6 +105,19 @@ def typeclass_of(dtype) -> typeclass:
     except ImportError:  # pragma: no cover
         pass
     return _BY_NP[np.dtype(dtype)]
+
+
+def to_numpy(tensor):
+    """The values of a tensor as a numpy array, those of bfloat16 in float32."""
+    import torch
+    tensor = tensor.detach()
+    return (tensor.float() if tensor.dtype == torch.bfloat16 else tensor).cpu().numpy()
+
+
+def from_numpy(values, dtype: typeclass):
+    """A CPU tensor of the type ``dtype``, which shares the memory of ``values`` where it can."""
+    import torch
+    return torch.from_numpy(np.asarray(values, order="C")).to(dtype.as_torch())
 
 
 class StorageType:
@@ -982,7 +996,7 @@ class CompiledSDFG:
                     raise TypeError(f"argument '{name}': expected shape {desc.shape}, got {a.shape}")
                 if typeclass_of(a.dtype) != desc.dtype:
                     a = a.astype(desc.dtype.np_dtype)  # python scalars / default float64
-                d = torch.from_numpy(np.ascontiguousarray(a)).to(self.device)
+                d = from_numpy(a, desc.dtype).to(self.device)
                 if name in self._written and isinstance(v, np.ndarray):
                     staged_back.append((v, d))
                 env[name] = d
@@ -1004,12 +1018,12 @@ class CompiledSDFG:
             self._program.run(key, torch.cuda.current_stream(self.device).cuda_stream)
         for host, dev in staged_back:
             if isinstance(host, np.ndarray):
-                host[...] = dev.cpu().numpy()
+                host[...] = to_numpy(dev)
             else:
                 host.copy_(dev)
         if self._returned:
             any_torch = any(isinstance(v, torch.Tensor) for v in kwargs.values())
-            outs = [env[n] if any_torch else env[n].cpu().numpy() for n in self._returned]
+            outs = [env[n] if any_torch else to_numpy(env[n]) for n in self._returned]
             return outs[0] if len(outs) == 1 else tuple(outs)
         return None
 
@@ -1117,6 +1131,7 @@ class CompiledSDFG:
             lines.append(f"    {{  // {node.label}")
             for conn, key in conn_to_key.items():
                 ctype = desc_of[key].dtype.ctype if key in desc_of else "float"
+                ctype = "uint16_t" if ctype == "half" else ctype   # (the host's compiler has no such type)
                 value = "nullptr" if key in left_out else f"({ctype}*)__arrays[{index[key]}]"
                 lines.append(f"        {ctype}* _{conn} = {value};")
                 lines.append(f"        (void)_{conn};")

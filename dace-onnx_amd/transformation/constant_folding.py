@@ -103,7 +103,8 @@ def fold_constants(model: ModelProto) -> ModelProto:
     inputs (the module's parameters under ``keep_initializers_as_inputs``). The caller's model is not
     modified."""
     graph = model.graph
-    consts = {t.name: np.asarray(t.array).reshape(t.dims) for t in graph.initializer}
+    # (of bfloat16, which numpy does not have, nothing is computed here)
+    consts = {t.name: np.asarray(t.array).reshape(t.dims) for t in graph.initializer if t.data_type != proto.TensorProto.BFLOAT16}
     listed = {v.name for v in graph.input}
     static_shapes = {v.name: v.shape for v in list(graph.input) + list(graph.value_info) + list(graph.output)
                      if v.shape is not None and all(isinstance(d, int) for d in v.shape)}

@@ -47,7 +47,7 @@ import numpy as np
 
 from .. import _lib
 
-from ..sdfg import SDFG, SDFGState, AccessNode, Array, _contiguous_strides
+from ..sdfg import SDFG, SDFGState, AccessNode, Array, _contiguous_strides, to_numpy
 
 log = logging.getLogger(__name__)
 
@@ -93,7 +93,7 @@ def _constant_value(sdfg, name) -> typing.Optional[np.ndarray]:
     if model is None:
         return None
     w = model.weight_of(name)
-    return None if w is None else w.detach().cpu().numpy()
+    return None if w is None else to_numpy(w)
 
 
 def _reshape_strides(shape, strides, new_shape):

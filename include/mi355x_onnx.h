@@ -450,6 +450,60 @@ int mi355x_permute_b32(const void* X, void* Y, int ndim, const int64_t* shape,
 int mi355x_cast(const void* X, int from_type, void* Y, int to_type, int64_t n,
                 void* stream);
 
+/* ---- quantised and differential transformers ------------------------------------------------------------
+ * The reference has none of these nodes. Arrays of element type `type` (MI355X_TYPE_FLOAT, MI355X_TYPE_FLOAT16 or
+ * MI355X_TYPE_BFLOAT16) are computed with in float32 and rounded once, to the nearest; all arrays are C-contiguous, at
+ * any address of their element type. */
+#define MI355X_TYPE_FLOAT16 10
+#define MI355X_TYPE_BFLOAT16 16
+
+/* s = X + skip;  Y = s / sqrt(mean(s^2) + epsilon) * gain;  Q = round(Y / q_scale), q_scale = max |Y| / 127 of the row.
+ * X, skip, Y, Sum (which receives s) are [rows, cols], gain is [cols]. skip may be NULL, as may Y, Sum, and Q with
+ * q_scale ([rows], float32), but not all of them. Y and Q come from s before it is rounded, Q from Y before it is. A row
+ * with a value that is not finite has a q_scale that is not a number and 0 in Q; a row of zeros has both 0.
+ * Sum or Y may be X or skip itself in rows of up to 16384 (float32) or 32768 elements. */
+int mi355x_skip_rms_norm(const void* X, const void* skip, const void* gain, void* Y, void* Sum, int8_t* Q,
+                         float* q_scale, int64_t rows, int64_t cols, int type, float epsilon, void* stream);
+
+/* Y = act(x_scale[m] * w_scale[n] * sum_k X[m,k] W[n,k] + bias[n]) + residual[m,n]; X [M,K] and W [N,K] int8, K below
+ * 2^17 (the sums are exact in int32). x_scale_count is 1 or M, w_scale_count 1 or N. bias [N], residual and Y [M,N] are of
+ * element type `type`; bias and residual may be NULL, residual may be Y itself. */
+#define MI355X_ACT_NONE 0
+#define MI355X_ACT_RELU 1
+#define MI355X_ACT_GELU 2 /* 0.5 v (1 + erf(v / sqrt(2))) */
+#define MI355X_ACT_SILU 3 /* v / (1 + exp(-v)) */
+int mi355x_quantized_linear(const int8_t* X, const int8_t* W, const float* x_scale, const float* w_scale,
+                            const void* bias, const void* residual, void* Y, int64_t M, int64_t N, int64_t K,
+                            int64_t x_scale_count, int64_t w_scale_count, int activation, int type, void* stream);
+
+/* Pair i of every head turned by positions[axis, token] * frequencies[i]: Q [tokens, heads, size] to Q_out and, in the
+ * same launch, K [tokens, kv_heads, size] to K_out (either count may be 0). `rotated` values of a head are turned: pairs
+ * are i and i + rotated / 2, neighbours 2 i and 2 i + 1 if `interleaved`; the others are copied. positions
+ * [axes, tokens] are integers of position_bytes (4 or 8), frequencies [rotated / 2] float32; sections[axes] (host
+ * memory) says how many pairs, in order, belong to each axis. axes <= 8. Q_out may be Q itself, K_out may be K. */
+int mi355x_rotary_positions(const void* Q, const void* K, const void* positions, const float* frequencies, void* Q_out,
+                            void* K_out, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t rotated,
+                            int64_t axes, const int64_t* sections, int interleaved, int position_bytes, int type,
+                            void* stream);
+
+/* O = (softmax(scale Q1 K1^T) - l softmax(scale Q2 K2^T)) V,  l = exp(q1 . k1) - exp(q2 . k2) + lambda_init.
+ * Q [batch, Sq, 2 heads, size] and K [batch, Sk, 2 groups, size] hold the two maps of a head next to each other, V is
+ * [batch, Sk, groups, 2 size], O [batch, Sq, heads, 2 size]; head h reads keys and values h / (heads / groups). size is
+ * 32, 64 or 128; the lambda_* are [vector] float32, scale is positive.
+ * lengths [batch] (device memory, NULL: Sk): keys from there on do not exist and are not read; numbers outside 0 to Sk
+ * count as the nearer of the two. If `causal`, query i sees the keys up to i + length - Sq. A row that sees no key is 0.
+ * `splits` workgroups share the keys of a row, 1 to 256; mi355x_differential_attention_splits says how many pay. From 2 on
+ * `scratch` has room for splits * batch * Sq * heads * (4 size + 4) floats, 16-byte aligned, and belongs to the
+ * call until it is done. Of values that a row does not see, but another row of the entry does, an infinity or NaN
+ * may still reach it; lengths keep them out. */
+int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups,
+                                             int64_t size, int type);
+int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1,
+                                  const float* lambda_k1, const float* lambda_q2, const float* lambda_k2,
+                                  const int32_t* lengths, void* O, float* scratch, int64_t batch, int64_t Sq, int64_t Sk,
+                                  int64_t heads, int64_t groups, int64_t size, int64_t vector, float lambda_init,
+                                  float scale, int causal, int64_t splits, int type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
