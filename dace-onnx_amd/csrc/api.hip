@@ -75,6 +75,7 @@ static void parse_tuning(Tuning& t) {
     t.attn_waves = env_int("MI355X_ATTN_WAVES", 0);
     t.attn_split = env_int("MI355X_ATTN_SPLIT", -1);
     t.attn_few = env_int("MI355X_ATTN_FEW", -1);
+    t.qlin_form = env_int("MI355X_QLIN_FORM", -1);
 }
 
 Tuning tuning() {

@@ -98,6 +98,104 @@ __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
     qlin_store<T, ACT, 4>(p, m0 + 16 * wave + l16, n0 + 4 * lq, s4);
 }
 
+// 16 bytes to a lane from global memory, base + the lane's offset, into LDS at lds + 16 lane; base and lds are the same for the wave, all 16-byte aligned.
+// Written as assembly because the compiler waits for every builtin transfer before the next LDS read.
+__device__ __forceinline__ void qlin_to_lds(const int8_t* base, uint32_t offset, uint32_t lds) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint64_t uniform = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory");
+}
+
+// Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, two stages. A row's 128 bytes of a step are eight
+// pieces of 16; piece c of row r lies at c ^ (r % 8), so that an operand read (one piece of 32 rows) meets every bank equally often. DIRECT (rows at
+// 16-byte boundaries): whole steps go from memory to LDS without registers, a step ahead; otherwise, and for a last part of a step, through registers.
+template <class T, int ACT, int WM, int WN, int TM, int TN, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int group_m) {
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 128, STAGE = (BM + BN) * BK;
+    constexpr int PER_WAVE = (BM + BN) / 8 / NW;   // transfers of 1 KB, eight rows, to a wave and step
+    static_assert((BM + BN) / 8 % NW == 0 && BM % 8 == 0, "whole transfers");
+    __shared__ __attribute__((aligned(1024))) int8_t lds[2 * STAGE];
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int l32 = lane % 32, h = lane / 32, wm = wave % WM, wn = wave / WM;
+    int64_t tm, tn;
+    tile_coords(xcd_remap(blockIdx.x, p.tiles_m * p.tiles_n), p.tiles_m, p.tiles_n, group_m, tm, tn);
+    const int64_t m0 = tm * BM, n0 = tn * BN;
+
+    // rows past the end are the last row again; what they give is not stored
+    const int8_t* base[PER_WAVE];
+    uint32_t offset[PER_WAVE];
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i) {
+        const int first = 8 * (wave + i * NW);
+        const bool is_x = first < BM;
+        const int64_t r0 = is_x ? m0 : n0, count = is_x ? p.M : p.N, r = (is_x ? first : first - BM) + lane / 8;
+        base[i] = (is_x ? p.X : p.W) + r0 * p.K;
+        offset[i] = (uint32_t)((r0 + r < count ? r : count - 1 - r0) * p.K) + 16u * (uint32_t)((lane % 8) ^ (lane / 8));
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+    const int64_t whole = DIRECT ? p.K / BK : 0, steps = (p.K + BK - 1) / BK;
+    i32x4 held[DIRECT ? 1 : PER_WAVE];
+    auto fetch = [&](int64_t step, auto&& to) __attribute__((always_inline)) {   // by registers
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i)
+            to(i, row_bytes(base[i] + step * BK + offset[i], p.K - step * BK - 16 * ((lane % 8) ^ (lane / 8))));
+    };
+    auto put = [&](int64_t step, int i, const i32x4& v) __attribute__((always_inline)) {
+        *reinterpret_cast<i32x4*>(lds + (step % 2) * STAGE + (wave + i * NW) * 1024 + 16 * lane) = v;
+    };
+    auto load = [&](int64_t step) __attribute__((always_inline)) {
+        if (step < whole) {
+#pragma unroll
+            for (int i = 0; i < PER_WAVE; ++i) qlin_to_lds(base[i] + step * BK, offset[i], lds0 + (uint32_t)((step % 2) * STAGE + (wave + i * NW) * 1024));
+        } else if constexpr (DIRECT) {
+            fetch(step, [&](int i, const i32x4& v) __attribute__((always_inline)) { put(step, i, v); });
+        } else {
+            fetch(step, [&](int i, const i32x4& v) __attribute__((always_inline)) { held[i] = v; });
+        }
+    };
+
+    i32x16 acc[TM][TN] = {};
+    auto multiply = [&](int64_t step) __attribute__((always_inline)) {
+        const int8_t* x = lds + (step % 2) * STAGE + (wm * 32 * TM + l32) * BK;
+        const int8_t* w = lds + (step % 2) * STAGE + (BM + wn * 32 * TN + l32) * BK;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const int piece = 16 * ((2 * ks + h) ^ (l32 % 8));
+            i32x4 fx[TM], fw[TN];
+#pragma unroll
+            for (int t = 0; t < TN; ++t) fw[t] = *reinterpret_cast<const i32x4*>(w + 32 * t * BK + piece);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) fx[t] = *reinterpret_cast<const i32x4*>(x + 32 * t * BK + piece);
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+#pragma unroll
+                for (int u = 0; u < TN; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[u], fx[t], acc[t][u], 0, 0, 0);
+        }
+    };
+    if (steps > 0) {
+        load(0);
+        for (int64_t step = 0; step < steps; ++step) {
+            if constexpr (!DIRECT) {
+#pragma unroll
+                for (int i = 0; i < PER_WAVE; ++i) put(step, i, held[i]);
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the step is in LDS, and nobody reads the other stage any more
+            __syncthreads();
+            if (step + 1 < steps) load(step + 1);
+            multiply(step);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+        for (int u = 0; u < TN; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int s4[4] = {acc[t][u][4 * g], acc[t][u][4 * g + 1], acc[t][u][4 * g + 2], acc[t][u][4 * g + 3]};
+                qlin_store<T, ACT, 4>(p, m0 + (wm * TM + t) * 32 + l32, n0 + (wn * TN + u) * 32 + 8 * g + 4 * h, s4);
+            }
+}
+
 template <class T, int ACT>
 static void launch_qlin(QLinArgs p, hipStream_t st) {
     auto direct = [&](auto mt) {
@@ -106,7 +204,23 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
         p.tiles_m = ceil_div(p.M, (int64_t)(16 * MT));
         hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(512), 0, st, p);
     };
-    if (p.M <= 16) direct(Int<1>{});
+    const bool aligned = p.K % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.W)) & 15) == 0;
+    auto tile = [&](auto wm, auto wn, auto tm, auto tn, int per_cu) {
+        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, TM = decltype(tm)::value, TN = decltype(tn)::value;
+        p.tiles_m = ceil_div(p.M, (int64_t)(32 * TM * WM));
+        p.tiles_n = ceil_div(p.N, (int64_t)(32 * TN * WN));
+        const int64_t nwg = p.tiles_m * p.tiles_n;
+        const int group_m = choose_group_m(p.tiles_m, ceil_div(nwg, (int64_t)NUM_XCD), (int64_t)per_cu * 32, 32 * TM * WM, 32 * TN * WN, p.K);
+        const dim3 grid((unsigned)nwg), block(64 * WM * WN);
+        if (aligned) hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, true>), grid, block, 0, st, p, group_m);
+        else hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, false>), grid, block, 0, st, p, group_m);
+    };
+    const int form = tuning().qlin_form;
+    const int pick = form >= 0 ? form : p.M <= 64 ? 0 : p.M * p.N <= (int64_t)64 * 64 * 512 ? 1 : p.M * p.N <= (int64_t)128 * 128 * 512 ? 2 : 3;
+    if (pick == 3) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, 1);
+    else if (pick == 2) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, 2);
+    else if (pick == 1) tile(Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}, 4);
+    else if (p.M <= 16) direct(Int<1>{});
     else if (p.M <= 32) direct(Int<2>{});
     else direct(Int<4>{});
 }

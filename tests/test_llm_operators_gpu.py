@@ -149,6 +149,18 @@ def test_linear(m, n, k, dtype):
         within(y, expected, linear_bound(size, expected, dtype))
 
 
+@pytest.mark.parametrize("form", [0, 1, 2, 3])
+@pytest.mark.parametrize("m, n, k", [(1, 1, 1), (63, 65, 16), (65, 63, 127), (129, 140, 128), (300, 270, 144), (257, 129, 272), (64, 513, 1009), (515, 40, 640), (7, 9, 0)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_linear_by_every_kernel(form, m, n, k, dtype, tuning):
+    x, w, xs, ws = eight(1, m, k), eight(2, n, k), normal(3, m).abs() / 74 + 1e-3, normal(4, n).abs() / 74 / max(k, 1) ** 0.5
+    bias, residual = normal(5, n, dtype=dtype), normal(6, m, n, dtype=dtype)
+    tuning(MI355X_QLIN_FORM=form)
+    y, = R.call("QuantizedLinear", [("x", x), ("w", w), ("xs", xs), ("ws", ws), ("b", bias), ("r", residual)], [("y", dtype, (m, n))], activation="gelu", to=R.ELEMENT[dtype])
+    expected, size = R.quantized_linear(x, w, xs, ws, bias, residual, "gelu")
+    within(y, expected, linear_bound(size, expected, dtype))
+
+
 def test_linear_with_one_scale_and_more_dimensions():
     x, w = eight(1, 2, 3, 70), eight(2, 50, 70)
     y, = R.call("QuantizedLinear", [("x", x), ("w", w), ("xs", normal(3, 1).abs()), ("ws", normal(4, 1).abs())], [("y", F32, (2, 3, 50))])
