@@ -51,12 +51,14 @@ __device__ __forceinline__ int64_t diff_length(const DiffArgs& p, int64_t b) {
     return n < 0 ? 0 : n > p.Sk ? p.Sk : n;
 }
 
-// A tile's geometry: KT keys of 2 D values (both maps' keys, or the values), in pieces of 16 bytes of which piece c of key k lies at c ^ (k & 7).
+// A tile's geometry: KT keys of 2 D values (both maps' keys, or the values), in pieces of 16 bytes of which piece c of key k lies at c ^ place(k): a bijection
+// of 16 keys (of one piece, as scores read them), and of four keys onto different quarters of the banks (the transposing reads).
 template <class T, int D>
 struct DiffTile {
-    static constexpr int KT = 32, E = 16 / sizeof(T), PIECES = 2 * D / E;   // (16 at least)
+    static constexpr int KT = 32, E = 16 / sizeof(T), PIECES = 2 * D / E;   // (8 at least)
     static constexpr int BYTES = KT * 2 * D * (int)sizeof(T);
-    static __device__ __forceinline__ int at(int key, int piece) { return (key * PIECES + (piece ^ (key & 7))) * E; }   // in values
+    static __device__ __forceinline__ int place(int key) { return PIECES == 8 ? (key >> 1 & 1) << 2 | (key >> 2 & 3) : (key & 3) << 2 | (key >> 2 & 3); }
+    static __device__ __forceinline__ int at(int key, int piece) { return (key * PIECES + (piece ^ place(key))) * E; }   // in values
 };
 
 // One map's operand of Q: D / (2 E) pieces of 16 bytes to a lane.

@@ -26,28 +26,39 @@ __device__ __forceinline__ float activated(float v) {
     return v;
 }
 
-// E results next to each other in row m, from column n on
-template <class T, int ACT, int E>
-__device__ __forceinline__ void qlin_store(const QLinArgs& p, int64_t m, int64_t n, const int (&acc)[E]) {
-    if (m >= p.M || n >= p.N) return;
-    const int64_t left = p.N - n;
-    const float xs = p.xs[m * p.xs_step];
-    float v[E], b[E], r[E];
+// The epilogue of R rows that a lane has four results next to each other of, in each of G groups: what it reads first, all at once, because stores hold
+// back reads that come after them (the residual may be Y itself). row(r), column(g): where; acc(r, g, e): the sums.
+template <class T, int ACT, int R, int G, class Row, class Column, class Sum>
+__device__ __forceinline__ void qlin_store(const QLinArgs& p, Row&& row, Column&& column, Sum&& acc) {
+    float xs[R], ws[G][4], b[G][4], res[R][G][4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = (float)acc[e] * xs * p.ws[p.ws_step ? (e < left ? n + e : n) : 0];
-    if (p.bias) {
-        load_values(b, static_cast<const T*>(p.bias) + n, left);
+    for (int r = 0; r < R; ++r) xs[r] = p.xs[(row(r) < p.M ? row(r) : p.M - 1) * p.xs_step];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] += b[e];
+    for (int g = 0; g < G; ++g) {
+        if (p.ws_step) load_values(ws[g], p.ws + column(g), p.N - column(g));
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ws[g][e] = p.ws[0];
+        if (p.bias) load_values(b[g], static_cast<const T*>(p.bias) + column(g), p.N - column(g));
+        if (p.residual) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) load_values(res[r][g], static_cast<const T*>(p.residual) + row(r) * p.N + column(g), row(r) < p.M ? p.N - column(g) : 0);
+        }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = activated<ACT>(v[e]);
-    if (p.residual) {
-        load_values(r, static_cast<const T*>(p.residual) + m * p.N + n, left);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] += r[e];
-    }
-    store_values(static_cast<T*>(p.Y) + m * p.N + n, v, left);
+        for (int g = 0; g < G; ++g) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = (float)acc(r, g, e) * xs[r] * ws[g][e];
+                if (p.bias) v[e] += b[g][e];
+                v[e] = activated<ACT>(v[e]);
+                if (p.residual) v[e] += res[r][g][e];
+            }
+            store_values(static_cast<T*>(p.Y) + row(r) * p.N + column(g), v, row(r) < p.M ? p.N - column(g) : 0);
+        }
 }
 
 // the 16 bytes from p on of which `left` belong to the row: the others as 0
@@ -94,8 +105,7 @@ __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
     i32x4 sum = part[0][wave][lane];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) sum += part[w][wave][lane];
-    const int s4[4] = {sum.x, sum.y, sum.z, sum.w};
-    qlin_store<T, ACT, 4>(p, m0 + 16 * wave + l16, n0 + 4 * lq, s4);
+    qlin_store<T, ACT, 1, 1>(p, [&](int) { return m0 + 16 * wave + l16; }, [&](int) { return n0 + 4 * lq; }, [&](int, int, int e) { return sum[e]; });
 }
 
 // 16 bytes to a lane from global memory, base + the lane's offset, into LDS at lds + 16 lane; base and lds are the same for the wave, all 16-byte aligned.
@@ -107,7 +117,8 @@ __device__ __forceinline__ void qlin_to_lds(const int8_t* base, uint32_t offset,
 }
 
 // Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, two stages. A row's 128 bytes of a step are eight
-// pieces of 16; piece c of row r lies at c ^ (r % 8), so that an operand read (one piece of 32 rows) meets every bank equally often. DIRECT (rows at
+// pieces of 16; piece c of row r lies at c ^ (r / 2 % 8), so that the 16 rows whose
+// pieces are read at a time lie in 16 different places of the 256 bytes that the banks hold. DIRECT (rows at
 // 16-byte boundaries): whole steps go from memory to LDS without registers, a step ahead; otherwise, and for a last part of a step, through registers.
 template <class T, int ACT, int WM, int WN, int TM, int TN, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int group_m) {
@@ -124,13 +135,15 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     // rows past the end are the last row again; what they give is not stored
     const int8_t* base[PER_WAVE];
     uint32_t offset[PER_WAVE];
+    int piece[PER_WAVE];
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i) {
         const int first = 8 * (wave + i * NW);
         const bool is_x = first < BM;
         const int64_t r0 = is_x ? m0 : n0, count = is_x ? p.M : p.N, r = (is_x ? first : first - BM) + lane / 8;
         base[i] = (is_x ? p.X : p.W) + r0 * p.K;
-        offset[i] = (uint32_t)((r0 + r < count ? r : count - 1 - r0) * p.K) + 16u * (uint32_t)((lane % 8) ^ (lane / 8));
+        piece[i] = (lane % 8) ^ (4 * (wave + i * NW) + lane / 16) % 8;
+        offset[i] = (uint32_t)((r0 + r < count ? r : count - 1 - r0) * p.K) + 16u * (uint32_t)piece[i];
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
     const int64_t whole = DIRECT ? p.K / BK : 0, steps = (p.K + BK - 1) / BK;
@@ -138,7 +151,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     auto fetch = [&](int64_t step, auto&& to) __attribute__((always_inline)) {   // by registers
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i)
-            to(i, row_bytes(base[i] + step * BK + offset[i], p.K - step * BK - 16 * ((lane % 8) ^ (lane / 8))));
+            to(i, row_bytes(base[i] + step * BK + offset[i], p.K - step * BK - 16 * piece[i]));
     };
     auto put = [&](int64_t step, int i, const i32x4& v) __attribute__((always_inline)) {
         *reinterpret_cast<i32x4*>(lds + (step % 2) * STAGE + (wave + i * NW) * 1024 + 16 * lane) = v;
@@ -158,18 +171,24 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     auto multiply = [&](int64_t step) __attribute__((always_inline)) {
         const int8_t* x = lds + (step % 2) * STAGE + (wm * 32 * TM + l32) * BK;
         const int8_t* w = lds + (step % 2) * STAGE + (BM + wn * 32 * TN + l32) * BK;
+        i32x4 fx[2][TM], fw[2][TN];
+        auto read = [&](int set, int ks) __attribute__((always_inline)) {
+            const int piece = 16 * ((2 * ks + h) ^ (l32 / 2 % 8));
+#pragma unroll
+            for (int t = 0; t < TN; ++t) fw[set][t] = *reinterpret_cast<const i32x4*>(w + 32 * t * BK + piece);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) fx[set][t] = *reinterpret_cast<const i32x4*>(x + 32 * t * BK + piece);
+        };
+        read(0, 0);
+        if (step + 1 < steps) load(step + 1);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-            const int piece = 16 * ((2 * ks + h) ^ (l32 % 8));
-            i32x4 fx[TM], fw[TN];
-#pragma unroll
-            for (int t = 0; t < TN; ++t) fw[t] = *reinterpret_cast<const i32x4*>(w + 32 * t * BK + piece);
-#pragma unroll
-            for (int t = 0; t < TM; ++t) fx[t] = *reinterpret_cast<const i32x4*>(x + 32 * t * BK + piece);
+            if (ks < 3) read((ks + 1) % 2, ks + 1);
 #pragma unroll
             for (int t = 0; t < TM; ++t)
 #pragma unroll
-                for (int u = 0; u < TN; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[u], fx[t], acc[t][u], 0, 0, 0);
+                for (int u = 0; u < TN; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[ks % 2][u], fx[ks % 2][t], acc[t][u], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (steps > 0) {
@@ -181,19 +200,58 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
             }
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the step is in LDS, and nobody reads the other stage any more
             __syncthreads();
-            if (step + 1 < steps) load(step + 1);
             multiply(step);
         }
     }
+    // The results leave by whole lines: a lane has four neighbours of one row, and of the next instruction's rows others; 32 rows at a time go through LDS, of which
+    // each wave has a share of its own, as floats (times the row's scale), and come back as rows. Stored as they lie, 16 bytes of each row at a time, a tile's
+    // results took 17 us.
+    constexpr int PIECES = 8 * TN, PER_STEP = WAVE / PIECES, COUNT = 32 / PER_STEP;   // pieces of 16 bytes in a row, rows to an instruction
+    constexpr int BATCH = COUNT < 8 ? COUNT : 8;
+    static_assert(NW * 32 * 32 * TN * 4 <= 2 * STAGE, "the waves' shares fit");
+    float* mine = reinterpret_cast<float*>(lds) + wave * 32 * 32 * TN;
+    auto at = [&](int row, int column) { return row * 32 * TN + 4 * (column / 4 ^ (TN == 1 ? row / 2 % 8 : row % 16)) + column % 4; };
+    const int c = 4 * (lane % PIECES);
+    const int64_t n = n0 + wn * 32 * TN + c, left = p.N - n;
+    float ws[4], bias[4] = {};
+    if (p.ws_step) load_values(ws, p.ws + n, left);
+    else ws[0] = ws[1] = ws[2] = ws[3] = p.ws[0];
+    if (p.bias) load_values(bias, static_cast<const T*>(p.bias) + n, left);
+    __syncthreads();   // nobody reads the stages any more
 #pragma unroll
-    for (int t = 0; t < TM; ++t)
+    for (int t = 0; t < TM; ++t) {
+        const int64_t m = m0 + (wm * TM + t) * 32;
+        const float xs = p.xs[(m + l32 < p.M ? m + l32 : p.M - 1) * p.xs_step];
 #pragma unroll
         for (int u = 0; u < TN; ++u)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int s4[4] = {acc[t][u][4 * g], acc[t][u][4 * g + 1], acc[t][u][4 * g + 2], acc[t][u][4 * g + 3]};
-                qlin_store<T, ACT, 4>(p, m0 + (wm * TM + t) * 32 + l32, n0 + (wn * TN + u) * 32 + 8 * g + 4 * h, s4);
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(mine + at(l32, 32 * u + 8 * g + 4 * h)) =
+                    f32x4{(float)acc[t][u][4 * g] * xs, (float)acc[t][u][4 * g + 1] * xs, (float)acc[t][u][4 * g + 2] * xs, (float)acc[t][u][4 * g + 3] * xs};
+#pragma unroll
+        for (int i0 = 0; i0 < COUNT; i0 += BATCH) {
+            float res[BATCH][4];
+            if (p.residual) {   // all at once: stores hold back reads that come after them, the residual may be Y itself
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int64_t r = m + (i0 + i) * PER_STEP + lane / PIECES;
+                    load_values(res[i], static_cast<const T*>(p.residual) + r * p.N + n, r < p.M ? left : 0);
+                }
             }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int row = (i0 + i) * PER_STEP + lane / PIECES;
+                const f32x4 sum = *reinterpret_cast<const f32x4*>(mine + at(row, c));
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = activated<ACT>(sum[e] * ws[e] + bias[e]);
+                    if (p.residual) v[e] += res[i][e];
+                }
+                store_values(static_cast<T*>(p.Y) + (m + row) * p.N + n, v, m + row < p.M ? left : 0);
+            }
+        }
+    }
 }
 
 template <class T, int ACT>
@@ -217,7 +275,10 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
     };
     const int form = tuning().qlin_form;
     const int pick = form >= 0 ? form : p.M <= 64 ? 0 : p.M * p.N <= (int64_t)64 * 64 * 512 ? 1 : p.M * p.N <= (int64_t)128 * 128 * 512 ? 2 : 3;
-    if (pick == 3) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, 1);
+    if (pick == 4) tile(Int<2>{}, Int<2>{}, Int<4>{}, Int<4>{}, 1);
+    else if (pick == 5) tile(Int<4>{}, Int<2>{}, Int<2>{}, Int<4>{}, 1);
+    else if (pick == 6) tile(Int<2>{}, Int<2>{}, Int<4>{}, Int<2>{}, 1);
+    else if (pick == 3) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, 1);
     else if (pick == 2) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, 2);
     else if (pick == 1) tile(Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}, 4);
     else if (p.M <= 16) direct(Int<1>{});
