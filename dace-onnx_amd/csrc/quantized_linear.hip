@@ -61,14 +61,24 @@ __device__ __forceinline__ void qlin_store(const QLinArgs& p, Row&& row, Column&
         }
 }
 
-// the 16 bytes from p on of which `left` belong to the row: the others as 0
-__device__ __forceinline__ i32x4 row_bytes(const int8_t* p, int64_t left) {
-    typedef i32x4 unaligned __attribute__((aligned(1)));
-    if (left >= 16) return *reinterpret_cast<const unaligned*>(p);
-    int8_t b[16];
+typedef i32x4 UnalignedBytes __attribute__((aligned(1)));
+
+// the 16 bytes from p on of which `left` belong to a row of K: the others as 0
+__device__ __forceinline__ i32x4 row_bytes(const int8_t* p, int64_t left, int64_t K) {
+    if (left >= 16) return *reinterpret_cast<const UnalignedBytes*>(p);
+    if (left <= 0) return i32x4{};
+    if (K < 16) {
+        int8_t b[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = i < left ? p[i] : (int8_t)0;
-    return __builtin_bit_cast(i32x4, b);
+        for (int i = 0; i < 16; ++i) b[i] = i < left ? p[i] : (int8_t)0;
+        return __builtin_bit_cast(i32x4, b);
+    }
+    // the row's last 16 bytes, moved down
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    u64x2 v = __builtin_bit_cast(u64x2, *reinterpret_cast<const UnalignedBytes*>(p - (16 - left)));
+    const int bits = 8 * (16 - (int)left);   // 8 to 120
+    v = bits >= 64 ? u64x2{v.y >> (bits - 64), 0} : u64x2{v.x >> bits | v.y << (64 - bits), v.y >> bits};
+    return __builtin_bit_cast(i32x4, v);
 }
 
 // Any shape and alignment, operands straight from memory. A workgroup has 16 columns and 16 MT rows of Y, its eight waves take turns at the
@@ -84,20 +94,24 @@ __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) x[t] = p.X + std::min(m0 + 16 * t + l16, p.M - 1) * p.K;
     i32x4 acc[MT] = {};
-    for (int64_t k = 128 * wave; k < p.K; k += 128 * WAVES) {
+    auto line = [&](int64_t k, auto&& bytes) __attribute__((always_inline)) {
         i32x4 a[2], b[2][MT];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int64_t at = k + 64 * s + 16 * lq;
-            a[s] = row_bytes(w + at, p.K - at);
+            a[s] = bytes(w + at, p.K - at);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) b[s][t] = row_bytes(x[t] + at, p.K - at);
+            for (int t = 0; t < MT; ++t) b[s][t] = bytes(x[t] + at, p.K - at);
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b[s][t], acc[t], 0, 0, 0);
-    }
+    };
+    int64_t k = 128 * wave;
+#pragma unroll 4
+    for (; k + 128 <= p.K; k += 128 * WAVES) line(k, [](const int8_t* at, int64_t) { return i32x4(*reinterpret_cast<const UnalignedBytes*>(at)); });
+    if (k < p.K) line(k, [&](const int8_t* at, int64_t left) { return row_bytes(at, left, p.K); });
 #pragma unroll
     for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
     __syncthreads();
@@ -116,16 +130,19 @@ __device__ __forceinline__ void qlin_to_lds(const int8_t* base, uint32_t offset,
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory");
 }
 
-// Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, two stages. A row's 128 bytes of a step are eight
+// Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, NS stages. A row's 128 bytes of a step are eight
 // pieces of 16; piece c of row r lies at c ^ (r / 2 % 8), so that the 16 rows whose
 // pieces are read at a time lie in 16 different places of the 256 bytes that the banks hold. DIRECT (rows at
-// 16-byte boundaries): whole steps go from memory to LDS without registers, a step ahead; otherwise, and for a last part of a step, through registers.
-template <class T, int ACT, int WM, int WN, int TM, int TN, bool DIRECT>
+// 16-byte boundaries): whole steps go from memory to LDS without registers, NS - 1 steps ahead; otherwise, two
+// steps ahead, and for a last part of a step, through registers.
+template <class T, int ACT, int WM, int WN, int TM, int TN, int NS, int BK, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int group_m) {
-    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 128, STAGE = (BM + BN) * BK;
-    constexpr int PER_WAVE = (BM + BN) / 8 / NW;   // transfers of 1 KB, eight rows, to a wave and step
-    static_assert((BM + BN) / 8 % NW == 0 && BM % 8 == 0, "whole transfers");
-    __shared__ __attribute__((aligned(1024))) int8_t lds[2 * STAGE];
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * BK;
+    constexpr int PPR = BK / 16, RPT = 64 / PPR;   // pieces of a row, rows of a transfer (1 KB)
+    constexpr int PER_WAVE = (BM + BN) / RPT / NW;  // transfers to a wave and step
+    static_assert((BM + BN) / RPT % NW == 0 && BM % RPT == 0 && (PPR == 8 || PPR == 16), "whole transfers");
+    auto place = [](int row) { return PPR == 8 ? row / 2 % 8 : row % 16; };
+    __shared__ __attribute__((aligned(1024))) int8_t lds[NS * STAGE];
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int l32 = lane % 32, h = lane / 32, wm = wave % WM, wn = wave / WM;
     int64_t tm, tn;
@@ -138,52 +155,57 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     int piece[PER_WAVE];
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i) {
-        const int first = 8 * (wave + i * NW);
+        const int first = RPT * (wave + i * NW);
         const bool is_x = first < BM;
-        const int64_t r0 = is_x ? m0 : n0, count = is_x ? p.M : p.N, r = (is_x ? first : first - BM) + lane / 8;
+        const int64_t r0 = is_x ? m0 : n0, count = is_x ? p.M : p.N, r = (is_x ? first : first - BM) + lane / PPR;
         base[i] = (is_x ? p.X : p.W) + r0 * p.K;
-        piece[i] = (lane % 8) ^ (4 * (wave + i * NW) + lane / 16) % 8;
+        piece[i] = (lane % PPR) ^ place(first + lane / PPR);
         offset[i] = (uint32_t)((r0 + r < count ? r : count - 1 - r0) * p.K) + 16u * (uint32_t)piece[i];
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
     const int64_t whole = DIRECT ? p.K / BK : 0, steps = (p.K + BK - 1) / BK;
-    i32x4 held[DIRECT ? 1 : PER_WAVE];
-    auto fetch = [&](int64_t step, auto&& to) __attribute__((always_inline)) {   // by registers
+    typedef i32x4 Held[PER_WAVE];
+    auto fetch = [&](int64_t step, Held& to) __attribute__((always_inline)) {   // by registers
+        if ((step + 1) * BK <= p.K) {
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i)
-            to(i, row_bytes(base[i] + step * BK + offset[i], p.K - step * BK - 16 * piece[i]));
+            for (int i = 0; i < PER_WAVE; ++i) to[i] = *reinterpret_cast<const UnalignedBytes*>(base[i] + step * BK + offset[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER_WAVE; ++i) to[i] = row_bytes(base[i] + step * BK + offset[i], p.K - step * BK - 16 * piece[i], p.K);
+        }
     };
-    auto put = [&](int64_t step, int i, const i32x4& v) __attribute__((always_inline)) {
-        *reinterpret_cast<i32x4*>(lds + (step % 2) * STAGE + (wave + i * NW) * 1024 + 16 * lane) = v;
+    auto put = [&](int stage, const Held& v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i) *reinterpret_cast<i32x4*>(lds + stage * STAGE + (wave + i * NW) * 1024 + 16 * lane) = v[i];
     };
-    auto load = [&](int64_t step) __attribute__((always_inline)) {
+    auto load = [&](int64_t step, int stage) __attribute__((always_inline)) {
         if (step < whole) {
 #pragma unroll
-            for (int i = 0; i < PER_WAVE; ++i) qlin_to_lds(base[i] + step * BK, offset[i], lds0 + (uint32_t)((step % 2) * STAGE + (wave + i * NW) * 1024));
-        } else if constexpr (DIRECT) {
-            fetch(step, [&](int i, const i32x4& v) __attribute__((always_inline)) { put(step, i, v); });
-        } else {
-            fetch(step, [&](int i, const i32x4& v) __attribute__((always_inline)) { held[i] = v; });
+            for (int i = 0; i < PER_WAVE; ++i) qlin_to_lds(base[i] + step * BK, offset[i], lds0 + (uint32_t)(stage * STAGE + (wave + i * NW) * 1024));
+        } else if (step < steps) {
+            Held part;
+            fetch(step, part);
+            put(stage, part);
         }
     };
 
     i32x16 acc[TM][TN] = {};
-    auto multiply = [&](int64_t step) __attribute__((always_inline)) {
-        const int8_t* x = lds + (step % 2) * STAGE + (wm * 32 * TM + l32) * BK;
-        const int8_t* w = lds + (step % 2) * STAGE + (BM + wn * 32 * TN + l32) * BK;
+    auto multiply = [&](int stage, auto&& meanwhile) __attribute__((always_inline)) {
+        const int8_t* x = lds + stage * STAGE + (wm * 32 * TM + l32) * BK;
+        const int8_t* w = lds + stage * STAGE + (BM + wn * 32 * TN + l32) * BK;
         i32x4 fx[2][TM], fw[2][TN];
         auto read = [&](int set, int ks) __attribute__((always_inline)) {
-            const int piece = 16 * ((2 * ks + h) ^ (l32 / 2 % 8));
+            const int piece = 16 * ((2 * ks + h) ^ place(l32));
 #pragma unroll
             for (int t = 0; t < TN; ++t) fw[set][t] = *reinterpret_cast<const i32x4*>(w + 32 * t * BK + piece);
 #pragma unroll
             for (int t = 0; t < TM; ++t) fx[set][t] = *reinterpret_cast<const i32x4*>(x + 32 * t * BK + piece);
         };
         read(0, 0);
-        if (step + 1 < steps) load(step + 1);
+        meanwhile();
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            if (ks < 3) read((ks + 1) % 2, ks + 1);
+        for (int ks = 0; ks < BK / 32; ++ks) {
+            if (ks + 1 < BK / 32) read((ks + 1) % 2, ks + 1);
 #pragma unroll
             for (int t = 0; t < TM; ++t)
 #pragma unroll
@@ -191,16 +213,32 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (steps > 0) {
-        load(0);
-        for (int64_t step = 0; step < steps; ++step) {
-            if constexpr (!DIRECT) {
+    if constexpr (DIRECT) {
 #pragma unroll
-                for (int i = 0; i < PER_WAVE; ++i) put(step, i, held[i]);
-            }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the step is in LDS, and nobody reads the other stage any more
+        for (int i = 0; i < NS - 1; ++i) load(i, i);
+        int stage = 0;
+        for (int64_t step = 0; step < steps; ++step) {
+            // The step is in LDS, and nobody reads any more what the transfer below writes. Transfers complete in order: those of the NS - 2 steps
+            // behind this one may be on their way, if they are transfers.
+            if (step + NS - 2 < whole) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * PER_WAVE) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __syncthreads();
-            multiply(step);
+            multiply(stage, [&] { load(step + NS - 1, stage == 0 ? NS - 1 : stage - 1); });
+            stage = stage + 1 == NS ? 0 : stage + 1;
+        }
+    } else {
+        Held held[2];
+        if (steps > 0) fetch(0, held[0]);
+        if (steps > 1) fetch(1, held[1]);
+        for (int64_t step = 0; step < steps; step += 2) {
+            static_for<2>([&](auto odd) __attribute__((always_inline)) {
+                constexpr int s = decltype(odd)::value;
+                if (step + s < steps) {
+                    put(s, held[s]);
+                    __syncthreads();
+                    multiply(s, [&] { if (step + s + 2 < steps) fetch(step + s + 2, held[s]); });
+                }
+            });
         }
     }
     // The results leave by whole lines: a lane has four neighbours of one row, and of the next instruction's rows others; 32 rows at a time go through LDS, of which
@@ -208,7 +246,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     // results took 17 us.
     constexpr int PIECES = 8 * TN, PER_STEP = WAVE / PIECES, COUNT = 32 / PER_STEP;   // pieces of 16 bytes in a row, rows to an instruction
     constexpr int BATCH = COUNT < 8 ? COUNT : 8;
-    static_assert(NW * 32 * 32 * TN * 4 <= 2 * STAGE, "the waves' shares fit");
+    static_assert(NW * 32 * 32 * TN * 4 <= NS * STAGE, "the waves' shares fit");
     float* mine = reinterpret_cast<float*>(lds) + wave * 32 * 32 * TN;
     auto at = [&](int row, int column) { return row * 32 * TN + 4 * (column / 4 ^ (TN == 1 ? row / 2 % 8 : row % 16)) + column % 4; };
     const int c = 4 * (lane % PIECES);
@@ -263,26 +301,32 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
         hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(512), 0, st, p);
     };
     const bool aligned = p.K % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.W)) & 15) == 0;
-    auto tile = [&](auto wm, auto wn, auto tm, auto tn, int per_cu) {
-        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, TM = decltype(tm)::value, TN = decltype(tn)::value;
+    auto tile = [&](auto wm, auto wn, auto tm, auto tn, auto ns, auto bk, int per_cu) {
+        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, TM = decltype(tm)::value, TN = decltype(tn)::value, NS = decltype(ns)::value, BK = decltype(bk)::value;
         p.tiles_m = ceil_div(p.M, (int64_t)(32 * TM * WM));
         p.tiles_n = ceil_div(p.N, (int64_t)(32 * TN * WN));
         const int64_t nwg = p.tiles_m * p.tiles_n;
         const int group_m = choose_group_m(p.tiles_m, ceil_div(nwg, (int64_t)NUM_XCD), (int64_t)per_cu * 32, 32 * TM * WM, 32 * TN * WN, p.K);
         const dim3 grid((unsigned)nwg), block(64 * WM * WN);
-        if (aligned) hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, true>), grid, block, 0, st, p, group_m);
-        else hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, false>), grid, block, 0, st, p, group_m);
+        if (aligned) hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, NS, BK, true>), grid, block, 0, st, p, group_m);
+        else hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, 2, 128, false>), grid, block, 0, st, p, group_m);
     };
+    // Which kernel, by microseconds of the forms at N = K = 4096, bfloat16 (M; 16 columns each direct / 64 x 64 / 128 x 128 one to a CU / two to a CU / 256 x 256):
+    // 4: 7.1 / 13.9 / 20 / 25 / 47; 64: 12.9 / 13.9 / 20 / 26 / 50; 128: 22 / 13.8 / 20 / 26 / 51; 512: 75 / 16.6 / 21.1 / 26 / 50; 1024: 151 / 31 / 26.0 / 29 / 51;
+    // 2048: 281 / 70 / 50 / 40 / 58; 8192 x 8192: 2239 / 439 / - / 317 / 256. Direct takes 3.5 us and 0.42 ns for each round of workgroups, k and 16 rows or columns of one
+    // (64 x 16384 x 1024: 12.9 us, 64 x 512 x 8192: 20.0); 64 x 64 as much and 2.5 ns for each round and k (7.5 and 20.2). The largest two by their rounds, 40 and 64 us each.
+    const int64_t tiles64 = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64), tiles128 = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
+    const int64_t tiles256 = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
+    const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+    const int64_t rounds16 = ceil_div(ceil_div(p.M, (int64_t)(16 * mt)) * ceil_div(p.N, (int64_t)16), (int64_t)256);
     const int form = tuning().qlin_form;
-    const int pick = form >= 0 ? form : p.M <= 64 ? 0 : p.M * p.N <= (int64_t)64 * 64 * 512 ? 1 : p.M * p.N <= (int64_t)128 * 128 * 512 ? 2 : 3;
-    if (pick == 4) tile(Int<2>{}, Int<2>{}, Int<4>{}, Int<4>{}, 1);
-    else if (pick == 5) tile(Int<4>{}, Int<2>{}, Int<2>{}, Int<4>{}, 1);
-    else if (pick == 6) tile(Int<2>{}, Int<2>{}, Int<4>{}, Int<2>{}, 1);
-    else if (pick == 3) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, 1);
-    else if (pick == 2) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, 2);
-    else if (pick == 1) tile(Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}, 4);
-    else if (p.M <= 16) direct(Int<1>{});
-    else if (p.M <= 32) direct(Int<2>{});
+    const int pick = form >= 0 ? form : rounds16 * (mt + 1) <= 6 * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
+    if (pick == 4) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, Int<2>{}, Int<128>{}, 1);
+    else if (pick == 3) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<128>{}, 2);
+    else if (pick == 2) tile(Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}, Int<3>{}, Int<128>{}, 1);
+    else if (pick == 1) tile(Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}, Int<2>{}, Int<256>{}, 2);
+    else if (mt == 1) direct(Int<1>{});
+    else if (mt == 2) direct(Int<2>{});
     else direct(Int<4>{});
 }
 

@@ -149,7 +149,7 @@ def test_linear(m, n, k, dtype):
         within(y, expected, linear_bound(size, expected, dtype))
 
 
-@pytest.mark.parametrize("form", [0, 1, 2, 3])
+@pytest.mark.parametrize("form", range(5))
 @pytest.mark.parametrize("m, n, k", [(1, 1, 1), (63, 65, 16), (65, 63, 127), (129, 140, 128), (300, 270, 144), (257, 129, 272), (64, 513, 1009), (515, 40, 640), (7, 9, 0)])
 @pytest.mark.parametrize("dtype", [F32, F16])
 def test_linear_by_every_kernel(form, m, n, k, dtype, tuning):
