@@ -76,6 +76,7 @@ static void parse_tuning(Tuning& t) {
     t.attn_split = env_int("MI355X_ATTN_SPLIT", -1);
     t.attn_few = env_int("MI355X_ATTN_FEW", -1);
     t.qlin_form = env_int("MI355X_QLIN_FORM", -1);
+    t.diff_splits = env_int("MI355X_DIFF_SPLITS", 0);
 }
 
 Tuning tuning() {

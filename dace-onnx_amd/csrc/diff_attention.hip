@@ -32,6 +32,8 @@ struct DiffArgs {
     int heads, groups, share, vector;   // share = heads / groups; vector: length of the learned vectors
     int causal, splits;
     int64_t row_blocks;                 // of the rows Sq * share of a slice (one batch entry, one group)
+    int per_xcd;                        // slices of an XCD whose blocks take turns; 0: one slice after the other
+    int fold;                           // if causal: all blocks run at once, long ones first, then from short to long
     float scale_log2, lambda_init;
 };
 
@@ -51,15 +53,21 @@ __device__ __forceinline__ int64_t diff_length(const DiffArgs& p, int64_t b) {
     return n < 0 ? 0 : n > p.Sk ? p.Sk : n;
 }
 
-// A tile's geometry: KT keys of 2 D values (both maps' keys, or the values), in pieces of 16 bytes of which piece c of key k lies at c ^ place(k): a bijection
+// Where keys (both maps', 2 D values) and values lie in LDS: rows of 16-byte pieces, of which piece c of key k lies at c ^ place(k): a bijection
 // of 16 keys (of one piece, as scores read them), and of four keys onto different quarters of the banks (the transposing reads).
 template <class T, int D>
 struct DiffTile {
-    static constexpr int KT = 32, E = 16 / sizeof(T), PIECES = 2 * D / E;   // (8 at least)
-    static constexpr int BYTES = KT * 2 * D * (int)sizeof(T);
+    static constexpr int E = 16 / sizeof(T), PIECES = 2 * D / E, ROW = 2 * D * (int)sizeof(T);   // (8 pieces at least)
     static __device__ __forceinline__ int place(int key) { return PIECES == 8 ? (key >> 1 & 1) << 2 | (key >> 2 & 3) : (key & 3) << 2 | (key >> 2 & 3); }
     static __device__ __forceinline__ int at(int key, int piece) { return (key * PIECES + (piece ^ place(key))) * E; }   // in values
 };
+
+// 16 bytes to a lane from global memory, base + the lane's offset, into LDS at lds + 16 lane; base and lds are the same for the wave.
+__device__ __forceinline__ void diff_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint64_t uniform = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory");
+}
 
 // One map's operand of Q: D / (2 E) pieces of 16 bytes to a lane.
 template <class T, int D>
@@ -132,54 +140,119 @@ struct DiffWave {
     }
 };
 
-template <class T, int D, int RB, int RW>
-__global__ __launch_bounds__(128 * RW) void diff_attention_kernel(DiffArgs p) {
+// Waves: two maps, RW blocks of 32 RB rows, KW shares of a stage's keys, 32 SUB each. Two stages: while one is multiplied the other is on its way. DIRECT: by
+// transfers that need no registers (arrays at 16-byte boundaries); the last stage, whose missing keys have to be zeros, always goes through registers.
+template <class T, int D, int RB, int RW, int KW, int SUB, bool DIRECT>
+__global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs p) {
     using Tile = DiffTile<T, D>;
     using Wave = DiffWave<T, D>;
     using Piece = typename Wave::Piece;
     using UnalignedPiece = typename Wave::UnalignedPiece;
-    constexpr int KT = Tile::KT, E = Tile::E, NT = 128 * RW, VT = Wave::VT, ROWS = 32 * RB * RW;
+    constexpr int KT = 32 * KW * SUB, E = Tile::E, NT = 128 * RW * KW, VT = Wave::VT, ROWS = 32 * RB * RW;
+    constexpr int HALF = KT * Tile::ROW, STAGE = 2 * HALF;            // keys, then values
     constexpr int PER_T = KT * Tile::PIECES / NT;
-    static_assert(KT * Tile::PIECES % NT == 0, "whole pieces to a thread");
-    constexpr int EXCHANGE = 32 * 2 * D * 4;   // bytes of a row block's output
-    constexpr int LDS = std::max(2 * Tile::BYTES, RW * EXCHANGE);
-    __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
-    T* lds_k = reinterpret_cast<T*>(lds);
-    T* lds_v = reinterpret_cast<T*>(lds + Tile::BYTES);
+    static_assert(KT * Tile::PIECES % NT == 0 && Tile::PIECES <= WAVE, "whole pieces to a thread, whole rows to a transfer");
+    constexpr int EXCHANGE = 32 * 2 * D;   // floats of a row block's output
+    static_assert(RW * EXCHANGE * 4 <= 2 * STAGE && (KW == 1 || KW * RW * RB * EXCHANGE * 4 <= 2 * STAGE) && KT * 16 <= STAGE, "room to exchange results");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
 
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    const int n = lane % 32, h = lane / 32, map = wave % 2, row_wave = wave / 2;
+    const int n = lane % 32, h = lane / 32, map = wave % 2, row_wave = wave / 2 % RW, key_wave = wave / (2 * RW);
     const int64_t logical = xcd_remap(blockIdx.x, (int64_t)gridDim.x);
-    const int64_t block = logical % p.row_blocks, rest = logical / p.row_blocks;
-    const int split = (int)(rest % p.splits);
-    const int64_t slice = rest / p.splits, b = slice / p.groups;
+    int64_t turn, slice;
+    int split = 0;
+    if (p.per_xcd) {
+        const int64_t each = p.row_blocks * p.per_xcd, local = logical % each;
+        turn = local / p.per_xcd;
+        slice = logical / each * p.per_xcd + local % p.per_xcd;
+    } else {
+        const int64_t rest = logical / p.row_blocks;
+        turn = logical % p.row_blocks;
+        split = (int)(rest % p.splits);
+        slice = rest / p.splits;
+    }
+    const int64_t half = (p.row_blocks + 1) / 2;
+    const int64_t block = !p.causal ? turn : p.fold && turn >= half ? turn - half : p.row_blocks - 1 - turn;
+    const int64_t b = slice / p.groups;
     const int group = (int)(slice % p.groups);
     const int64_t rows = p.Sq * p.share, length = diff_length(p, b);
     const int64_t ahead = length - p.Sq;   // if causal, query i sees the keys up to i + ahead
+    auto keys_of = [&](int64_t row) { return p.causal ? std::max((int64_t)0, std::min(length, row / p.share + ahead + 1)) : length; };
 
     // ---- queries: row r of a slice is head r % share of query r / share ------------------------------------
-    int64_t row[RB], seen[RB];   // seen: keys of the row
+    const int64_t row0 = block * ROWS + row_wave * RB * 32;   // of the wave
+    int seen[RB];   // keys of the row
     Piece q[RB][Wave::QP];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-        row[i] = block * ROWS + (row_wave * RB + i) * 32 + n;
-        const int64_t r = row[i] < rows ? row[i] : rows - 1, query = r / p.share;
+        const int64_t row = row0 + 32 * i + n, r = row < rows ? row : rows - 1, query = r / p.share;
         const int head = group * p.share + (int)(r % p.share);
-        seen[i] = p.causal ? std::max((int64_t)0, std::min(length, query + ahead + 1)) : length;
+        seen[i] = (int)keys_of(r);
         const T* from = static_cast<const T*>(p.Q) + ((b * p.Sq + query) * 2 * p.heads + 2 * head + map) * D + h * E;
 #pragma unroll
         for (int s = 0; s < Wave::QP; ++s) q[i][s] = *reinterpret_cast<const UnalignedPiece*>(from + 2 * s * E);
     }
-    // keys that any row of the workgroup sees, and that the last of its rows sees all of
-    const int64_t last = std::min(rows, (block + 1) * ROWS) - 1;
-    const int64_t end = p.causal ? std::max((int64_t)0, std::min(length, last / p.share + ahead + 1)) : length;
-    const int64_t all = p.causal ? std::max((int64_t)0, std::min(length, block * ROWS / p.share + ahead + 1)) : length;
-    const int64_t tiles = (end + KT - 1) / KT, per_split = (tiles + p.splits - 1) / p.splits;
-    const int64_t first_tile = split * per_split, end_tile = std::min(tiles, first_tile + per_split);
+    // keys that any row of the workgroup sees; that any row of the wave sees, and that all of its rows see
+    const int end = (int)keys_of(std::min(rows, (block + 1) * ROWS) - 1);
+    const int wave_end = __builtin_amdgcn_readfirstlane((int)keys_of(std::min(rows, row0 + 32 * RB) - 1));
+    const int wave_all = __builtin_amdgcn_readfirstlane((int)keys_of(std::min(rows - 1, row0)));
+    const int stages = (end + KT - 1) / KT, per_split = (stages + p.splits - 1) / p.splits;
+    const int first = split * per_split, last = std::min(stages, first + per_split);
 
     const T* K = static_cast<const T*>(p.K) + (b * p.Sk * p.groups + group) * 2 * D;
     const T* V = static_cast<const T*>(p.V) + (b * p.Sk * p.groups + group) * 2 * D;
     const int64_t key_stride = (int64_t)p.groups * 2 * D;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+
+    // piece tid + j NT of a stage's keys, or values: where it is in memory and, of a transfer, what of it this lane fetches
+    uint32_t offset[DIRECT ? PER_T : 1];
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int j = 0; j < PER_T; ++j) {
+            const int key = (tid + j * NT) / Tile::PIECES, piece = (tid + j * NT) % Tile::PIECES ^ Tile::place(key);
+            offset[j] = (uint32_t)((key * key_stride + piece * E) * sizeof(T));
+        }
+    }
+    Piece hk[PER_T], hv[PER_T];
+    auto fetch = [&](int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < PER_T; ++j) {
+            const int key = (tid + j * NT) / Tile::PIECES, piece = (tid + j * NT) % Tile::PIECES;
+            hk[j] = hv[j] = Piece{};
+            if (stage * KT + key < length) {   // (keys that do not exist may lie outside, or hold anything)
+                const int64_t at = (stage * (int64_t)KT + key) * key_stride + piece * E;
+                hk[j] = *reinterpret_cast<const UnalignedPiece*>(K + at);
+                hv[j] = *reinterpret_cast<const UnalignedPiece*>(V + at);
+            }
+        }
+    };
+    auto put = [&](int buffer) __attribute__((always_inline)) {
+        T* to = reinterpret_cast<T*>(lds + buffer * STAGE);
+#pragma unroll
+        for (int j = 0; j < PER_T; ++j) {
+            const int key = (tid + j * NT) / Tile::PIECES, piece = (tid + j * NT) % Tile::PIECES;
+            *reinterpret_cast<Piece*>(to + Tile::at(key, piece)) = hk[j];
+            *reinterpret_cast<Piece*>(to + HALF / sizeof(T) + Tile::at(key, piece)) = hv[j];
+        }
+    };
+    auto load = [&](int stage, int buffer) __attribute__((always_inline)) {
+        if constexpr (DIRECT) {
+            if ((stage + 1) * (int64_t)KT <= length) {
+                const int64_t at = stage * (int64_t)KT * key_stride;
+#pragma unroll
+                for (int j = 0; j < PER_T; ++j) {
+                    const uint32_t to = lds0 + (uint32_t)(buffer * STAGE + (wave * WAVE + j * NT) * 16);
+                    diff_to_lds(K + at, offset[j], to);
+                    diff_to_lds(V + at, offset[j], to + HALF);
+                }
+            } else {
+                fetch(stage);
+                put(buffer);
+            }
+        } else {
+            fetch(stage);
+        }
+    };
 
     f32x16 out[RB][VT];
     float most[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
@@ -191,69 +264,113 @@ __global__ __launch_bounds__(128 * RW) void diff_attention_kernel(DiffArgs p) {
         for (int c = 0; c < VT; ++c) out[i][c] = f32x16{};
     }
 
-    for (int64_t tile = first_tile; tile < end_tile; ++tile) {
-        Piece k[PER_T], v[PER_T];
+    if (first < last) load(first, 0);
+    for (int stage = first, buffer = 0; stage < last; ++stage, buffer ^= 1) {
+        if constexpr (!DIRECT) put(buffer);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the stage is in LDS, and nobody reads the other one any more
+        __syncthreads();
+        if (stage + 1 < last) load(stage + 1, buffer ^ 1);
 #pragma unroll
-        for (int j = 0; j < PER_T; ++j) {
-            const int piece = (tid + j * NT) % Tile::PIECES, key = (tid + j * NT) / Tile::PIECES;
-            k[j] = v[j] = Piece{};
-            if (tile * KT + key < length) {   // (keys that do not exist may lie outside, or hold anything)
-                const int64_t at = (tile * KT + key) * key_stride + piece * E;
-                k[j] = *reinterpret_cast<const UnalignedPiece*>(K + at);
-                v[j] = *reinterpret_cast<const UnalignedPiece*>(V + at);
+        for (int u = 0; u < SUB; ++u) {
+            const int local = (key_wave * SUB + u) * 32, key0 = stage * KT + local;
+            if (key0 >= wave_end) break;   // (the same for the wave)
+            const T* lds_k = reinterpret_cast<const T*>(lds + buffer * STAGE) + local * 2 * D;
+            const T* lds_v = lds_k + HALF / sizeof(T);
+            f32x16 s[RB];
+#pragma unroll
+            for (int i = 0; i < RB; ++i) s[i] = Wave::scores(lds_k, map, n, h, q[i]);
+            if (key0 + 32 > wave_all) {
+#pragma unroll
+                for (int i = 0; i < RB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (key0 + 8 * (r / 4) + 4 * h + r % 4 >= seen[i]) s[i][r] = -__builtin_inff();
+            }
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                float m = s[i][0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) m = fmaxf(m, s[i][r]);
+                m = fmaxf(m, __shfl_xor(m, 32, WAVE)) * p.scale_log2;
+                if (__any(m > most[i])) {
+                    const float now = fmaxf(most[i], m), factor = most[i] == now ? 1.0f : __builtin_amdgcn_exp2f(most[i] - now);
+                    most[i] = now;
+                    sum[i] *= factor;
+#pragma unroll
+                    for (int c = 0; c < VT; ++c) out[i][c] *= factor;
+                }
+                const float base = most[i] == -__builtin_inff() ? 0.0f : most[i];   // no key so far: exp2(-inf)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -base));
+                    sum[i] += s[i][r];
+                }
+            }
+            Wave::values(lds_v, n, h, s, out);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RB; ++i) sum[i] += __shfl_xor(sum[i], 32, WAVE);
+
+    // ---- the shares of the keys meet, in pairs ------------------------------------------------------------
+    float* exchange = reinterpret_cast<float*>(lds);
+    if constexpr (KW > 1) {
+        __shared__ float most_sum[KW][RW][2][RB][2][32];
+        __syncthreads();   // nobody reads the stages any more
+        if (h == 0) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                most_sum[key_wave][row_wave][map][i][0][n] = most[i];
+                most_sum[key_wave][row_wave][map][i][1][n] = sum[i];
             }
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < PER_T; ++j) {
-            const int piece = (tid + j * NT) % Tile::PIECES, key = (tid + j * NT) / Tile::PIECES;
-            *reinterpret_cast<Piece*>(lds_k + Tile::at(key, piece)) = k[j];
-            *reinterpret_cast<Piece*>(lds_v + Tile::at(key, piece)) = v[j];
-        }
-        __syncthreads();
-
-        f32x16 s[RB];
-#pragma unroll
-        for (int i = 0; i < RB; ++i) s[i] = Wave::scores(lds_k, map, n, h, q[i]);
-        if ((tile + 1) * KT > all) {
-#pragma unroll
-            for (int i = 0; i < RB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (tile * KT + 8 * (r / 4) + 4 * h + r % 4 >= seen[i]) s[i][r] = -__builtin_inff();
-        }
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
-            float m = s[i][0];
+            float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-            for (int r = 1; r < 16; ++r) m = fmaxf(m, s[i][r]);
-            m = fmaxf(m, __shfl_xor(m, 32, WAVE)) * p.scale_log2;
-            if (__any(m > most[i])) {
-                const float now = fmaxf(most[i], m), factor = most[i] == now ? 1.0f : __builtin_amdgcn_exp2f(most[i] - now);
-                most[i] = now;
-                sum[i] *= factor;
+            for (int w = 0; w < KW; ++w) top = fmaxf(top, most_sum[w][row_wave][map][i][0][n]);
+            const float base = top == -__builtin_inff() ? 0.0f : top, factor = __builtin_amdgcn_exp2f(most[i] - base);
 #pragma unroll
-                for (int c = 0; c < VT; ++c) out[i][c] *= factor;
-            }
-            const float base = most[i] == -__builtin_inff() ? 0.0f : most[i];   // no key so far: exp2(-inf)
+            for (int w = 0; w < KW; ++w) total = fmaf(most_sum[w][row_wave][map][i][1][n], __builtin_amdgcn_exp2f(most_sum[w][row_wave][map][i][0][n] - base), total);
+            most[i] = top;
+            sum[i] = total;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -base));
-                sum[i] += s[i][r];
-            }
+            for (int c = 0; c < VT; ++c) out[i][c] *= factor;
         }
-        Wave::values(lds_v, n, h, s, out);
+#pragma unroll
+        for (int step = KW / 2; step >= 1; step /= 2) {
+            const int slot = ((key_wave % step) * RW + row_wave) * 2 + map;
+            if (key_wave >= step && key_wave < 2 * step) {
+#pragma unroll
+                for (int i = 0; i < RB; ++i)
+#pragma unroll
+                    for (int c = 0; c < VT; ++c)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) exchange[(slot * RB + i) * EXCHANGE + (16 * c + r) * WAVE + lane] = out[i][c][r];
+            }
+            __syncthreads();
+            if (key_wave < step) {
+#pragma unroll
+                for (int i = 0; i < RB; ++i)
+#pragma unroll
+                    for (int c = 0; c < VT; ++c)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) out[i][c][r] += exchange[(slot * RB + i) * EXCHANGE + (16 * c + r) * WAVE + lane];
+            }
+            __syncthreads();
+        }
     }
 
     // ---- the two maps meet --------------------------------------------------------------------------------
-    float* exchange = reinterpret_cast<float*>(lds) + row_wave * (EXCHANGE / 4);
+    const bool result = key_wave == 0;
     const float weight = p.splits > 1 ? 0.0f : diff_lambda(p);
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-        sum[i] += __shfl_xor(sum[i], 32, WAVE);
+        const int64_t row = row0 + 32 * i + n;
         if (p.splits > 1) {
-            if (row[i] < rows) {
-                const int64_t at = ((split * p.batch * p.groups + slice) * rows + row[i]) * 2 + map;
+            if (result && row < rows) {
+                const int64_t at = ((split * p.batch * p.groups + slice) * rows + row) * 2 + map;
                 if (h == 0) {
                     p.partial_ml[2 * at] = most[i];
                     p.partial_ml[2 * at + 1] = sum[i];
@@ -268,17 +385,18 @@ __global__ __launch_bounds__(128 * RW) void diff_attention_kernel(DiffArgs p) {
             continue;
         }
         const float factor = sum[i] == 0.0f ? 0.0f : (map ? weight : 1.0f) / sum[i];   // a row without keys: 0
+        float* other = exchange + row_wave * EXCHANGE;
         __syncthreads();
-        if (map == 1) {
+        if (result && map == 1) {
 #pragma unroll
             for (int c = 0; c < VT; ++c)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) exchange[(16 * c + r) * WAVE + lane] = out[i][c][r] * factor;
+                for (int r = 0; r < 16; ++r) other[(16 * c + r) * WAVE + lane] = out[i][c][r] * factor;
         }
         __syncthreads();
-        if (map == 0 && row[i] < rows) {
-            const int64_t query = row[i] / p.share;
-            const int head = group * p.share + (int)(row[i] % p.share);
+        if (result && map == 0 && row < rows) {
+            const int64_t query = row / p.share;
+            const int head = group * p.share + (int)(row % p.share);
             T* to = static_cast<T*>(p.O) + ((b * p.Sq + query) * p.heads + head) * 2 * D;
 #pragma unroll
             for (int c = 0; c < VT; ++c)
@@ -286,7 +404,7 @@ __global__ __launch_bounds__(128 * RW) void diff_attention_kernel(DiffArgs p) {
                 for (int g = 0; g < 4; ++g) {
                     float o[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = out[i][c][4 * g + e] * factor - exchange[(16 * c + 4 * g + e) * WAVE + lane];
+                    for (int e = 0; e < 4; ++e) o[e] = out[i][c][4 * g + e] * factor - other[(16 * c + 4 * g + e) * WAVE + lane];
                     store_values(to + 32 * c + 8 * g + 4 * h, o, 4);
                 }
         }
@@ -325,16 +443,37 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs p) {
     store_values(static_cast<T*>(p.O) + ((b * p.Sq + row / p.share) * p.heads + head) * 2 * D + lane * PER_LANE, result, PER_LANE);
 }
 
+// How a type and head size are cut: rows of a wave for many rows, keys of a stage, and key waves for few rows.
+template <class T, int D>
+struct DiffForm {
+    static constexpr int BYTES = D * (int)sizeof(T);   // 64 to 512
+    static constexpr int RB = BYTES <= 128 ? 2 : 1, RW = 2, SUB = BYTES <= 128 ? 2 : 1;
+    static constexpr int KW = BYTES <= 128 ? 4 : BYTES <= 256 ? 2 : 1;
+};
+constexpr int64_t DIFF_FEW = 32;   // rows of a slice up to which a workgroup has one block of them
+
 template <class T, int D>
 static int launch_diff(DiffArgs p, hipStream_t st) {
-    constexpr int RB = D * sizeof(T) <= 128 ? 2 : 1, RW = 2;
-    const int64_t rows = p.Sq * p.share;
-    p.row_blocks = ceil_div(rows, (int64_t)(32 * RB * RW));
-    const int64_t grid = p.row_blocks * p.splits * p.batch * p.groups;
-    MI355X_REQUIRE(grid_fits(grid, 128 * RW), "differential_attention: too large");
-    hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW>), dim3((unsigned)grid), dim3(128 * RW), 0, st, p);
+    using F = DiffForm<T, D>;
+    const int64_t rows = p.Sq * p.share, slices = p.batch * p.groups;
+    const bool direct = ((reinterpret_cast<uintptr_t>(p.K) | reinterpret_cast<uintptr_t>(p.V)) & 15) == 0 && (int64_t)p.groups * D < 1 << 20;
+    int64_t grid = 0;
+    auto launch = [&](auto rb, auto rw, auto kw, auto sub) {
+        constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value;
+        p.row_blocks = ceil_div(rows, (int64_t)(32 * RB * RW));
+        grid = p.row_blocks * p.splits * slices;
+        if (!grid_fits(grid, 128 * RW * KW)) return;
+        p.per_xcd = p.causal && p.splits == 1 && slices % NUM_XCD == 0 ? (int)(slices / NUM_XCD) : 0;
+        p.fold = grid <= 512;
+        const dim3 g((unsigned)grid), block(128 * RW * KW);
+        if (direct) hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, true>), g, block, 0, st, p);
+        else hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, false>), g, block, 0, st, p);
+    };
+    if (rows <= DIFF_FEW) launch(Int<1>{}, Int<1>{}, Int<F::KW>{}, Int<1>{});
+    else launch(Int<F::RB>{}, Int<F::RW>{}, Int<1>{}, Int<F::SUB>{});
+    MI355X_REQUIRE(grid_fits(grid, 512), "differential_attention: too large");
     if (p.splits > 1) {
-        const int64_t all = p.batch * p.groups * rows;
+        const int64_t all = slices * rows;
         hipLaunchKernelGGL((diff_join_kernel<T, D>), dim3((unsigned)ceil_div(all, (int64_t)4)), dim3(256), 0, st, p);
     }
     return check_launch("diff_attention_kernel");
@@ -343,8 +482,15 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
 }  // namespace mi355x
 
 extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups, int64_t size, int type) {
-    (void)batch; (void)Sq; (void)Sk; (void)heads; (void)groups; (void)size; (void)type;
-    return 1;
+    using namespace mi355x;
+    if (!is_mixed_type(type) || (size != 32 && size != 64 && size != 128) || groups < 1 || heads < 1 || heads % groups || batch < 1 || Sq < 1 || Sk < 1) return 1;
+    const int64_t rows = Sq * (heads / groups), bytes = size * (type == MI355X_TYPE_FLOAT ? 4 : 2);
+    const int64_t few = rows <= DIFF_FEW, keys = few ? (bytes <= 128 ? 128 : bytes <= 256 ? 64 : 32) : bytes <= 128 ? 64 : 32;   // of a stage
+    const int64_t workgroups = batch * groups * ceil_div(rows, few ? 32 : bytes <= 128 ? 128 : 64), stages = ceil_div(Sk, keys);
+    const int form = tuning().diff_splits;
+    if (form > 0) return std::min(form, 256);
+    const int64_t room = 512 / workgroups;   // two workgroups to a CU
+    return std::max((int64_t)1, std::min({room, stages / 2, (int64_t)256}));
 }
 
 extern "C" int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1, const float* lambda_k1,
