@@ -46,6 +46,15 @@ __device__ __forceinline__ float diff_lambda(const DiffArgs& p) {
     return expf(wave_sum(a)) - expf(wave_sum(b)) + p.lambda_init;
 }
 
+// f(a lane's value, that of the lane 32 from it)
+template <class F>
+__device__ __forceinline__ float across_halves(float v, F&& f) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto both = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);   // the lower lanes' values, the upper lanes'
+    const uint32_t lower = both[0], upper = both[1];   // (a bit_cast of a vector's element is one of its first)
+    return f(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
+}
+
 // keys that batch entry b has; what a caller wrote beyond the array is taken as all of it
 __device__ __forceinline__ int64_t diff_length(const DiffArgs& p, int64_t b) {
     if (!p.lengths) return p.Sk;
@@ -143,7 +152,7 @@ struct DiffWave {
 // Waves: two maps, RW blocks of 32 RB rows, KW shares of a stage's keys, 32 SUB each. Two stages: while one is multiplied the other is on its way. DIRECT: by
 // transfers that need no registers (arrays at 16-byte boundaries); the last stage, whose missing keys have to be zeros, always goes through registers.
 template <class T, int D, int RB, int RW, int KW, int SUB, bool DIRECT>
-__global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs p) {
+__global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffArgs p) {
     using Tile = DiffTile<T, D>;
     using Wave = DiffWave<T, D>;
     using Piece = typename Wave::Piece;
@@ -255,10 +264,10 @@ __global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs 
     };
 
     f32x16 out[RB][VT];
-    float most[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
+    float base[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-        most[i] = -__builtin_inff();
+        base[i] = -__builtin_inff();
         sum[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < VT; ++c) out[i][c] = f32x16{};
@@ -286,23 +295,33 @@ __global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs 
                     for (int r = 0; r < 16; ++r)
                         if (key0 + 8 * (r / 4) + 4 * h + r % 4 >= seen[i]) s[i][r] = -__builtin_inff();
             }
+            // the base of a row's powers is the largest score so far, or up to 8 below it: P is at most 2^8, and outputs are rarely scaled
+            float m[RB];
+            bool far = false;
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                float m = s[i][0];
+                m[i] = s[i][0];
 #pragma unroll
-                for (int r = 1; r < 16; ++r) m = fmaxf(m, s[i][r]);
-                m = fmaxf(m, __shfl_xor(m, 32, WAVE)) * p.scale_log2;
-                if (__any(m > most[i])) {
-                    const float now = fmaxf(most[i], m), factor = most[i] == now ? 1.0f : __builtin_amdgcn_exp2f(most[i] - now);
-                    most[i] = now;
+                for (int r = 1; r < 16; ++r) m[i] = fmaxf(m[i], s[i][r]);
+                m[i] = across_halves(m[i], [](float x, float y) { return fmaxf(x, y); }) * p.scale_log2;
+                far |= m[i] > base[i] + 8.0f;
+            }
+            if (__any(far)) {
+#pragma unroll
+                for (int i = 0; i < RB; ++i) {
+                    const float now = fmaxf(base[i], m[i]), factor = base[i] == now ? 1.0f : __builtin_amdgcn_exp2f(base[i] - now);
+                    base[i] = now;
                     sum[i] *= factor;
 #pragma unroll
                     for (int c = 0; c < VT; ++c) out[i][c] *= factor;
                 }
-                const float base = most[i] == -__builtin_inff() ? 0.0f : most[i];   // no key so far: exp2(-inf)
+            }
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                const float from = base[i] == -__builtin_inff() ? 0.0f : base[i];   // no key so far: exp2(-inf)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -base));
+                    s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from));
                     sum[i] += s[i][r];
                 }
             }
@@ -310,18 +329,18 @@ __global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs 
         }
     }
 #pragma unroll
-    for (int i = 0; i < RB; ++i) sum[i] += __shfl_xor(sum[i], 32, WAVE);
+    for (int i = 0; i < RB; ++i) sum[i] = across_halves(sum[i], [](float x, float y) { return x + y; });
 
     // ---- the shares of the keys meet, in pairs ------------------------------------------------------------
     float* exchange = reinterpret_cast<float*>(lds);
     if constexpr (KW > 1) {
-        __shared__ float most_sum[KW][RW][2][RB][2][32];
+        __shared__ float base_sum[KW][RW][2][RB][2][32];
         __syncthreads();   // nobody reads the stages any more
         if (h == 0) {
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                most_sum[key_wave][row_wave][map][i][0][n] = most[i];
-                most_sum[key_wave][row_wave][map][i][1][n] = sum[i];
+                base_sum[key_wave][row_wave][map][i][0][n] = base[i];
+                base_sum[key_wave][row_wave][map][i][1][n] = sum[i];
             }
         }
         __syncthreads();
@@ -329,11 +348,11 @@ __global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs 
         for (int i = 0; i < RB; ++i) {
             float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < KW; ++w) top = fmaxf(top, most_sum[w][row_wave][map][i][0][n]);
-            const float base = top == -__builtin_inff() ? 0.0f : top, factor = __builtin_amdgcn_exp2f(most[i] - base);
+            for (int w = 0; w < KW; ++w) top = fmaxf(top, base_sum[w][row_wave][map][i][0][n]);
+            const float from = top == -__builtin_inff() ? 0.0f : top, factor = __builtin_amdgcn_exp2f(base[i] - from);
 #pragma unroll
-            for (int w = 0; w < KW; ++w) total = fmaf(most_sum[w][row_wave][map][i][1][n], __builtin_amdgcn_exp2f(most_sum[w][row_wave][map][i][0][n] - base), total);
-            most[i] = top;
+            for (int w = 0; w < KW; ++w) total = fmaf(base_sum[w][row_wave][map][i][1][n], __builtin_amdgcn_exp2f(base_sum[w][row_wave][map][i][0][n] - from), total);
+            base[i] = top;
             sum[i] = total;
 #pragma unroll
             for (int c = 0; c < VT; ++c) out[i][c] *= factor;
@@ -372,7 +391,7 @@ __global__ __launch_bounds__(128 * RW * KW) void diff_attention_kernel(DiffArgs 
             if (result && row < rows) {
                 const int64_t at = ((split * p.batch * p.groups + slice) * rows + row) * 2 + map;
                 if (h == 0) {
-                    p.partial_ml[2 * at] = most[i];
+                    p.partial_ml[2 * at] = base[i];
                     p.partial_ml[2 * at + 1] = sum[i];
                 }
 #pragma unroll
@@ -423,16 +442,43 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs p) {
     float result[PER_LANE] = {};
 #pragma unroll
     for (int map = 0; map < 2; ++map) {
-        float most = -__builtin_inff();
-        for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.partial_ml[2 * ((s * all + at) * 2 + map)]);
-        const float base = most == -__builtin_inff() ? 0.0f : most;
-        float sum = 0.0f, o[PER_LANE] = {};
-        for (int s = 0; s < p.splits; ++s) {
-            const int64_t i = (s * all + at) * 2 + map;
-            const float factor = __builtin_amdgcn_exp2f(p.partial_ml[2 * i] - base);
-            sum = fmaf(p.partial_ml[2 * i + 1], factor, sum);
+        // lane s has the base and the sum of splits s, s + 64, ...
+        float base[4], sums[4], top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(p.partial_o[i * 2 * D + lane * PER_LANE + e], factor, o[e]);
+        for (int i = 0; i < 4; ++i) {
+            const int s = lane + i * WAVE;
+            const bool is = s < p.splits;
+            base[i] = is ? p.partial_ml[2 * ((s * all + at) * 2 + map)] : -__builtin_inff();
+            sums[i] = is ? p.partial_ml[2 * ((s * all + at) * 2 + map) + 1] : 0.0f;
+            top = fmaxf(top, base[i]);
+        }
+        top = wave_max(top);
+        const float from = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            base[i] = __builtin_amdgcn_exp2f(base[i] - from);
+            sum = fmaf(sums[i], base[i], sum);
+        }
+        sum = wave_sum(sum);
+        float o[PER_LANE] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int count = p.splits - i * WAVE < WAVE ? p.splits - i * WAVE : WAVE;
+            const float* from_split = p.partial_o + ((i * WAVE * all + at) * 2 + map) * 2 * D + lane * PER_LANE;
+            for (int s0 = 0; s0 < count; s0 += 8) {   // eight at a time on their way
+                float part[8][PER_LANE];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int s = s0 + j < count ? s0 + j : count - 1;
+                    load_values(part[j], from_split + s * all * 4 * D, PER_LANE);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float factor = s0 + j < count ? readlane_f32(base[i], s0 + j) : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(part[j][e], factor, o[e]);
+                }
+            }
         }
         const float factor = sum == 0.0f ? 0.0f : (map ? -weight : 1.0f) / sum;
 #pragma unroll
