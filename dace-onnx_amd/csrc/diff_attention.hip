@@ -7,7 +7,7 @@
 //   * S^T = K Q^T by 32 x 32 MFMA tiles: lane (n, h) gets 16 scores of row n, of the keys 8 (r / 4) + 4 h + r % 4. Largest score and sum of a row are
 //     15 steps in the lane and one across lanes n and n + 32.
 //   * Those registers are the second product's operand as they stand: O^T = V^T P^T, whose k indices are dealt to the lanes the same way. With 16-bit
-//     values V's operand comes from LDS by transposing reads, with float32 by 4-byte reads. Every lane has one row: a running maximum that
+//     values V's operand comes from LDS by transposing reads, with float32 by 4-byte reads (and is split in three, see Operand). Every lane has one row: a running maximum that
 //     changes is one factor to a lane.
 //   * Keys and values are staged through LDS for all waves, 16-byte pieces permuted within a row so that reads of a column meet no bank twice.
 // P is rounded to the arrays' type for the second product, half a step of it; the sum is that of the values before.
@@ -78,79 +78,126 @@ __device__ __forceinline__ void diff_to_lds(const void* base, uint32_t offset, u
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory");
 }
 
-// One map's operand of Q: D / (2 E) pieces of 16 bytes to a lane.
+// Eight values of an operand as the matrix unit takes them: one vector of 16-bit numbers, or a float32 as the sum of three bfloat16 numbers, its
+// first, middle and last eight bits. Of the nine partial products of two such values the six largest are taken; those left out are below 2^-23 of the
+// product. (An infinity is no such sum: it gives NaN.)
+template <class T>
+struct Operand {
+    typedef T Vector __attribute__((ext_vector_type(8)));
+    Vector part[1];
+    __device__ __forceinline__ void set(const T (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[0][e] = v[e];
+    }
+    static __device__ __forceinline__ void product(const Operand& a, const Operand& b, f32x16& acc) {
+        if constexpr (std::is_same_v<T, f16>) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.part[0], b.part[0], acc, 0, 0, 0);
+        else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.part[0], b.part[0], acc, 0, 0, 0);
+    }
+};
+template <>
+struct Operand<float> {
+    u32x4 part[3];
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x[2] = {v[2 * e], v[2 * e + 1]};
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const uint32_t bits[2] = {__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1])};
+                part[i][e] = __builtin_amdgcn_perm(bits[1], bits[0], 0x07060302u);   // the upper halves
+                if (i == 2) break;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) x[j] -= __builtin_bit_cast(float, bits[j] & 0xffff0000u);
+            }
+        }
+    }
+    static __device__ __forceinline__ void product(const Operand& a, const Operand& b, f32x16& acc) {
+        auto one = [&](int i, int j) __attribute__((always_inline)) {
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.part[i]), __builtin_bit_cast(bf16x8, b.part[j]), acc, 0, 0, 0);
+        };
+        one(0, 2), one(1, 1), one(2, 0), one(0, 1), one(1, 0), one(0, 0);   // the smallest first
+    }
+};
+
 template <class T, int D>
 struct DiffWave {
     using Tile = DiffTile<T, D>;
-    static constexpr int E = Tile::E, QP = D / (2 * E), VT = 2 * D / 32;
+    static constexpr int E = Tile::E, QP = D / 16, VT = 2 * D / 32;   // operands of a map's query or key, tiles of 32 value columns
 
     typedef T Piece __attribute__((ext_vector_type(E)));
     typedef Piece UnalignedPiece __attribute__((aligned(sizeof(T))));
 
+    // Addresses in LDS of what a lane reads differ by constants in the bits of the piece (an exclusive or) and in those of the key (an offset of the
+    // instruction). Two of them are kept and the others made where they are used: kept as well they took 64 registers, and the accumulators went to memory.
+    template <class V>
+    static __device__ __forceinline__ V read(uint32_t at, int offset) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) V*>(reinterpret_cast<const __attribute__((address_space(3))) char*>(at) + offset);
+    }
+    static __device__ __forceinline__ uint32_t key_address(int map, int n, int h) { return Tile::at(n, (map * D + 8 * h) / E) * sizeof(T); }
+    static __device__ __forceinline__ uint32_t value_address(int lane, int n, int h) {
+        if constexpr (std::is_same_v<T, float>) return Tile::at(4 * h, n / E) * sizeof(T) + n % E * sizeof(T);
+        const int row = lane % 16 / 4, col = 16 * (lane / 16 % 2) + 4 * (lane % 4);   // what a transposing read fetches for others
+        return Tile::at(4 * h + row, col / 8) * sizeof(T) + col % 8 * sizeof(T);
+    }
+
     // S^T of 32 keys and 32 rows
-    static __device__ __forceinline__ f32x16 scores(const T* lds_k, int map, int n, int h, const Piece (&q)[QP]) {
+    static __device__ __forceinline__ f32x16 scores(uint32_t lds_k, const Operand<T> (&q)[QP]) {
         f32x16 acc = {};
 #pragma unroll
         for (int s = 0; s < QP; ++s) {
-            const Piece k = *reinterpret_cast<const Piece*>(lds_k + Tile::at(n, map * (D / E) + 2 * s + h));
-            if constexpr (std::is_same_v<T, float>) {
+            T v[8];
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[s][e], acc, 0, 0, 0);
-            } else if constexpr (std::is_same_v<T, f16>) {
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], acc, 0, 0, 0);
-            } else {
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[s], acc, 0, 0, 0);
+            for (int i = 0; i < 8 / E; ++i) {
+                const Piece piece = read<Piece>(lds_k ^ (16 * (16 / E * s + i)), 0);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[i * E + e] = piece[e];
             }
+            Operand<T> k;
+            k.set(v);
+            Operand<T>::product(k, q[s], acc);
         }
         return acc;
     }
 
-    // O^T += V^T P^T over 32 keys
+    // O^T += V^T P^T over 32 keys; element e of half h of a k-step t is key 16 t + 4 h + e, from e = 4 on four more
     template <int RB>
-    static __device__ __forceinline__ void values(const T* lds_v, int n, int h, const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT]) {
-        if constexpr (std::is_same_v<T, float>) {
+    static __device__ __forceinline__ void values(uint32_t lds_v, const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT]) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int key = 8 * (r / 4) + 4 * h + r % 4;
+        for (int t = 0; t < 2; ++t) {
+            Operand<T> pr[RB];
 #pragma unroll
-                for (int c = 0; c < VT; ++c) {
-                    const int col = 32 * c + n;
-                    const float v = lds_v[Tile::at(key, col / E) + col % E];
+            for (int b = 0; b < RB; ++b) {
+                T v[8];
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) out[b][c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, prob[b][r], out[b][c], 0, 0, 0);
-                }
+                for (int e = 0; e < 8; ++e) v[e] = (T)prob[b][8 * t + e];
+                pr[b].set(v);
             }
-        } else {
-            const int lane = threadIdx.x % WAVE, row = lane % 16 / 4, col = 16 * (lane / 16 % 2) + 4 * (lane % 4);   // what a transposing read fetches for others
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                Piece pr[RB];
+            for (int c = 0; c < VT; ++c) {
+                Operand<T> v;
+                if constexpr (std::is_same_v<T, float>) {
+                    float x[8];
 #pragma unroll
-                for (int b = 0; b < RB; ++b)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) pr[b][e] = (T)prob[b][8 * t + e];
-#pragma unroll
-                for (int c = 0; c < VT; ++c) {
+                    for (int e = 0; e < 8; ++e) x[e] = read<float>(lds_v ^ (16 * (8 * c ^ (e % 4) << 2 ^ 2 * (e / 4))), (16 * t + 8 * (e / 4) + e % 4) * Tile::ROW);
+                    v.set(x);
+                } else {
                     s16x4 half[2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = 16 * t + 8 * i + 4 * h + row, value = 32 * c + col;
-                        half[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_v + Tile::at(key, value / 8) + value % 8));
-                    }
-                    const Piece v = __builtin_bit_cast(Piece, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        if constexpr (std::is_same_v<T, f16>) out[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pr[b], out[b][c], 0, 0, 0);
-                        else out[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pr[b], out[b][c], 0, 0, 0);
-                    }
+                    for (int i = 0; i < 2; ++i)
+                        half[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(reinterpret_cast<__attribute__((address_space(3))) char*>(
+                            lds_v ^ (16 * (4 * c ^ 2 * i))) + (16 * t + 8 * i) * Tile::ROW));
+                    v.part[0] = __builtin_bit_cast(typename Operand<T>::Vector, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
                 }
+#pragma unroll
+                for (int b = 0; b < RB; ++b) Operand<T>::product(v, pr[b], out[b][c]);
             }
         }
     }
 };
 
 // Waves: two maps, RW blocks of 32 RB rows, KW shares of a stage's keys, 32 SUB each. Two stages: while one is multiplied the other is on its way. DIRECT: by
-// transfers that need no registers (arrays at 16-byte boundaries); the last stage, whose missing keys have to be zeros, always goes through registers.
+// transfers that need no registers (arrays at 16-byte boundaries); the last stage, whose missing keys have to be zeros, always goes through registers, and
+// so do all stages of arrays at other addresses.
 template <class T, int D, int RB, int RW, int KW, int SUB, bool DIRECT>
 __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffArgs p) {
     using Tile = DiffTile<T, D>;
@@ -191,15 +238,24 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
     // ---- queries: row r of a slice is head r % share of query r / share ------------------------------------
     const int64_t row0 = block * ROWS + row_wave * RB * 32;   // of the wave
     int seen[RB];   // keys of the row
-    Piece q[RB][Wave::QP];
+    Operand<T> q[RB][Wave::QP];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
         const int64_t row = row0 + 32 * i + n, r = row < rows ? row : rows - 1, query = r / p.share;
         const int head = group * p.share + (int)(r % p.share);
         seen[i] = (int)keys_of(r);
-        const T* from = static_cast<const T*>(p.Q) + ((b * p.Sq + query) * 2 * p.heads + 2 * head + map) * D + h * E;
+        const T* from = static_cast<const T*>(p.Q) + ((b * p.Sq + query) * 2 * p.heads + 2 * head + map) * D + 8 * h;
 #pragma unroll
-        for (int s = 0; s < Wave::QP; ++s) q[i][s] = *reinterpret_cast<const UnalignedPiece*>(from + 2 * s * E);
+        for (int s = 0; s < Wave::QP; ++s) {
+            T v[8];
+#pragma unroll
+            for (int j = 0; j < 8 / E; ++j) {
+                const Piece piece = *reinterpret_cast<const UnalignedPiece*>(from + 16 * s + j * E);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[j * E + e] = piece[e];
+            }
+            q[i][s].set(v);
+        }
     }
     // keys that any row of the workgroup sees; that any row of the wave sees, and that all of its rows see
     const int end = (int)keys_of(std::min(rows, (block + 1) * ROWS) - 1);
@@ -222,27 +278,27 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
             offset[j] = (uint32_t)((key * key_stride + piece * E) * sizeof(T));
         }
     }
-    Piece hk[PER_T], hv[PER_T];
-    auto fetch = [&](int stage) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < PER_T; ++j) {
-            const int key = (tid + j * NT) / Tile::PIECES, piece = (tid + j * NT) % Tile::PIECES;
-            hk[j] = hv[j] = Piece{};
-            if (stage * KT + key < length) {   // (keys that do not exist may lie outside, or hold anything)
-                const int64_t at = (stage * (int64_t)KT + key) * key_stride + piece * E;
-                hk[j] = *reinterpret_cast<const UnalignedPiece*>(K + at);
-                hv[j] = *reinterpret_cast<const UnalignedPiece*>(V + at);
-            }
-        }
-    };
-    auto put = [&](int buffer) __attribute__((always_inline)) {
+    auto by_registers = [&](int stage, int buffer) __attribute__((always_inline)) {
+        constexpr int BATCH = PER_T < 4 ? PER_T : 4;
         T* to = reinterpret_cast<T*>(lds + buffer * STAGE);
 #pragma unroll
-        for (int j = 0; j < PER_T; ++j) {
-            const int key = (tid + j * NT) / Tile::PIECES, piece = (tid + j * NT) % Tile::PIECES;
-            *reinterpret_cast<Piece*>(to + Tile::at(key, piece)) = hk[j];
-            *reinterpret_cast<Piece*>(to + HALF / sizeof(T) + Tile::at(key, piece)) = hv[j];
-        }
+        for (int half = 0; half < 2; ++half)
+#pragma unroll 1
+            for (int j0 = 0; j0 < PER_T; j0 += BATCH) {
+                Piece held[BATCH];
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const int at = tid + (j0 + j) * NT, piece = at % Tile::PIECES, key = at / Tile::PIECES;
+                    held[j] = Piece{};
+                    if (stage * (int64_t)KT + key < length)   // (keys that do not exist may lie outside, or hold anything)
+                        held[j] = *reinterpret_cast<const UnalignedPiece*>((half ? V : K) + (stage * (int64_t)KT + key) * key_stride + piece * E);
+                }
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const int at = tid + (j0 + j) * NT, piece = at % Tile::PIECES, key = at / Tile::PIECES;
+                    *reinterpret_cast<Piece*>(to + half * (HALF / (int)sizeof(T)) + Tile::at(key, piece)) = held[j];
+                }
+            }
     };
     auto load = [&](int stage, int buffer) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
@@ -254,15 +310,13 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
                     diff_to_lds(K + at, offset[j], to);
                     diff_to_lds(V + at, offset[j], to + HALF);
                 }
-            } else {
-                fetch(stage);
-                put(buffer);
+                return;
             }
-        } else {
-            fetch(stage);
         }
+        by_registers(stage, buffer);
     };
 
+    const uint32_t key_at = Wave::key_address(map, n, h), value_at = Wave::value_address(lane, n, h);
     f32x16 out[RB][VT];
     float base[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
 #pragma unroll
@@ -273,9 +327,9 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
         for (int c = 0; c < VT; ++c) out[i][c] = f32x16{};
     }
 
+    static_assert(PER_T % (PER_T < 4 ? PER_T : 4) == 0, "whole batches");
     if (first < last) load(first, 0);
     for (int stage = first, buffer = 0; stage < last; ++stage, buffer ^= 1) {
-        if constexpr (!DIRECT) put(buffer);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the stage is in LDS, and nobody reads the other one any more
         __syncthreads();
         if (stage + 1 < last) load(stage + 1, buffer ^ 1);
@@ -283,11 +337,12 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
         for (int u = 0; u < SUB; ++u) {
             const int local = (key_wave * SUB + u) * 32, key0 = stage * KT + local;
             if (key0 >= wave_end) break;   // (the same for the wave)
-            const T* lds_k = reinterpret_cast<const T*>(lds + buffer * STAGE) + local * 2 * D;
-            const T* lds_v = lds_k + HALF / sizeof(T);
+            uint32_t lds_k = lds0 + (uint32_t)(buffer * STAGE + local * Tile::ROW), lds_v = lds_k + HALF + value_at;
+            lds_k += key_at;
+            asm volatile("" : "+v"(lds_k), "+v"(lds_v));   // (nothing made of them is kept from one pass to the next)
             f32x16 s[RB];
 #pragma unroll
-            for (int i = 0; i < RB; ++i) s[i] = Wave::scores(lds_k, map, n, h, q[i]);
+            for (int i = 0; i < RB; ++i) s[i] = Wave::scores(lds_k, q[i]);
             if (key0 + 32 > wave_all) {
 #pragma unroll
                 for (int i = 0; i < RB; ++i)
@@ -325,7 +380,7 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
                     sum[i] += s[i][r];
                 }
             }
-            Wave::values(lds_v, n, h, s, out);
+            Wave::values(lds_v, s, out);
         }
     }
 #pragma unroll
@@ -535,8 +590,8 @@ extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t S
     const int64_t workgroups = batch * groups * ceil_div(rows, few ? 32 : bytes <= 128 ? 128 : 64), stages = ceil_div(Sk, keys);
     const int form = tuning().diff_splits;
     if (form > 0) return std::min(form, 256);
-    const int64_t room = 512 / workgroups;   // two workgroups to a CU
-    return std::max((int64_t)1, std::min({room, stages / 2, (int64_t)256}));
+    const int64_t room = (few ? 256 : 512) / workgroups;   // one workgroup to a CU, or two
+    return std::max((int64_t)1, std::min({room, stages / 4, (int64_t)256}));
 }
 
 extern "C" int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1, const float* lambda_k1,
