@@ -77,6 +77,7 @@ static void parse_tuning(Tuning& t) {
     t.attn_few = env_int("MI355X_ATTN_FEW", -1);
     t.qlin_form = env_int("MI355X_QLIN_FORM", -1);
     t.diff_splits = env_int("MI355X_DIFF_SPLITS", 0);
+    t.diff_form = env_int("MI355X_DIFF_FORM", -1);
 }
 
 Tuning tuning() {

@@ -33,7 +33,6 @@ struct DiffArgs {
     int causal, splits;
     int64_t row_blocks;                 // of the rows Sq * share of a slice (one batch entry, one group)
     int per_xcd;                        // slices of an XCD whose blocks take turns; 0: one slice after the other
-    int fold;                           // if causal: all blocks run at once, long ones first, then from short to long
     float scale_log2, lambda_init;
 };
 
@@ -209,8 +208,7 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
     constexpr int PER_T = KT * Tile::PIECES / NT;
     static_assert(KT * Tile::PIECES % NT == 0 && Tile::PIECES <= WAVE, "whole pieces to a thread, whole rows to a transfer");
     constexpr int EXCHANGE = 32 * 2 * D;   // floats of a row block's output
-    static_assert(RW * EXCHANGE * 4 <= 2 * STAGE && (KW == 1 || KW * RW * RB * EXCHANGE * 4 <= 2 * STAGE) && KT * 16 <= STAGE, "room to exchange results");
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[std::max(2 * STAGE, 4 * EXCHANGE * (KW == 1 ? RW : KW * RW * RB))];
 
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int n = lane % 32, h = lane / 32, map = wave % 2, row_wave = wave / 2 % RW, key_wave = wave / (2 * RW);
@@ -227,13 +225,13 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
         split = (int)(rest % p.splits);
         slice = rest / p.splits;
     }
-    const int64_t half = (p.row_blocks + 1) / 2;
-    const int64_t block = !p.causal ? turn : p.fold && turn >= half ? turn - half : p.row_blocks - 1 - turn;
     const int64_t b = slice / p.groups;
     const int group = (int)(slice % p.groups);
     const int64_t rows = p.Sq * p.share, length = diff_length(p, b);
     const int64_t ahead = length - p.Sq;   // if causal, query i sees the keys up to i + ahead
     auto keys_of = [&](int64_t row) { return p.causal ? std::max((int64_t)0, std::min(length, row / p.share + ahead + 1)) : length; };
+
+    const int64_t block = p.causal ? p.row_blocks - 1 - turn : turn;   // long ones first
 
     // ---- queries: row r of a slice is head r % share of query r / share ------------------------------------
     const int64_t row0 = block * ROWS + row_wave * RB * 32;   // of the wave
@@ -341,8 +339,10 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
             lds_k += key_at;
             asm volatile("" : "+v"(lds_k), "+v"(lds_v));   // (nothing made of them is kept from one pass to the next)
             f32x16 s[RB];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < RB; ++i) s[i] = Wave::scores(lds_k, q[i]);
+            __builtin_amdgcn_s_setprio(0);
             if (key0 + 32 > wave_all) {
 #pragma unroll
                 for (int i = 0; i < RB; ++i)
@@ -380,7 +380,9 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
                     sum[i] += s[i][r];
                 }
             }
+            __builtin_amdgcn_s_setprio(1);
             Wave::values(lds_v, s, out);
+            __builtin_amdgcn_s_setprio(0);
         }
     }
 #pragma unroll
@@ -544,14 +546,26 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs p) {
     store_values(static_cast<T*>(p.O) + ((b * p.Sq + row / p.share) * p.heads + head) * 2 * D + lane * PER_LANE, result, PER_LANE);
 }
 
-// How a type and head size are cut: rows of a wave for many rows, keys of a stage, and key waves for few rows.
+// How a type and head size are cut: with many rows RW x RB blocks of 32 and SUB blocks of 32 keys in a stage, by one key wave or WIDE; with few rows one block and KW key waves.
 template <class T, int D>
 struct DiffForm {
     static constexpr int BYTES = D * (int)sizeof(T);   // 64 to 512
     static constexpr int RB = BYTES <= 128 ? 2 : 1, RW = 2, SUB = BYTES <= 128 ? 2 : 1;
-    static constexpr int KW = BYTES <= 128 ? 4 : BYTES <= 256 ? 2 : 1;
+    static constexpr int KW = BYTES <= 128 ? 4 : BYTES <= 256 ? 2 : 1, WIDE = BYTES <= 256 ? 2 : 1;
 };
-constexpr int64_t DIFF_FEW = 32;   // rows of a slice up to which a workgroup has one block of them
+
+// Which form: one block of rows to a workgroup (FEW) up to two workgroups for each CU; then two key waves (WIDE) for a causal mask, whose long and short blocks
+// even out over one workgroup to a CU, and for few workgroups; otherwise one (TALL). Microseconds FEW / TALL / WIDE, bfloat16, 8 heads of 64: 512 queries and keys 11.0 /
+// 21.7 / 20.7; 2048 49 / 68 / 54; 8192 699 / 394 / 441, causal 348 / 277 / 232. float32: 3 x 333 with 6 heads of 64 24.8 / 32.8 / 29.9.
+enum { DIFF_FEW, DIFF_TALL, DIFF_WIDE };
+struct DiffCut { int form; int64_t workgroups, stages; };
+static DiffCut diff_cut(int64_t rows, int64_t slices, int64_t Sk, int bytes, int causal) {
+    const int form = tuning().diff_form;
+    const int64_t few = ceil_div(rows, (int64_t)32) * slices, wide = ceil_div(rows, (int64_t)(bytes <= 128 ? 128 : 64)) * slices;
+    const int pick = form >= 0 ? form : rows <= 32 || (few <= 512 && bytes <= 256) ? DIFF_FEW : causal || wide <= 256 ? DIFF_WIDE : DIFF_TALL;
+    const int64_t keys = bytes > 256 ? 32 : pick == DIFF_FEW && bytes <= 128 ? 128 : 64;
+    return {pick, pick == DIFF_FEW ? few : wide, ceil_div(Sk, keys)};
+}
 
 template <class T, int D>
 static int launch_diff(DiffArgs p, hipStream_t st) {
@@ -565,12 +579,13 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
         grid = p.row_blocks * p.splits * slices;
         if (!grid_fits(grid, 128 * RW * KW)) return;
         p.per_xcd = p.causal && p.splits == 1 && slices % NUM_XCD == 0 ? (int)(slices / NUM_XCD) : 0;
-        p.fold = grid <= 512;
         const dim3 g((unsigned)grid), block(128 * RW * KW);
         if (direct) hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, true>), g, block, 0, st, p);
         else hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, false>), g, block, 0, st, p);
     };
-    if (rows <= DIFF_FEW) launch(Int<1>{}, Int<1>{}, Int<F::KW>{}, Int<1>{});
+    const int form = diff_cut(rows, slices, p.Sk, F::BYTES, p.causal).form;
+    if (form == DIFF_FEW) launch(Int<1>{}, Int<1>{}, Int<F::KW>{}, Int<1>{});
+    else if (form == DIFF_WIDE) launch(Int<F::RB>{}, Int<F::RW>{}, Int<F::WIDE>{}, Int<1>{});
     else launch(Int<F::RB>{}, Int<F::RW>{}, Int<1>{}, Int<F::SUB>{});
     MI355X_REQUIRE(grid_fits(grid, 512), "differential_attention: too large");
     if (p.splits > 1) {
@@ -585,13 +600,12 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
 extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups, int64_t size, int type) {
     using namespace mi355x;
     if (!is_mixed_type(type) || (size != 32 && size != 64 && size != 128) || groups < 1 || heads < 1 || heads % groups || batch < 1 || Sq < 1 || Sk < 1) return 1;
-    const int64_t rows = Sq * (heads / groups), bytes = size * (type == MI355X_TYPE_FLOAT ? 4 : 2);
-    const int64_t few = rows <= DIFF_FEW, keys = few ? (bytes <= 128 ? 128 : bytes <= 256 ? 64 : 32) : bytes <= 128 ? 64 : 32;   // of a stage
-    const int64_t workgroups = batch * groups * ceil_div(rows, few ? 32 : bytes <= 128 ? 128 : 64), stages = ceil_div(Sk, keys);
-    const int form = tuning().diff_splits;
-    if (form > 0) return std::min(form, 256);
-    const int64_t room = (few ? 256 : 512) / workgroups;   // one workgroup to a CU, or two
-    return std::max((int64_t)1, std::min({room, stages / 4, (int64_t)256}));
+    const DiffCut cut = diff_cut(Sq * (heads / groups), batch * groups, Sk, (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2), 0);
+    const int forced = tuning().diff_splits;
+    if (forced > 0) return std::min(forced, 256);
+    // A workgroup to each CU, with four stages at least (8 x 1 of 8192 keys, 16 heads in 4 groups, 64, bfloat16: 97 us in one part, 38 in 4, 31 in 8, 35 in 16); of many rows, whose
+    // sums are joined for 7 us and more, eight (512 of 512 keys, 8 heads: 11.0 us in one part, 18.4 in two; float32, 8 heads of 128, 1024 of 1024 keys: 159 and 104).
+    return std::max((int64_t)1, std::min({256 / cut.workgroups, cut.stages / (Sq * (heads / groups) <= 32 ? 4 : 8), (int64_t)256}));
 }
 
 extern "C" int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1, const float* lambda_k1,

@@ -22,7 +22,7 @@ template <int ACT>
 __device__ __forceinline__ float activated(float v) {
     if (ACT == MI355X_ACT_RELU) return v < 0.0f ? 0.0f : v;
     if (ACT == MI355X_ACT_GELU) return gelu_erf(v);
-    if (ACT == MI355X_ACT_SILU) return v / (1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+    if (ACT == MI355X_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
     return v;
 }
 

@@ -53,14 +53,19 @@ __global__ __launch_bounds__(ROTARY_THREADS) void rotary_positions_kernel(Rotary
         const T* x = static_cast<const T*>(key ? p.k : p.q) + offset;
         T* y = static_cast<T*>(key ? p.k_out : p.q_out) + offset;
         if (step >= turning) {   // values that are not turned, bit by bit
+            typedef typename Values<T, 2 * VEC>::unaligned Vector;
             const int c0 = p.rotated + (step - turning) * 2 * VEC;
-            T v[2 * VEC];
+            if (c0 + 2 * VEC <= p.size) {
+                *reinterpret_cast<Vector*>(y + c0) = *reinterpret_cast<const Vector*>(x + c0);
+            } else {
+                T v[2 * VEC];
 #pragma unroll
-            for (int e = 0; e < 2 * VEC; ++e)
-                if (c0 + e < p.size) v[e] = x[c0 + e];
+                for (int e = 0; e < 2 * VEC; ++e)
+                    if (c0 + e < p.size) v[e] = x[c0 + e];
 #pragma unroll
-            for (int e = 0; e < 2 * VEC; ++e)
-                if (c0 + e < p.size) y[c0 + e] = v[e];
+                for (int e = 0; e < 2 * VEC; ++e)
+                    if (c0 + e < p.size) y[c0 + e] = v[e];
+            }
             continue;
         }
         const int pair = step * VEC;

@@ -45,7 +45,7 @@ from ... import _lib
 from ...sdfg import SDFG, SDFGState, Ptr, Stream, I64Array, U32Array, F32Array, PtrArray, AliasNode
 from ...util.utils import in_desc_with_name, out_desc_with_name, prod
 from ..forward_implementation_abc import ONNXForward
-from .utils import op_implementation, kernel_call_for_node, empty_sdfg_for_node
+from .utils import op_implementation, kernel_call_for_node
 
 IMPLEMENTATION_NAME = "mi355x"
 MAX_ELTWISE_DIMS = 8
@@ -1017,21 +1017,13 @@ class MI355XDifferentialAttention(ONNXForward):
         B, Sq, Sk, H, G, D, vector, scale, kind = MI355XDifferentialAttention._plan(node, state, sdfg)
         splits = _lib.library().mi355x_differential_attention_splits(B, Sq, Sk, H, G, D, kind)
         lengths = "lengths" if _has_input(node, state, "lengths") else None
-        call = kernel_call_for_node(node, state, "mi355x_differential_attention", [
+        if splits > 1:
+            scratch = sdfg.free_name(node.label + "_scratch")
+            sdfg.add_transient(scratch, [splits * B * Sq * H * (4 * D + 4)], dace.float32)
+            state.add_edge(node, "_scratch", state.add_write(scratch), None, sdfg.make_array_memlet(scratch))
+        return kernel_call_for_node(node, state, "mi355x_differential_attention", [
             *(Ptr(c) for c in ("Q", "K", "V", "lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")), Ptr(lengths), Ptr("O"),
             Ptr("_scratch" if splits > 1 else None), B, Sq, Sk, H, G, D, vector, float(node.lambda_init), scale, int(bool(node.causal)), splits, kind, Stream()])
-        if splits == 1:
-            return call
-        nsdfg, nstate, inputs, outputs = empty_sdfg_for_node(sdfg, state, node)
-        nsdfg.add_transient("_scratch", [splits * B * Sq * H * (4 * D + 4)], dace.float32)
-        call.add_out_connector("_scratch")
-        nstate.add_node(call)
-        for side, array in inputs.items():
-            nstate.add_edge(array, None, call, side, nsdfg.make_array_memlet(side))
-        for side, array in outputs.items():
-            nstate.add_edge(call, side, array, None, nsdfg.make_array_memlet(side))
-        nstate.add_edge(call, "_scratch", nstate.add_write("_scratch"), None, nsdfg.make_array_memlet("_scratch"))
-        return nsdfg
 
 
 # ------------------------------------------------------------------------------------

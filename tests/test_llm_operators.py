@@ -69,6 +69,19 @@ def test_nodes_expand_to_one_call(make, function):
     assert f"{function}(" in calls[0].as_cpp()
 
 
+def test_sums_of_splits_are_a_transient_of_the_graph():
+    """Where keys are dealt to several workgroups the graph has an array for their sums, and one to a node."""
+    q, k, v = _z(1, 1, 4, 64, dtype=BF), _z(1, 4096, 4, 64, dtype=BF), _z(1, 4096, 2, 128, dtype=BF)
+    vectors = tuple(_z(8) for _ in range(4))
+    m = _attention(q, k, v, vectors)
+    call, = _functions(m)
+    splits = _lib.library().mi355x_differential_attention_splits(1, 1, 4096, 2, 2, 64, 16)
+    transients = [d for d in m.sdfg.arrays.values() if d.transient]
+    assert splits > 1 and call.args[-4] == 0 and call.args[-3] == splits
+    assert [tuple(d.shape) for d in transients] == [(splits * 2 * (4 * 64 + 4),)] and transients[0].dtype == dace.float32
+    assert not any(d.transient for d in _attention().expand().arrays.values())
+
+
 @pytest.mark.parametrize("make", [
     lambda: _norm(outs="Q"), lambda: _norm(outs="q"), lambda: _norm(gain=_z(3)), lambda: _norm(skip=_z(1, 8)), lambda: _norm(epsilon=-1.0),
     lambda: _norm(epsilon=float("nan")), lambda: _norm(_z(3, 0), _z(0)),

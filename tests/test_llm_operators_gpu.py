@@ -305,6 +305,24 @@ def test_attention_of_few_rows(dtype, d, b, sq, sk, h, g):
     check_attention(b, sq, sk, h, g, d, dtype, lengths=lengths, causal=1)
 
 
+@pytest.mark.parametrize("form", [0, 1, 2])
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("b, sq, sk, h, g", [(1, 3, 40, 2, 1), (2, 150, 129, 2, 2), (8, 130, 300, 1, 1), (1, 70, 260, 4, 1)])
+def test_attention_by_every_kernel(form, dtype, d, causal, b, sq, sk, h, g, tuning):
+    tuning(MI355X_DIFF_FORM=form)
+    check_attention(b, sq, sk, h, g, d, dtype, causal=causal, lengths=[sk - 3 * i for i in range(b)])
+
+
+@pytest.mark.parametrize("splits", [2, 5, 100])
+@pytest.mark.parametrize("sq, sk", [(1, 700), (90, 333)])
+def test_attention_in_any_number_of_parts(splits, sq, sk, tuning):
+    for dtype in R.TYPES:
+        tuning(MI355X_DIFF_SPLITS=splits)
+        check_attention(2, sq, sk, 4, 2, 64, dtype, causal=1, lengths=[sk, sq + 5])
+
+
 @pytest.mark.parametrize("dtype", R.TYPES)
 @pytest.mark.parametrize("causal", [0, 1])
 @pytest.mark.parametrize("sq, sk", [(1, 1500), (70, 100)])
