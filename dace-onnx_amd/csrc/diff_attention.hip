@@ -139,23 +139,63 @@ struct DiffWave {
         return Tile::at(4 * h + row, col / 8) * sizeof(T) + col % 8 * sizeof(T);
     }
 
-    // S^T of 32 keys and 32 rows
-    static __device__ __forceinline__ f32x16 scores(uint32_t lds_k, const Operand<T> (&q)[QP]) {
-        f32x16 acc = {};
+    // use(i, operand) for operands i = 0 .. N - 1, MFMAS products each. Of float32, which takes 44 instructions to split, operand i + 1 is split between the products of
+    // operand i, and operand i + 2 is on its way from LDS: a wave issues in order, and a product holds the matrix unit for the time of seven instructions.
+    template <int N, int MFMAS, class Read, class Use>
+    static __device__ __forceinline__ void each_operand(Read&& fetch, Use&& use) {
+        if constexpr (!std::is_same_v<T, float>) {
+            static_for<N>([&](auto i) __attribute__((always_inline)) {
+                Operand<T> v;
+                fetch(i, v.part[0]);
+                use(i, v);
+            });
+        } else {
+            float x[8];
+            Operand<T> now;
+            fetch(Int<0>{}, x);
+            now.set(x);
+            if constexpr (N > 1) fetch(Int<1>{}, x);
+            static_for<N>([&](auto i) __attribute__((always_inline)) {
+                constexpr int I = decltype(i)::value;
+                float y[8];
+                Operand<T> next;
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (I + 2 < N) fetch(Int<I + 2>{}, y);
+                if constexpr (I + 1 < N) next.set(x);
+                use(i, now);
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);   // LDS reads
+                static_for<MFMAS>([&](auto) __attribute__((always_inline)) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                  // a product
+                    __builtin_amdgcn_sched_group_barrier(0x002, 48 / MFMAS + 1, 0);   // other arithmetic
+                });
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (I + 1 < N) now = next;
+                if constexpr (I + 2 < N) {
 #pragma unroll
-        for (int s = 0; s < QP; ++s) {
-            T v[8];
-#pragma unroll
-            for (int i = 0; i < 8 / E; ++i) {
-                const Piece piece = read<Piece>(lds_k ^ (16 * (16 / E * s + i)), 0);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[i * E + e] = piece[e];
-            }
-            Operand<T> k;
-            k.set(v);
-            Operand<T>::product(k, q[s], acc);
+                    for (int e = 0; e < 8; ++e) x[e] = y[e];
+                }
+            });
         }
-        return acc;
+    }
+
+    // S^T of 32 keys and 32 rows
+    template <int RB>
+    static __device__ __forceinline__ void scores(uint32_t lds_k, const Operand<T> (&q)[RB][QP], f32x16 (&acc)[RB]) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) acc[b] = f32x16{};
+        each_operand<QP, 6 * RB>(
+            [&](auto s, auto& v) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 8 / E; ++i) {
+                    const Piece piece = read<Piece>(lds_k ^ (16 * (16 / E * decltype(s)::value + i)), 0);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[i * E + e] = piece[e];
+                }
+            },
+            [&](auto s, const Operand<T>& k) __attribute__((always_inline)) {
+#pragma unroll
+                for (int b = 0; b < RB; ++b) Operand<T>::product(k, q[b][decltype(s)::value], acc[b]);
+            });
     }
 
     // O^T += V^T P^T over 32 keys; element e of half h of a k-step t is key 16 t + 4 h + e, from e = 4 on four more
@@ -171,25 +211,25 @@ struct DiffWave {
                 for (int e = 0; e < 8; ++e) v[e] = (T)prob[b][8 * t + e];
                 pr[b].set(v);
             }
+            each_operand<VT, 6 * RB>(
+                [&](auto column, auto& v) __attribute__((always_inline)) {
+                    constexpr int c = decltype(column)::value;
+                    if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-            for (int c = 0; c < VT; ++c) {
-                Operand<T> v;
-                if constexpr (std::is_same_v<T, float>) {
-                    float x[8];
+                        for (int e = 0; e < 8; ++e) v[e] = read<float>(lds_v ^ (16 * (8 * c ^ (e % 4) << 2 ^ 2 * (e / 4))), (16 * t + 8 * (e / 4) + e % 4) * Tile::ROW);
+                    } else {
+                        s16x4 half[2];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = read<float>(lds_v ^ (16 * (8 * c ^ (e % 4) << 2 ^ 2 * (e / 4))), (16 * t + 8 * (e / 4) + e % 4) * Tile::ROW);
-                    v.set(x);
-                } else {
-                    s16x4 half[2];
+                        for (int i = 0; i < 2; ++i)
+                            half[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(reinterpret_cast<__attribute__((address_space(3))) char*>(
+                                lds_v ^ (16 * (4 * c ^ 2 * i))) + (16 * t + 8 * i) * Tile::ROW));
+                        v = __builtin_bit_cast(typename Operand<T>::Vector, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+                },
+                [&](auto column, const Operand<T>& v) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        half[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(reinterpret_cast<__attribute__((address_space(3))) char*>(
-                            lds_v ^ (16 * (4 * c ^ 2 * i))) + (16 * t + 8 * i) * Tile::ROW));
-                    v.part[0] = __builtin_bit_cast(typename Operand<T>::Vector, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                }
-#pragma unroll
-                for (int b = 0; b < RB; ++b) Operand<T>::product(v, pr[b], out[b][c]);
-            }
+                    for (int b = 0; b < RB; ++b) Operand<T>::product(v, pr[b], out[b][decltype(column)::value]);
+                });
         }
     }
 };
@@ -340,8 +380,7 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
             asm volatile("" : "+v"(lds_k), "+v"(lds_v));   // (nothing made of them is kept from one pass to the next)
             f32x16 s[RB];
             __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < RB; ++i) s[i] = Wave::scores(lds_k, q[i]);
+            Wave::scores(lds_k, q, s);
             __builtin_amdgcn_s_setprio(0);
             if (key0 + 32 > wave_all) {
 #pragma unroll
