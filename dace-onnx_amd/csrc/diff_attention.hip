@@ -32,7 +32,7 @@ struct DiffArgs {
     int heads, groups, share, vector;   // share = heads / groups; vector: length of the learned vectors
     int causal, splits;
     int64_t row_blocks;                 // of the rows Sq * share of a slice (one batch entry, one group)
-    int per_xcd;                        // slices of an XCD whose blocks take turns; 0: one slice after the other
+    int per_xcd;                        // slices of an XCD whose blocks take turns; 0: one slice after the other; -1: all slices take turns
     float scale_log2, lambda_init;
 };
 
@@ -255,7 +255,11 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
     const int64_t logical = xcd_remap(blockIdx.x, (int64_t)gridDim.x);
     int64_t turn, slice;
     int split = 0;
-    if (p.per_xcd) {
+    if (p.per_xcd < 0) {
+        const int64_t slices = p.batch * p.groups;
+        turn = blockIdx.x / slices;
+        slice = blockIdx.x % slices;
+    } else if (p.per_xcd) {
         const int64_t each = p.row_blocks * p.per_xcd, local = logical % each;
         turn = local / p.per_xcd;
         slice = logical / each * p.per_xcd + local % p.per_xcd;
@@ -585,7 +589,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs p) {
     store_values(static_cast<T*>(p.O) + ((b * p.Sq + row / p.share) * p.heads + head) * 2 * D + lane * PER_LANE, result, PER_LANE);
 }
 
-// How a type and head size are cut: with many rows RW x RB blocks of 32 and SUB blocks of 32 keys in a stage, by one key wave or WIDE; with few rows one block and KW key waves.
+// How a type and head size are cut: with many rows RW x RB blocks of 32 and SUB blocks of 32 keys in a stage; with few rows one block and KW key waves.
 template <class T, int D>
 struct DiffForm {
     static constexpr int BYTES = D * (int)sizeof(T);   // 64 to 512
@@ -593,17 +597,20 @@ struct DiffForm {
     static constexpr int KW = BYTES <= 128 ? 4 : BYTES <= 256 ? 2 : 1, WIDE = BYTES <= 256 ? 2 : 1;
 };
 
-// Which form: one block of rows to a workgroup (FEW) up to two workgroups for each CU; then two key waves (WIDE) for a causal mask, whose long and short blocks
-// even out over one workgroup to a CU, and for few workgroups; otherwise one (TALL). Microseconds FEW / TALL / WIDE, bfloat16, 8 heads of 64: 512 queries and keys 11.0 /
-// 21.7 / 20.7; 2048 49 / 68 / 54; 8192 699 / 394 / 441, causal 348 / 277 / 232. float32: 3 x 333 with 6 heads of 64 24.8 / 32.8 / 29.9.
-enum { DIFF_FEW, DIFF_TALL, DIFF_WIDE };
+// Which form. FEW: one block of rows and KW key waves to a workgroup, one workgroup to a CU; SMALL: half the key waves, two to a CU (small heads); WIDE: many rows by
+// two key waves, one to a CU, where the long and short blocks of a causal mask even out; TALL: by one, two to a CU. Microseconds FEW / SMALL / WIDE / TALL, bfloat16,
+// 8 heads of 64: 512 queries and keys 11.0 / 11.8 / 20.7 / 21.7; 1039 (264 blocks of rows) 34 / 23 / 35 / 41; 1500 43 / 31 / 45 / 54; 2048 49 / - / 54 / 68; 8192 699 / - /
+// 441 / 394, causal 348 / - / 232 / 277. Heads of 128, 1039: 75 / 59 / 40 / 50. float32, heads of 64: 3 x 333 24.8 / - / 29.9 / 32.8, 1039 117 / 102 / 79 / 93.
+enum { DIFF_FEW, DIFF_TALL, DIFF_WIDE, DIFF_SMALL };
 struct DiffCut { int form; int64_t workgroups, stages; };
 static DiffCut diff_cut(int64_t rows, int64_t slices, int64_t Sk, int bytes, int causal) {
-    const int form = tuning().diff_form;
+    const int forced = tuning().diff_form;
     const int64_t few = ceil_div(rows, (int64_t)32) * slices, wide = ceil_div(rows, (int64_t)(bytes <= 128 ? 128 : 64)) * slices;
-    const int pick = form >= 0 ? form : rows <= 32 || (few <= 512 && bytes <= 256) ? DIFF_FEW : causal || wide <= 256 ? DIFF_WIDE : DIFF_TALL;
-    const int64_t keys = bytes > 256 ? 32 : pick == DIFF_FEW && bytes <= 128 ? 128 : 64;
-    return {pick, pick == DIFF_FEW ? few : wide, ceil_div(Sk, keys)};
+    const int form = forced >= 0 && forced <= DIFF_SMALL ? forced : rows <= 32 || (few <= 256 && bytes <= 256) ? DIFF_FEW : few <= 512 && bytes <= 128 ? DIFF_SMALL :
+                     causal || wide <= 256 ? DIFF_WIDE : DIFF_TALL;
+    const bool one_block = form == DIFF_FEW || form == DIFF_SMALL;
+    const int64_t keys = bytes > 256 ? 32 : form == DIFF_FEW && bytes <= 128 ? 128 : form == DIFF_SMALL && bytes > 128 ? 32 : 64;
+    return {form, one_block ? few : wide, ceil_div(Sk, keys)};
 }
 
 template <class T, int D>
@@ -617,13 +624,15 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
         p.row_blocks = ceil_div(rows, (int64_t)(32 * RB * RW));
         grid = p.row_blocks * p.splits * slices;
         if (!grid_fits(grid, 128 * RW * KW)) return;
-        p.per_xcd = p.causal && p.splits == 1 && slices % NUM_XCD == 0 ? (int)(slices / NUM_XCD) : 0;
+        // long blocks of a causal mask first, whichever slice they are of: of the slices whose keys an XCD's L2 holds, or of all
+        p.per_xcd = !p.causal || p.splits > 1 ? 0 : slices % NUM_XCD == 0 ? (int)(slices / NUM_XCD) : -1;
         const dim3 g((unsigned)grid), block(128 * RW * KW);
         if (direct) hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, true>), g, block, 0, st, p);
         else hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, false>), g, block, 0, st, p);
     };
     const int form = diff_cut(rows, slices, p.Sk, F::BYTES, p.causal).form;
     if (form == DIFF_FEW) launch(Int<1>{}, Int<1>{}, Int<F::KW>{}, Int<1>{});
+    else if (form == DIFF_SMALL) launch(Int<1>{}, Int<1>{}, Int<(F::KW > 1 ? F::KW / 2 : 1)>{}, Int<1>{});
     else if (form == DIFF_WIDE) launch(Int<F::RB>{}, Int<F::RW>{}, Int<F::WIDE>{}, Int<1>{});
     else launch(Int<F::RB>{}, Int<F::RW>{}, Int<1>{}, Int<F::SUB>{});
     MI355X_REQUIRE(grid_fits(grid, 512), "differential_attention: too large");
@@ -642,9 +651,18 @@ extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t S
     const DiffCut cut = diff_cut(Sq * (heads / groups), batch * groups, Sk, (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2), 0);
     const int forced = tuning().diff_splits;
     if (forced > 0) return std::min(forced, 256);
-    // A workgroup to each CU, with four stages at least (8 x 1 of 8192 keys, 16 heads in 4 groups, 64, bfloat16: 97 us in one part, 38 in 4, 31 in 8, 35 in 16); of many rows, whose
-    // sums are joined for 7 us and more, eight (512 of 512 keys, 8 heads: 11.0 us in one part, 18.4 in two; float32, 8 heads of 128, 1024 of 1024 keys: 159 and 104).
-    return std::max((int64_t)1, std::min({256 / cut.workgroups, cut.stages / (Sq * (heads / groups) <= 32 ? 4 : 8), (int64_t)256}));
+    // By what a workgroup's stages take, what joining takes (a launch, and the sums written and read), and a workgroup to each CU at most. Measured, microseconds: 8 x 1 of
+    // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 97 in one part, 38 in 4, 31 in 8, 35 in 16; 1 x 1 of them 16.6 in 16, 16.3 in 32, 20 in 64; 16 x 1 of 1000 keys, 8 heads, float16:
+    // 20.1 in one part, 20.7 in 2; 512 of 512, 8 heads: 11.0 and 18.4; float32, 8 heads of 128, 1024 of 1024: 159 and 104.
+    const bool wide = type == MI355X_TYPE_FLOAT;
+    const double stage = wide ? (size == 128 ? 4.5 : 2.3) : 1.3, sums = 16.0 * (double)(batch * Sq * heads) * (double)(2 * size + 2) / 4e6;   // us; of one part
+    int64_t best = 1;
+    double least = stage * (double)cut.stages;
+    for (int64_t n = 2; n <= std::min({256 / cut.workgroups, cut.stages, (int64_t)256}); ++n) {
+        const double cost = stage * (double)ceil_div(cut.stages, n) + 7.0 + (double)n * (0.05 + sums);
+        if (cost < least) least = cost, best = n;
+    }
+    return best;
 }
 
 extern "C" int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1, const float* lambda_k1,

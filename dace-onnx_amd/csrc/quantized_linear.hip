@@ -317,10 +317,12 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
     // (64 x 16384 x 1024: 12.9 us, 64 x 512 x 8192: 20.0); 64 x 64 as much and 2.5 ns for each round and k (7.5 and 20.2). The largest two by their rounds, 40 and 64 us each.
     const int64_t tiles64 = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64), tiles128 = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t tiles256 = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
-    const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    const int64_t rounds16 = ceil_div(ceil_div(p.M, (int64_t)(16 * mt)) * ceil_div(p.N, (int64_t)16), (int64_t)256);
+    int mt = 1;   // rows / 16 of a workgroup, direct
+    auto direct_cost = [&](int rows16) { return ceil_div(ceil_div(p.M, (int64_t)(16 * rows16)) * ceil_div(p.N, (int64_t)16), (int64_t)256) * (rows16 + 1); };
+    for (int rows16 = 2; rows16 <= 4; rows16 *= 2)
+        if (direct_cost(rows16) < direct_cost(mt)) mt = rows16;
     const int form = tuning().qlin_form;
-    const int pick = form >= 0 ? form : rounds16 * (mt + 1) <= 6 * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
+    const int pick = form >= 0 ? form : direct_cost(mt) <= 6 * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
     if (pick == 4) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, Int<2>{}, Int<128>{}, 1);
     else if (pick == 3) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<128>{}, 2);
     else if (pick == 2) tile(Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}, Int<3>{}, Int<128>{}, 1);

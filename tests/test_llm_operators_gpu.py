@@ -305,7 +305,7 @@ def test_attention_of_few_rows(dtype, d, b, sq, sk, h, g):
     check_attention(b, sq, sk, h, g, d, dtype, lengths=lengths, causal=1)
 
 
-@pytest.mark.parametrize("form", [0, 1, 2])
+@pytest.mark.parametrize("form", range(4))
 @pytest.mark.parametrize("dtype", R.TYPES)
 @pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("causal", [0, 1])
