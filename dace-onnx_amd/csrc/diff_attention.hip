@@ -10,7 +10,7 @@
 //     values V's operand comes from LDS by transposing reads, with float32 by 4-byte reads (and is split in three, see Operand). Every lane has one row: a running maximum that
 //     changes is one factor to a lane.
 //   * Keys and values are staged through LDS for all waves, 16-byte pieces permuted within a row so that reads of a column meet no bank twice.
-// P is rounded to the arrays' type for the second product, half a step of it; the sum is that of the values before.
+// P is rounded to the arrays' type for the second product, half a step of it; the sum is that of the rounded values.
 // Few rows: the keys are dealt to `splits` workgroups, whose maxima, sums and outputs a second launch joins.
 #include "mixed.h"
 #include "gemm_tile.h"
@@ -88,6 +88,16 @@ struct Operand {
 #pragma unroll
         for (int e = 0; e < 8; ++e) part[0][e] = v[e];
     }
+    // sum + the eight values as they are rounded, two to an instruction
+    __device__ __forceinline__ void add_to(float& sum, const T (&)[8]) const {
+        typedef T Pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const Pair two = {part[0][e], part[0][e + 1]};
+            if constexpr (std::is_same_v<T, f16>) sum = __builtin_amdgcn_fdot2(two, Pair{(T)1.0f, (T)1.0f}, sum, false);
+            else sum = __builtin_amdgcn_fdot2_f32_bf16(two, Pair{(T)1.0f, (T)1.0f}, sum, false);
+        }
+    }
     static __device__ __forceinline__ void product(const Operand& a, const Operand& b, f32x16& acc) {
         if constexpr (std::is_same_v<T, f16>) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.part[0], b.part[0], acc, 0, 0, 0);
         else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.part[0], b.part[0], acc, 0, 0, 0);
@@ -109,6 +119,10 @@ struct Operand<float> {
                 for (int j = 0; j < 2; ++j) x[j] -= __builtin_bit_cast(float, bits[j] & 0xffff0000u);
             }
         }
+    }
+    __device__ __forceinline__ void add_to(float& sum, const float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += v[e];
     }
     static __device__ __forceinline__ void product(const Operand& a, const Operand& b, f32x16& acc) {
         auto one = [&](int i, int j) __attribute__((always_inline)) {
@@ -198,9 +212,9 @@ struct DiffWave {
             });
     }
 
-    // O^T += V^T P^T over 32 keys; element e of half h of a k-step t is key 16 t + 4 h + e, from e = 4 on four more
+    // O^T += V^T P^T and the lane's share of the rows' sums of P over 32 keys; element e of half h of a k-step t is key 16 t + 4 h + e, from e = 4 on four more
     template <int RB>
-    static __device__ __forceinline__ void values(uint32_t lds_v, const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT]) {
+    static __device__ __forceinline__ void values(uint32_t lds_v, const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             Operand<T> pr[RB];
@@ -210,6 +224,7 @@ struct DiffWave {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = (T)prob[b][8 * t + e];
                 pr[b].set(v);
+                pr[b].add_to(sum[b], v);
             }
             each_operand<VT, 6 * RB>(
                 [&](auto column, auto& v) __attribute__((always_inline)) {
@@ -418,13 +433,10 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
             for (int i = 0; i < RB; ++i) {
                 const float from = base[i] == -__builtin_inff() ? 0.0f : base[i];   // no key so far: exp2(-inf)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from));
-                    sum[i] += s[i][r];
-                }
+                for (int r = 0; r < 16; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from));
             }
             __builtin_amdgcn_s_setprio(1);
-            Wave::values(lds_v, s, out);
+            Wave::values(lds_v, s, out, sum);
             __builtin_amdgcn_s_setprio(0);
         }
     }
