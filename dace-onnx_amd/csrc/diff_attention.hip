@@ -615,10 +615,11 @@ struct DiffForm {
 // 441 / 394, causal 348 / - / 232 / 277. Heads of 128, 1039: 75 / 59 / 40 / 50. float32, heads of 64: 3 x 333 24.8 / - / 29.9 / 32.8, 1039 117 / 102 / 79 / 93.
 enum { DIFF_FEW, DIFF_TALL, DIFF_WIDE, DIFF_SMALL };
 struct DiffCut { int form; int64_t workgroups, stages; };
-static DiffCut diff_cut(int64_t rows, int64_t slices, int64_t Sk, int bytes, int causal) {
+static DiffCut diff_cut(int64_t rows, int64_t slices, int64_t Sk, int bytes, int causal, bool in_parts) {
     const int forced = tuning().diff_form;
     const int64_t few = ceil_div(rows, (int64_t)32) * slices, wide = ceil_div(rows, (int64_t)(bytes <= 128 ? 128 : 64)) * slices;
-    const int form = forced >= 0 && forced <= DIFF_SMALL ? forced : rows <= 32 || (few <= 256 && bytes <= 256) ? DIFF_FEW : few <= 512 && bytes <= 128 ? DIFF_SMALL :
+    const int form = forced >= 0 && forced <= DIFF_SMALL ? forced : rows <= 32 && in_parts && bytes <= 128 ? DIFF_SMALL : rows <= 32 || (few <= 256 && bytes <= 256) ? DIFF_FEW :
+                     few <= 512 && bytes <= 128 ? DIFF_SMALL :
                      causal || wide <= 256 ? DIFF_WIDE : DIFF_TALL;
     const bool one_block = form == DIFF_FEW || form == DIFF_SMALL;
     const int64_t keys = bytes > 256 ? 32 : form == DIFF_FEW && bytes <= 128 ? 128 : form == DIFF_SMALL && bytes > 128 ? 32 : 64;
@@ -642,7 +643,7 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
         if (direct) hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, true>), g, block, 0, st, p);
         else hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, false>), g, block, 0, st, p);
     };
-    const int form = diff_cut(rows, slices, p.Sk, F::BYTES, p.causal).form;
+    const int form = diff_cut(rows, slices, p.Sk, F::BYTES, p.causal, p.splits > 1).form;
     if (form == DIFF_FEW) launch(Int<1>{}, Int<1>{}, Int<F::KW>{}, Int<1>{});
     else if (form == DIFF_SMALL) launch(Int<1>{}, Int<1>{}, Int<(F::KW > 1 ? F::KW / 2 : 1)>{}, Int<1>{});
     else if (form == DIFF_WIDE) launch(Int<F::RB>{}, Int<F::RW>{}, Int<F::WIDE>{}, Int<1>{});
@@ -660,18 +661,21 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
 extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups, int64_t size, int type) {
     using namespace mi355x;
     if (!is_mixed_type(type) || (size != 32 && size != 64 && size != 128) || groups < 1 || heads < 1 || heads % groups || batch < 1 || Sq < 1 || Sk < 1) return 1;
-    const DiffCut cut = diff_cut(Sq * (heads / groups), batch * groups, Sk, (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2), 0);
+    const int64_t rows = Sq * (heads / groups), slices = batch * groups;
+    const int bytes = (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2);
+    const DiffCut whole = diff_cut(rows, slices, Sk, bytes, 0, false), part = diff_cut(rows, slices, Sk, bytes, 0, true);
     const int forced = tuning().diff_splits;
     if (forced > 0) return std::min(forced, 256);
-    // By what a workgroup's stages take, what joining takes (a launch, and the sums written and read), and a workgroup to each CU at most. Measured, microseconds: 8 x 1 of
-    // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 97 in one part, 38 in 4, 31 in 8, 35 in 16; 1 x 1 of them 16.6 in 16, 16.3 in 32, 20 in 64; 16 x 1 of 1000 keys, 8 heads, float16:
-    // 20.1 in one part, 20.7 in 2; 512 of 512, 8 heads: 11.0 and 18.4; float32, 8 heads of 128, 1024 of 1024: 159 and 104.
-    const bool wide = type == MI355X_TYPE_FLOAT;
-    const double stage = wide ? (size == 128 ? 4.5 : 2.3) : 1.3, sums = 16.0 * (double)(batch * Sq * heads) * (double)(2 * size + 2) / 4e6;   // us; of one part
+    // By what a workgroup's stages take, what joining takes (a launch, and the sums written and read), and one round of workgroups at most. Measured, microseconds: 8 x 1 of
+    // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 97 in one part (FEW), 34 in 8, 30 in 16, 36 in 32 (SMALL); 1 x 1 of them 18.2 in 16, 16.1 in 32, 19.6 in 64; 16 x 1 of 1000 keys, 8 heads,
+    // float16: 20.7 in one part, 21.7 in 2, 20.0 in 4; 512 of 512, 8 heads: 11.0 and 18.4; float32, 8 heads of 128, 1024 of 1024: 159 and 104.
+    auto stage = [&](const DiffCut& c) { return type == MI355X_TYPE_FLOAT ? (size == 128 ? 4.5 : 2.3) : c.form == DIFF_SMALL ? 1.0 : 1.3; };   // us
+    const double sums = 16.0 * (double)(batch * Sq * heads) * (double)(2 * size + 2) / 4e6;                                                  // of one part
+    const int64_t room = (part.form == DIFF_SMALL ? 512 : 256) / part.workgroups;
     int64_t best = 1;
-    double least = stage * (double)cut.stages;
-    for (int64_t n = 2; n <= std::min({256 / cut.workgroups, cut.stages, (int64_t)256}); ++n) {
-        const double cost = stage * (double)ceil_div(cut.stages, n) + 7.0 + (double)n * (0.05 + sums);
+    double least = stage(whole) * (double)whole.stages;
+    for (int64_t n = 2; n <= std::min({room, part.stages, (int64_t)256}); ++n) {
+        const double cost = stage(part) * (double)ceil_div(part.stages, n) + 7.0 + (double)n * (0.1 + sums);
         if (cost < least) least = cost, best = n;
     }
     return best;
