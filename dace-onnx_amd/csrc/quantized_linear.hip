@@ -125,9 +125,7 @@ __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
 // 16 bytes to a lane from global memory, base + the lane's offset, into LDS at lds + 16 lane; base and lds are the same for the wave, all 16-byte aligned.
 // Written as assembly because the compiler waits for every builtin transfer before the next LDS read.
 __device__ __forceinline__ void qlin_to_lds(const int8_t* base, uint32_t offset, uint32_t lds) {
-    const uint64_t b = reinterpret_cast<uint64_t>(base);
-    const uint64_t uniform = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(base) : "memory");
 }
 
 // Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, NS stages. A row's 128 bytes of a step are eight
@@ -149,29 +147,34 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     tile_coords(xcd_remap(blockIdx.x, p.tiles_m * p.tiles_n), p.tiles_m, p.tiles_n, group_m, tm, tn);
     const int64_t m0 = tm * BM, n0 = tn * BN;
 
-    // rows past the end are the last row again; what they give is not stored
-    const int8_t* base[PER_WAVE];
+    // Transfer i of a wave is of X for i below X_COUNT, of W otherwise: a pointer that is the same for the wave and 32 bits of offset to a lane (64 bits to a lane take the
+    // memory path several times as long). Rows past the end are the last row again; what they give is not stored.
+    constexpr int X_COUNT = BM / RPT / NW;
+    static_assert(BM / RPT % NW == 0, "a transfer is of one operand for all waves");
+    const int8_t *x_tile = p.X + m0 * p.K, *w_tile = p.W + n0 * p.K;
     uint32_t offset[PER_WAVE];
     int piece[PER_WAVE];
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i) {
-        const int first = RPT * (wave + i * NW);
-        const bool is_x = first < BM;
-        const int64_t r0 = is_x ? m0 : n0, count = is_x ? p.M : p.N, r = (is_x ? first : first - BM) + lane / PPR;
-        base[i] = (is_x ? p.X : p.W) + r0 * p.K;
+        const int first = RPT * (wave + i * NW), r = (i < X_COUNT ? first : first - BM) + lane / PPR;
+        const int64_t left = i < X_COUNT ? p.M - m0 : p.N - n0;
         piece[i] = (lane % PPR) ^ place(first + lane / PPR);
-        offset[i] = (uint32_t)((r0 + r < count ? r : count - 1 - r0) * p.K) + 16u * (uint32_t)piece[i];
+        offset[i] = (uint32_t)((r < left ? r : left - 1) * p.K) + 16u * (uint32_t)piece[i];
     }
+    auto base = [&](int i, int64_t step) __attribute__((always_inline)) {
+        const uint64_t at = reinterpret_cast<uint64_t>((i < X_COUNT ? x_tile : w_tile) + step * BK);
+        return reinterpret_cast<const int8_t*>(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at));
+    };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
     const int64_t whole = DIRECT ? p.K / BK : 0, steps = (p.K + BK - 1) / BK;
     typedef i32x4 Held[PER_WAVE];
     auto fetch = [&](int64_t step, Held& to) __attribute__((always_inline)) {   // by registers
         if ((step + 1) * BK <= p.K) {
 #pragma unroll
-            for (int i = 0; i < PER_WAVE; ++i) to[i] = *reinterpret_cast<const UnalignedBytes*>(base[i] + step * BK + offset[i]);
+            for (int i = 0; i < PER_WAVE; ++i) to[i] = *(const __attribute__((address_space(1))) UnalignedBytes*)(base(i, step) + offset[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < PER_WAVE; ++i) to[i] = row_bytes(base[i] + step * BK + offset[i], p.K - step * BK - 16 * piece[i], p.K);
+            for (int i = 0; i < PER_WAVE; ++i) to[i] = row_bytes((i < X_COUNT ? x_tile : w_tile) + step * BK + offset[i], p.K - step * BK - 16 * piece[i], p.K);
         }
     };
     auto put = [&](int stage, const Held& v) __attribute__((always_inline)) {
@@ -181,7 +184,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     auto load = [&](int64_t step, int stage) __attribute__((always_inline)) {
         if (step < whole) {
 #pragma unroll
-            for (int i = 0; i < PER_WAVE; ++i) qlin_to_lds(base[i] + step * BK, offset[i], lds0 + (uint32_t)(stage * STAGE + (wave + i * NW) * 1024));
+            for (int i = 0; i < PER_WAVE; ++i) qlin_to_lds(base(i, step), offset[i], lds0 + (uint32_t)(stage * STAGE + (wave + i * NW) * 1024));
         } else if (step < steps) {
             Held part;
             fetch(step, part);
@@ -315,6 +318,7 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
     // 4: 7.1 / 13.9 / 20 / 25 / 47; 64: 12.9 / 13.9 / 20 / 26 / 50; 128: 22 / 13.8 / 20 / 26 / 51; 512: 75 / 16.6 / 21.1 / 26 / 50; 1024: 151 / 31 / 26.0 / 29 / 51;
     // 2048: 281 / 70 / 50 / 40 / 58; 8192 x 8192: 2239 / 439 / - / 317 / 256. Direct takes 3.5 us and 0.42 ns for each round of workgroups, k and 16 rows or columns of one
     // (64 x 16384 x 1024: 12.9 us, 64 x 512 x 8192: 20.0); 64 x 64 as much and 2.5 ns for each round and k (7.5 and 20.2). The largest two by their rounds, 40 and 64 us each.
+    // Rows at other addresses, whose bytes wait in registers: 5923 x 4002 x 1206 100 / 65 / 117 / 80, 1134 x 15690 x 3927 251 / 161 / 278 / 217 (64 x 64 / 128 x 128 one to a CU / two / 256 x 256).
     const int64_t tiles64 = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64), tiles128 = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t tiles256 = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
     int mt = 1;   // rows / 16 of a workgroup, direct
@@ -322,7 +326,7 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
     for (int rows16 = 2; rows16 <= 4; rows16 *= 2)
         if (direct_cost(rows16) < direct_cost(mt)) mt = rows16;
     const int form = tuning().qlin_form;
-    const int pick = form >= 0 ? form : direct_cost(mt) <= 6 * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
+    const int pick = form >= 0 ? form : direct_cost(mt) <= 6 * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 || !aligned ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
     if (pick == 4) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, Int<2>{}, Int<128>{}, 1);
     else if (pick == 3) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<128>{}, 2);
     else if (pick == 2) tile(Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}, Int<3>{}, Int<128>{}, 1);
