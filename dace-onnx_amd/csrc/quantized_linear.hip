@@ -1,6 +1,9 @@
 // QuantizedLinear: Y = act(xs[m] ws[n] sum_k X[m,k] W[n,k] + b[n]) + R[m,n]; X and W in int8, both k-contiguous (W as a linear layer keeps it), Y, b
 // and R in float32, float16 or bfloat16. The sums are int32 and exact (K below 2^17), everything behind them float32, rounded once. The reference has
 // no such node: it runs MatMulInteger, a Cast, two Muls and the rest one after the other.
+// Bound by the matrix unit in tiles: 8192 x 8192 x 4096 256 us (2.15 POP/s; the vendor's int8 product alone 258 to 271, 2.03 to 2.13), of which the results' way out is 43;
+// its loop runs at 2.6 POP/s, where the operands' reads from LDS (six of 1 KB for eight products of a wave) take as long as the products. Few rows by the
+// weights' way in: 4 x 4096 x 4096 6.1 us, 2.7 TB/s, of which 3.5 do not depend on the size.
 #include "mixed.h"
 #include "gemm_tile.h"
 

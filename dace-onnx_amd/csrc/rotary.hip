@@ -4,7 +4,10 @@
 //
 // An angle is an integer position times a float32 frequency: exact in float64, where it is brought into one turn too. Positions far into a context
 // are thousands of turns, of which float32 would leave few right digits (position 100000: 0.004 radians). Cosine and sine of what is left are float32.
-// A workgroup has a few tokens: their angles are computed once, into LDS, and then serve all heads. Bound by the bytes of the heads.
+// A workgroup has a few tokens: their angles are computed once, into LDS, and then serve all heads. Four tokens keep enough loads of a thread in flight and leave the
+// angles' float64 hidden behind other workgroups' bytes. Bound by the bytes of the heads: 32768 tokens of 16 + 4 heads of 128 in bfloat16 61 us, 5.5 TB/s (a copy of 1
+// GiB 5.1); 4616 tokens of 12 heads of 64, 48 of them turned, in float32 7.6 us. One token to a request, 8 x 40 heads: 4.4 us, the launch and one chain of
+// position, angle, head.
 #include "mixed.h"
 
 #include <algorithm>
