@@ -70,13 +70,15 @@ __device__ __forceinline__ uint32_t threads_max(uint32_t v, uint32_t* part) {
 }
 
 // What the squares are taken of: squares of values from 2^64 on do not fit float32, those below 2^-63 are lost. Where that matters the row is
-// summed again, scaled by a power of two.
-constexpr float RMS_UP = 0x1p64f, RMS_DOWN = 0x1p-64f;
+// summed again, scaled by a power of two: 2^31 squares of the largest values times 2^-96 stay below 2^96, those of rows whose mean square is below 2^-80
+// times 2^88 below 2^127, and the least value above zero is then 2^-61.
+constexpr float RMS_UP = 0x1p88f, RMS_DOWN = 0x1p-96f;
 __device__ __forceinline__ float rms_rescale(float mean_square, float eps) {
     if (mean_square == __builtin_inff()) return RMS_DOWN;
     return mean_square < 0x1p-80f && eps < 0x1p-60f ? RMS_UP : 1.0f;
 }
-__device__ __forceinline__ float rms_factor(float mean_square, float eps, float scale) { return scale / sqrtf(mean_square + eps * scale * scale); }
+// what the values times that power of two are multiplied by
+__device__ __forceinline__ float rms_factor(float mean_square, float eps, float scale) { return 1.0f / sqrtf(mean_square + eps * scale * scale); }
 
 // The scale of a row whose largest |y| has the bits `most`, and what y is multiplied by, twice, to become q: one factor would leave float32's
 // range for the smallest rows. Bits from those of infinity on: not every value is finite.
@@ -148,7 +150,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void rms_norm_rows(RmsArgs p) 
         load_values(g, static_cast<const T*>(p.gain) + (t + j * TH) * E, cols - (t + j * TH) * E);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            v[j][e] = v[j][e] * factor * g[e];
+            v[j][e] = v[j][e] * scale * factor * g[e];
             const bool inside = (t + j * TH) * E + e < cols;   // (0 times an infinite factor outside)
             const uint32_t bits = inside ? __builtin_bit_cast(uint32_t, v[j][e]) & 0x7fffffffu : 0u;
             most = most > bits ? most : bits;
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long(RmsArgs p) {
     const float factor = rms_factor(mean, p.eps, scale);
     uint32_t most = 0;
     for (int64_t c = threadIdx.x; c < p.cols; c += TH) {
-        const float s = value(c), y = s * factor * (float)gain[c];
+        const float s = value(c), y = s * scale * factor * (float)gain[c];
         const uint32_t bits = __builtin_bit_cast(uint32_t, y) & 0x7fffffffu;
         most = most > bits ? most : bits;
         if (p.Sum) static_cast<T*>(p.Sum)[row * p.cols + c] = (T)s;
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long(RmsArgs p) {
     }
     if (p.Q) {
         const RowScale s = row_scale(threads_max<TH>(most, part_max));
-        for (int64_t c = threadIdx.x; c < p.cols; c += TH) p.Q[row * p.cols + c] = eight_bits(value(c) * factor * (float)gain[c], s);
+        for (int64_t c = threadIdx.x; c < p.cols; c += TH) p.Q[row * p.cols + c] = eight_bits(value(c) * scale * factor * (float)gain[c], s);
         if (threadIdx.x == 0) p.q_scale[row] = s.scale;
     }
 }

@@ -98,6 +98,18 @@ def test_norm_of_extreme_rows(columns):
             assert y[4].isnan().all()
 
 
+@pytest.mark.parametrize("columns", [40, 300, 16000, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_norm_of_rows_at_the_ends_of_the_exponents(columns, dtype):
+    """Rows whose values are the largest that there are, one such value among ones, and the smallest."""
+    x = normal(6, 4, columns).clamp(-3.9, 3.9)
+    x = torch.stack([x[0].sign() * torch.finfo(dtype).max, x[1] * 2.0 ** 126, x[2], x[3] * 2.0 ** -130]).to(dtype)
+    x[2, 7] = -torch.finfo(dtype).max
+    gain = normal(7, columns, dtype=dtype)
+    y, q, scale = R.call("SkipRMSNormalization", [("x", x), ("g", gain), ("skip", None)], [("y", dtype, x.shape), None, ("q", torch.int8, x.shape), ("qs", F32, (4,))], epsilon=0.0)
+    check_norm(x, gain, None, y, None, q, scale, 0.0)
+
+
 @pytest.mark.parametrize("dtype", R.TYPES)
 @pytest.mark.parametrize("columns", [5, 24, 777, 9000])
 def test_norm_at_any_address_and_over_its_input(dtype, columns):
