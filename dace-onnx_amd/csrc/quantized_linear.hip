@@ -20,11 +20,13 @@ struct QLinArgs {
     int64_t tiles_m, tiles_n;
 };
 
-// NaN stays NaN
-template <int ACT>
+// NaN stays NaN. Silu of 16-bit results with one reciprocal and one power of two, off by |v| 2^-24 of the result where v is negative: 2^-17 at most before it vanishes.
+// float32 results by the library's exponential and a division.
+template <class T, int ACT>
 __device__ __forceinline__ float activated(float v) {
     if (ACT == MI355X_ACT_RELU) return v < 0.0f ? 0.0f : v;
     if (ACT == MI355X_ACT_GELU) return gelu_erf(v);
+    if (ACT == MI355X_ACT_SILU && std::is_same_v<T, float>) return v / (1.0f + expf(-v));
     if (ACT == MI355X_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
     return v;
 }
@@ -57,7 +59,7 @@ __device__ __forceinline__ void qlin_store(const QLinArgs& p, Row&& row, Column&
             for (int e = 0; e < 4; ++e) {
                 v[e] = (float)acc(r, g, e) * xs[r] * ws[g][e];
                 if (p.bias) v[e] += b[g][e];
-                v[e] = activated<ACT>(v[e]);
+                v[e] = activated<T, ACT>(v[e]);
                 if (p.residual) v[e] += res[r][g][e];
             }
             store_values(static_cast<T*>(p.Y) + row(r) * p.N + column(g), v, row(r) < p.M ? p.N - column(g) : 0);
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[e] = activated<ACT>(sum[e] * ws[e] + bias[e]);
+                    v[e] = activated<T, ACT>(sum[e] * ws[e] + bias[e]);
                     if (p.residual) v[e] += res[i][e];
                 }
                 store_values(static_cast<T*>(p.Y) + (m + row) * p.N + n, v, m + row < p.M ? left : 0);

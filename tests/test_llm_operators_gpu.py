@@ -180,6 +180,20 @@ def test_linear_with_one_scale_and_more_dimensions():
     within(y.reshape(6, 50), expected, linear_bound(size, expected, F32))
 
 
+@pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("dtype", R.TYPES)
+def test_linear_small_results_of_silu(m, dtype):
+    """Silu of -1 to -87, exact before it, with errors relative to the results: in float32 of the exponential, the sum and the division 2 U each, in 16 bits |v| U more."""
+    n, k = 88, 32
+    x, w = torch.full((m, k), -1, dtype=torch.int8, device="cuda"), torch.zeros(n, k, dtype=torch.int8, device="cuda")
+    w[:, 0] = torch.arange(n)
+    one = torch.ones(1, device="cuda")
+    y, = R.call("QuantizedLinear", [("x", x), ("w", w), ("xs", one), ("ws", one)], [("y", dtype, (m, n))], activation="silu", to=R.ELEMENT[dtype])
+    v = -torch.arange(n).cuda().double().expand(m, n)
+    expected = v / (1 + torch.exp(-v))
+    within(y, expected, ((8 + (0 if dtype == F32 else 2) * v.abs()) * U + R.HALF[dtype]) * expected.abs() + TINY[dtype])
+
+
 @pytest.mark.parametrize("m", [2, 40, 300])
 def test_linear_largest_sums_and_scales_that_are_not_numbers(m):
     k = (1 << 17) - 1
