@@ -382,6 +382,21 @@ def test_attention_of_far_scores(dtype):
         within(o, expected, attention_bound(q, k, size, expected, 0.125, 8))
 
 
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("sq", [1, 40])
+@pytest.mark.parametrize("first", [0, 777, 19999])
+def test_attention_of_many_keys_of_little_weight(dtype, sq, first):
+    """One key has nearly all of the weight and no value, 19999 others share 2^-9 of it. (Scores are exact, 0 and 16.)"""
+    b, sk, h, d = 1, 20000, 2, 64
+    q, k, v = normal(1, b, sq, 2 * h, d, dtype=dtype), torch.zeros(b, sk, 2, d, dtype=dtype, device="cuda"), normal(3, b, sk, 1, 2 * d, dtype=dtype).abs()
+    q[..., 0] = 2.0 ** 4
+    k[:, first, :, 0], v[:, first] = 1.0, 0.0
+    vectors = [normal(4 + i, 8, scale=0.3) for i in range(4)]
+    expected, size = R.differential_attention(q, k, v, vectors, 0.4, 1.0)
+    o, = R.call("DifferentialAttention", [("q", q), ("k", k), ("v", v)] + [(f"l{i}", w) for i, w in enumerate(vectors)], [("o", dtype, (b, sq, h, 2 * d))], lambda_init=0.4, scale=1.0)
+    within(o, expected, attention_bound(q, k, size, expected, 1.0, 8))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("sq, splits", [(5, 1), (5, 3), (1, 7), (5, 256)])
 def test_attention_at_any_address_and_any_splits(dtype, sq, splits):
