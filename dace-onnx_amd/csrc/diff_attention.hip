@@ -638,12 +638,13 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
     using F = DiffForm<T, D>;
     const int64_t rows = p.Sq * p.share, slices = p.batch * p.groups;
     const bool direct = ((reinterpret_cast<uintptr_t>(p.K) | reinterpret_cast<uintptr_t>(p.V)) & 15) == 0 && (int64_t)p.groups * D < 1 << 20;
-    int64_t grid = 0;
+    bool fits = true;
     auto launch = [&](auto rb, auto rw, auto kw, auto sub) {
         constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value;
         p.row_blocks = ceil_div(rows, (int64_t)(32 * RB * RW));
-        grid = p.row_blocks * p.splits * slices;
-        if (!grid_fits(grid, 128 * RW * KW)) return;
+        const int64_t grid = p.row_blocks * p.splits * slices;
+        fits = grid_fits(grid, 128 * RW * KW) && (p.splits == 1 || grid_fits(ceil_div(slices * rows, (int64_t)4), 256));
+        if (!fits) return;
         // long blocks of a causal mask first, whichever slice they are of: of the slices whose keys an XCD's L2 holds, or of all
         p.per_xcd = !p.causal || p.splits > 1 ? 0 : slices % NUM_XCD == 0 ? (int)(slices / NUM_XCD) : -1;
         const dim3 g((unsigned)grid), block(128 * RW * KW);
@@ -655,7 +656,7 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
     else if (form == DIFF_SMALL) launch(Int<1>{}, Int<1>{}, Int<(F::KW > 1 ? F::KW / 2 : 1)>{}, Int<1>{});
     else if (form == DIFF_WIDE) launch(Int<F::RB>{}, Int<F::RW>{}, Int<F::WIDE>{}, Int<1>{});
     else launch(Int<F::RB>{}, Int<F::RW>{}, Int<1>{}, Int<F::SUB>{});
-    MI355X_REQUIRE(grid_fits(grid, 512), "differential_attention: too large");
+    MI355X_REQUIRE(fits, "differential_attention: too large");
     if (p.splits > 1) {
         const int64_t all = slices * rows;
         hipLaunchKernelGGL((diff_join_kernel<T, D>), dim3((unsigned)ceil_div(all, (int64_t)4)), dim3(256), 0, st, p);
@@ -663,11 +664,17 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
     return check_launch("diff_attention_kernel");
 }
 
+// whether products of them fit 64 bits, and keys with the stage that they end in 32
+static bool diff_fits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups) {
+    return Sq < (int64_t)1 << 31 && Sk < ((int64_t)1 << 31) - 256 && heads < 1 << 20 && batch < (int64_t)1 << 31 && (double)batch * Sq * heads < 0x1p40 &&
+           (double)batch * Sk * groups < 0x1p40;
+}
+
 }  // namespace mi355x
 
 extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups, int64_t size, int type) {
     using namespace mi355x;
-    if (!is_mixed_type(type) || (size != 32 && size != 64 && size != 128) || groups < 1 || heads < 1 || heads % groups || batch < 1 || Sq < 1 || Sk < 1) return 1;
+    if (!is_mixed_type(type) || (size != 32 && size != 64 && size != 128) || groups < 1 || heads < 1 || heads % groups || batch < 1 || Sq < 1 || Sk < 1 || !diff_fits(batch, Sq, Sk, heads, groups)) return 1;
     const int64_t rows = Sq * (heads / groups), slices = batch * groups;
     const int bytes = (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2);
     const DiffCut whole = diff_cut(rows, slices, Sk, bytes, 0, false), part = diff_cut(rows, slices, Sk, bytes, 0, true);
@@ -702,7 +709,7 @@ extern "C" int mi355x_differential_attention(const void* Q, const void* K, const
     if (batch == 0 || Sq == 0 || heads == 0) return MI355X_OK;
     MI355X_REQUIRE(Q && O && (Sk == 0 || (K && V)) && (vector == 0 || (lambda_q1 && lambda_k1 && lambda_q2 && lambda_k2)), "differential_attention: null pointer");
     MI355X_REQUIRE(splits == 1 || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0), "differential_attention: splits need scratch memory, 16-byte aligned");
-    MI355X_REQUIRE(Sq < (int64_t)1 << 31 && Sk < (int64_t)1 << 31 && heads < 1 << 20 && vector < 1 << 20 && batch < (int64_t)1 << 31, "differential_attention: too large");
+    MI355X_REQUIRE(diff_fits(batch, Sq, Sk, heads, groups) && vector < 1 << 20, "differential_attention: too large");
     DiffArgs p = {};
     p.Q = Q; p.K = K; p.V = V; p.O = O; p.q1 = lambda_q1; p.k1 = lambda_k1; p.q2 = lambda_q2; p.k2 = lambda_k2; p.lengths = lengths;
     p.batch = batch; p.Sq = Sq; p.Sk = Sk; p.heads = (int)heads; p.groups = (int)groups; p.share = (int)(heads / groups); p.vector = (int)vector;

@@ -147,7 +147,9 @@ ATTENTION = dict(Q=P, K=P, V=P, q1=P, k1=P, q2=P, k2=P, lengths=P, O=P, scratch=
     ("mi355x_differential_attention", ATTENTION, dict(scale=float("nan")), "scale"), ("mi355x_differential_attention", ATTENTION, dict(splits=0), "splits"),
     ("mi355x_differential_attention", ATTENTION, dict(splits=2, scratch=None), "scratch"), ("mi355x_differential_attention", ATTENTION, dict(splits=2, scratch=P + 4), "scratch"),
     ("mi355x_differential_attention", ATTENTION, dict(V=None), "null"), ("mi355x_differential_attention", ATTENTION, dict(q1=None), "null"),
-    ("mi355x_differential_attention", ATTENTION, dict(Sk=1 << 31), "too large"), ("mi355x_differential_attention", ATTENTION, dict(batch=1 << 20, Sq=1 << 16), "too large"),
+    ("mi355x_differential_attention", ATTENTION, dict(Sk=1 << 31), "too large"),
+    ("mi355x_differential_attention", ATTENTION, dict(Sk=(1 << 31) - 1), "too large"), ("mi355x_differential_attention", ATTENTION, dict(batch=1 << 30, Sq=1 << 30, heads=16, groups=16), "too large"),
+    ("mi355x_differential_attention", ATTENTION, dict(batch=1 << 26, splits=256), "too large"), ("mi355x_differential_attention", ATTENTION, dict(batch=1 << 20, Sq=1 << 16), "too large"),
     ("mi355x_differential_attention", ATTENTION, dict(type=2), "element type"), ("mi355x_differential_attention", ATTENTION, dict(batch=-1), "negative")])
 def test_calls_that_are_refused(name, base, change, message):
     status, error = _status(name, *{**base, **change}.values())
@@ -161,6 +163,13 @@ def test_calls_that_are_refused(name, base, change, message):
     ("mi355x_differential_attention", ATTENTION, dict(batch=0)), ("mi355x_differential_attention", ATTENTION, dict(Sq=0)), ("mi355x_differential_attention", ATTENTION, dict(heads=0))])
 def test_empty_calls_launch_nothing(name, base, change):
     assert _status(name, *{**base, **change}.values())[0] == 0
+
+
+def test_parts_of_sizes_that_do_not_exist():
+    splits = _lib.library().mi355x_differential_attention_splits
+    assert splits(1, 1, 8192, 16, 4, 64, 16) > 1
+    for sizes in [(1 << 31, 1 << 31, 1 << 31, 4, 4), (1 << 30, 1 << 30, 1 << 30, 16, 16), (0, 1, 1, 1, 1), (1, 1, 1 << 40, 1, 1), (-1, 1, 1, 1, 1), (1, 1, 1, 3, 2), (1, 1, 1, 1, 0)]:
+        assert splits(*sizes, 64, 1) == 1
 
 
 # ---------------------------------------------------------------------------------------------- bfloat16 on the host
