@@ -175,7 +175,9 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "O = (softmax(scale Q1 K1^T) - l softmax(scale Q2 K2^T)) V with l = exp(q1 . k1) - exp(q2 . k2) + lambda_init; Q [B, Sq, 2 H, d] and "
                "K [B, Sk, 2 G, d] hold the two maps of a head next to each other, V is [B, Sk, G, 2 d], O [B, Sq, H, 2 d]; H / G heads "
                "share keys and values. Keys from lengths[b] on do not exist; if `causal`, query i sees the keys up to i + lengths[b] - Sq. A row "
-               "without keys is 0. `scale` is 1 / sqrt(d) if it is left out."),
+               "without keys is 0. `scale` is 1 / sqrt(d) if it is left out. Prompts padded behind their end need no lengths if `causal`: no valid "
+               "query sees the padding. In float32 an infinite query, key or value that a row sees makes it not a number, and so may, in any type, a value "
+               "that is not finite of a later key that a neighbouring row of a `causal` call sees."),
     # Pad only ever runs folded into the Conv that reads it (transformation/fusion.py, the reference's PadConvFusion)
     ONNXSchema("Pad", 11,
                [ONNXParameter("data", "T"), ONNXParameter("pads", "tensor(int64)"), ONNXParameter("constant_value", "T", _O)],
