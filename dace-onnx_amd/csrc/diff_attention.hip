@@ -549,63 +549,71 @@ __global__ __launch_bounds__(128 * RW * KW, 2) void diff_attention_kernel(DiffAr
     }
 }
 
-// The splits of a row joined: one wave to a row, its lanes the 2 D values.
-template <class T, int D>
+// The splits of a row joined: a wave to a row and map, its lanes the 2 D values, its first BATCH
+// reads on their way before anything is needed.
+template <class T, int D, int BATCH>
 __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs p) {
     constexpr int PER_LANE = 2 * D / WAVE;
+    __shared__ float other[2][2 * D];
     const int64_t rows = p.Sq * p.share, all = p.batch * p.groups * rows;
-    const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;   // of a slice's row
-    const int lane = threadIdx.x % WAVE;
-    if (at >= all) return;
-    const float weight = diff_lambda(p);
-    float result[PER_LANE] = {};
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), map = wave % 2;
+    int64_t at = (int64_t)blockIdx.x * 2 + wave / 2;   // of a slice's row
+    const bool mine = at < all;
+    if (!mine) at = all - 1;
+    // lane s has the base and the sum of splits s, s + 64, ...
+    float base[4], sums[4], top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
-    for (int map = 0; map < 2; ++map) {
-        // lane s has the base and the sum of splits s, s + 64, ...
-        float base[4], sums[4], top = -__builtin_inff(), sum = 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const int s = lane + i * WAVE;
+        const bool is = s < p.splits;
+        base[i] = is ? p.partial_ml[2 * ((s * all + at) * 2 + map)] : -__builtin_inff();
+        sums[i] = is ? p.partial_ml[2 * ((s * all + at) * 2 + map) + 1] : 0.0f;
+    }
+    const float* from_split = p.partial_o + (at * 2 + map) * 2 * D + lane * PER_LANE;
+    float part[BATCH][PER_LANE];
+    auto fetch = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = lane + i * WAVE;
-            const bool is = s < p.splits;
-            base[i] = is ? p.partial_ml[2 * ((s * all + at) * 2 + map)] : -__builtin_inff();
-            sums[i] = is ? p.partial_ml[2 * ((s * all + at) * 2 + map) + 1] : 0.0f;
-            top = fmaxf(top, base[i]);
-        }
-        top = wave_max(top);
-        const float from = top == -__builtin_inff() ? 0.0f : top;
+        for (int j = 0; j < BATCH; ++j) load_values(part[j], from_split + (s0 + j < p.splits ? s0 + j : p.splits - 1) * all * 4 * D, PER_LANE);
+    };
+    fetch(0);
+    const float weight = map ? diff_lambda(p) : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            base[i] = __builtin_amdgcn_exp2f(base[i] - from);
-            sum = fmaf(sums[i], base[i], sum);
-        }
-        sum = wave_sum(sum);
-        float o[PER_LANE] = {};
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, base[i]);
+    top = wave_max(top);
+    const float from = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int count = p.splits - i * WAVE < WAVE ? p.splits - i * WAVE : WAVE;
-            const float* from_split = p.partial_o + ((i * WAVE * all + at) * 2 + map) * 2 * D + lane * PER_LANE;
-            for (int s0 = 0; s0 < count; s0 += 8) {   // eight at a time on their way
-                float part[8][PER_LANE];
+    for (int i = 0; i < 4; ++i) {
+        base[i] = __builtin_amdgcn_exp2f(base[i] - from);
+        sum = fmaf(sums[i], base[i], sum);
+    }
+    sum = wave_sum(sum);
+    float o[PER_LANE] = {};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int s = s0 + j < count ? s0 + j : count - 1;
-                    load_values(part[j], from_split + s * all * 4 * D, PER_LANE);
-                }
+    for (int i = 0; i < 4; ++i) {
+        const int count = p.splits - i * WAVE < WAVE ? p.splits - i * WAVE : WAVE;
+        for (int s0 = 0; s0 < count; s0 += BATCH) {
+            if (i || s0) fetch(i * WAVE + s0);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float factor = s0 + j < count ? readlane_f32(base[i], s0 + j) : 0.0f;
+            for (int j = 0; j < BATCH; ++j) {
+                const bool is = s0 + j < count;
+                const float factor = is ? readlane_f32(base[i], s0 + j) : 0.0f;
 #pragma unroll
-                    for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(part[j][e], factor, o[e]);
-                }
+                for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(is ? part[j][e] : 0.0f, factor, o[e]);
             }
         }
-        const float factor = sum == 0.0f ? 0.0f : (map ? -weight : 1.0f) / sum;
-#pragma unroll
-        for (int e = 0; e < PER_LANE; ++e) result[e] += o[e] * factor;
     }
+    const float factor = sum == 0.0f ? 0.0f : weight / sum;
+    if (map) {
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) other[wave / 2][lane * PER_LANE + e] = o[e] * factor;
+    }
+    __syncthreads();
+    if (map || !mine) return;
+#pragma unroll
+    for (int e = 0; e < PER_LANE; ++e) o[e] = o[e] * factor - other[wave / 2][lane * PER_LANE + e];
     const int64_t slice = at / rows, row = at % rows, b = slice / p.groups;
     const int head = (int)(slice % p.groups) * p.share + (int)(row % p.share);
-    store_values(static_cast<T*>(p.O) + ((b * p.Sq + row / p.share) * p.heads + head) * 2 * D + lane * PER_LANE, result, PER_LANE);
+    store_values(static_cast<T*>(p.O) + ((b * p.Sq + row / p.share) * p.heads + head) * 2 * D + lane * PER_LANE, o, PER_LANE);
 }
 
 // How a type and head size are cut: with many rows RW x RB blocks of 32 and SUB blocks of 32 keys in a stage; with few rows one block and KW key waves.
@@ -643,7 +651,7 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
         constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value;
         p.row_blocks = ceil_div(rows, (int64_t)(32 * RB * RW));
         const int64_t grid = p.row_blocks * p.splits * slices;
-        fits = grid_fits(grid, 128 * RW * KW) && (p.splits == 1 || grid_fits(ceil_div(slices * rows, (int64_t)4), 256));
+        fits = grid_fits(grid, 128 * RW * KW) && (p.splits == 1 || grid_fits(ceil_div(slices * rows, (int64_t)2), 256));
         if (!fits) return;
         // long blocks of a causal mask first, whichever slice they are of: of the slices whose keys an XCD's L2 holds, or of all
         p.per_xcd = !p.causal || p.splits > 1 ? 0 : slices % NUM_XCD == 0 ? (int)(slices / NUM_XCD) : -1;
@@ -658,8 +666,10 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
     else launch(Int<F::RB>{}, Int<F::RW>{}, Int<1>{}, Int<F::SUB>{});
     MI355X_REQUIRE(fits, "differential_attention: too large");
     if (p.splits > 1) {
-        const int64_t all = slices * rows;
-        hipLaunchKernelGGL((diff_join_kernel<T, D>), dim3((unsigned)ceil_div(all, (int64_t)4)), dim3(256), 0, st, p);
+        // (2 parts of 8192 rows by sixteen reads 4 us more than by four)
+        const dim3 g((unsigned)ceil_div(slices * rows, (int64_t)2));
+        if (p.splits <= 4) hipLaunchKernelGGL((diff_join_kernel<T, D, 4>), g, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((diff_join_kernel<T, D, 16>), g, dim3(256), 0, st, p);
     }
     return check_launch("diff_attention_kernel");
 }
