@@ -68,8 +68,25 @@ __device__ __forceinline__ void qlin_store(const QLinArgs& p, Row&& row, Column&
 
 typedef i32x4 UnalignedBytes __attribute__((aligned(1)));
 
+// The 16 bytes from p on by the aligned words that hold them: 16-byte accesses at other boundaries than those of words take the memory unit up to four times
+// as long (64 x 4097 x 4095 straight from memory: 58 us, so 27; 19 with K = 4092). What is read lies between p - 3 and p + 19; the
+// bytes before p are the array's own, as that begins at a word.
+__device__ __forceinline__ i32x4 words_at(const int8_t* p) {
+    typedef i32x4 AtWord __attribute__((aligned(4)));
+    const uint32_t bytes = (uint32_t)reinterpret_cast<uintptr_t>(p) & 3;
+    const int8_t* first = p - bytes;
+    const i32x4 w = *reinterpret_cast<const AtWord*>(first);
+    const int next = *reinterpret_cast<const int*>(first + (bytes ? 16 : 12));
+    i32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_amdgcn_alignbyte((uint32_t)(i < 3 ? w[i + 1] : next), (uint32_t)w[i], bytes);
+    return v;
+}
+
 // the 16 bytes from p on of which `left` belong to a row of K: the others as 0
+template <bool WORDS>
 __device__ __forceinline__ i32x4 row_bytes(const int8_t* p, int64_t left, int64_t K) {
+    if (WORDS && left >= 19) return words_at(p);
     if (left >= 16) return *reinterpret_cast<const UnalignedBytes*>(p);
     if (left <= 0) return i32x4{};
     if (K < 16) {
@@ -87,8 +104,8 @@ __device__ __forceinline__ i32x4 row_bytes(const int8_t* p, int64_t left, int64_
 }
 
 // Any shape and alignment, operands straight from memory. A workgroup has 16 columns and 16 MT rows of Y, its eight waves take turns at the
-// 128-byte lines of K and their sums meet in LDS.
-template <class T, int ACT, int MT>
+// 128-byte lines of K and their sums meet in LDS. WORDS: rows at addresses that are no multiples of 4, in arrays that are, by aligned words.
+template <class T, int ACT, int MT, bool WORDS>
 __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
     constexpr int WAVES = 8;
     __shared__ __attribute__((aligned(16))) i32x4 part[WAVES][MT][WAVE];
@@ -115,8 +132,12 @@ __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
     };
     int64_t k = 128 * wave;
 #pragma unroll 4
-    for (; k + 128 <= p.K; k += 128 * WAVES) line(k, [](const int8_t* at, int64_t) { return i32x4(*reinterpret_cast<const UnalignedBytes*>(at)); });
-    if (k < p.K) line(k, [&](const int8_t* at, int64_t left) { return row_bytes(at, left, p.K); });
+    for (; k + (WORDS ? 131 : 128) <= p.K; k += 128 * WAVES)
+        line(k, [](const int8_t* at, int64_t) {
+            if constexpr (WORDS) return words_at(at);
+            else return i32x4(*reinterpret_cast<const UnalignedBytes*>(at));
+        });
+    if (k < p.K) line(k, [&](const int8_t* at, int64_t left) { return row_bytes<WORDS>(at, left, p.K); });
 #pragma unroll
     for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
     __syncthreads();
@@ -173,13 +194,13 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
     const int64_t whole = DIRECT ? p.K / BK : 0, steps = (p.K + BK - 1) / BK;
     typedef i32x4 Held[PER_WAVE];
-    auto fetch = [&](int64_t step, Held& to) __attribute__((always_inline)) {   // by registers
+    auto fetch = [&](int64_t step, Held& to) __attribute__((always_inline)) {   // by registers (words and what follows them wait in more of them: 124 us become 190 at 4095^3)
         if ((step + 1) * BK <= p.K) {
 #pragma unroll
             for (int i = 0; i < PER_WAVE; ++i) to[i] = *(const __attribute__((address_space(1))) UnalignedBytes*)(base(i, step) + offset[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < PER_WAVE; ++i) to[i] = row_bytes((i < X_COUNT ? x_tile : w_tile) + step * BK + offset[i], p.K - step * BK - 16 * piece[i], p.K);
+            for (int i = 0; i < PER_WAVE; ++i) to[i] = row_bytes<false>((i < X_COUNT ? x_tile : w_tile) + step * BK + offset[i], p.K - step * BK - 16 * piece[i], p.K);
         }
     };
     auto put = [&](int stage, const Held& v) __attribute__((always_inline)) {
@@ -302,11 +323,14 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
 
 template <class T, int ACT>
 static void launch_qlin(QLinArgs p, hipStream_t st) {
+    const bool words = ((reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.W)) & 3) == 0;
     auto direct = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         p.tiles_n = ceil_div(p.N, (int64_t)16);
         p.tiles_m = ceil_div(p.M, (int64_t)(16 * MT));
-        hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(512), 0, st, p);
+        const dim3 grid((unsigned)(p.tiles_m * p.tiles_n)), block(512);
+        if (words && p.K % 4) hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT, true>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT, false>), grid, block, 0, st, p);
     };
     const bool aligned = p.K % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.W)) & 15) == 0;
     auto tile = [&](auto wm, auto wn, auto tm, auto tn, auto ns, auto bk, int per_cu) {
@@ -317,21 +341,24 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
         const int group_m = choose_group_m(p.tiles_m, ceil_div(nwg, (int64_t)NUM_XCD), (int64_t)per_cu * 32, 32 * TM * WM, 32 * TN * WN, p.K);
         const dim3 grid((unsigned)nwg), block(64 * WM * WN);
         if (aligned) hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, NS, BK, true>), grid, block, 0, st, p, group_m);
-        else hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, 2, 128, false>), grid, block, 0, st, p, group_m);
+        else hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, 2, BK, false>), grid, block, 0, st, p, group_m);
     };
     // Which kernel, by microseconds of the forms at N = K = 4096, bfloat16 (M; 16 columns each direct / 64 x 64 / 128 x 128 one to a CU / two to a CU / 256 x 256):
     // 4: 7.1 / 13.9 / 20 / 25 / 47; 64: 12.9 / 13.9 / 20 / 26 / 50; 128: 22 / 13.8 / 20 / 26 / 51; 512: 75 / 16.6 / 21.1 / 26 / 50; 1024: 151 / 31 / 26.0 / 29 / 51;
     // 2048: 281 / 70 / 50 / 40 / 58; 8192 x 8192: 2239 / 439 / - / 317 / 256. Direct takes 3.5 us and 0.42 ns for each round of workgroups, k and 16 rows or columns of one
     // (64 x 16384 x 1024: 12.9 us, 64 x 512 x 8192: 20.0); 64 x 64 as much and 2.5 ns for each round and k (7.5 and 20.2). The largest two by their rounds, 40 and 64 us each.
-    // Rows at other addresses, whose bytes wait in registers: 5923 x 4002 x 1206 100 / 65 / 117 / 80, 1134 x 15690 x 3927 251 / 161 / 278 / 217 (64 x 64 / 128 x 128 one to a CU / two / 256 x 256).
+    // Rows that begin at words take 0.37 and 5.2 ns (197 x 2049 x 1004: 7.9 / 8.8 us), others in arrays that do 0.65 and 6.9 (64 x 4097 x 4095: 27 / 30; 4 x 4099 x 4097: 10.1 /
+    // 30), the rest 1.35 and 6.9.
+    // Large ones at other addresses, whose bytes wait in registers: 5923 x 4002 x 1206 100 / 65 / 117 / 80, 1134 x 15690 x 3927 251 / 161 / 278 / 217 (64 x 64 / 128 x 128 one to a CU / two / 256 x 256).
     const int64_t tiles64 = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64), tiles128 = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t tiles256 = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
     int mt = 1;   // rows / 16 of a workgroup, direct
     auto direct_cost = [&](int rows16) { return ceil_div(ceil_div(p.M, (int64_t)(16 * rows16)) * ceil_div(p.N, (int64_t)16), (int64_t)256) * (rows16 + 1); };
     for (int rows16 = 2; rows16 <= 4; rows16 *= 2)
         if (direct_cost(rows16) < direct_cost(mt)) mt = rows16;
+    const int per_tile = aligned ? 6 : !words ? 5 : p.K % 4 ? 10 : 15;
     const int form = tuning().qlin_form;
-    const int pick = form >= 0 ? form : direct_cost(mt) <= 6 * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 || !aligned ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
+    const int pick = form >= 0 ? form : direct_cost(mt) <= per_tile * ceil_div(tiles64, (int64_t)512) ? 0 : tiles64 <= 512 ? 1 : tiles128 <= 256 || !aligned ? 2 : 40 * ceil_div(tiles128, (int64_t)512) <= 64 * ceil_div(tiles256, (int64_t)256) ? 3 : 4;
     if (pick == 4) tile(Int<2>{}, Int<4>{}, Int<4>{}, Int<2>{}, Int<2>{}, Int<128>{}, 1);
     else if (pick == 3) tile(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<128>{}, 2);
     else if (pick == 2) tile(Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}, Int<3>{}, Int<128>{}, 1);

@@ -180,6 +180,21 @@ def test_linear_with_one_scale_and_more_dimensions():
     within(y.reshape(6, 50), expected, linear_bound(size, expected, F32))
 
 
+@pytest.mark.parametrize("k", [17, 18, 19, 127, 129, 130, 131, 133, 1155, 2049, 4091, 4094, 4095])
+@pytest.mark.parametrize("m, n", [(1, 1), (5, 33), (70, 40)])
+def test_linear_straight_from_memory_of_odd_rows(m, n, k, tuning):
+    """Arrays that begin at words and rows that do not, arrays that do not; what lies before and behind them would change the sums."""
+    tuning(MI355X_QLIN_FORM=0)
+    lib = _lib.library()
+    for front in (4, 3):
+        x, w = (torch.cat([t.new_full((front,), 127), t.reshape(-1), t.new_full((32,), 127)]) for t in (eight(1, m, k), eight(2, n, k)))
+        y, one = torch.zeros(m, n, device="cuda"), torch.ones(1, device="cuda")
+        _lib.check(lib.mi355x_quantized_linear(x[front:].data_ptr(), w[front:].data_ptr(), one.data_ptr(), one.data_ptr(), None, None, y.data_ptr(), m, n, k, 1, 1, 0, 1, _lib.current_stream()),
+                   "linear")
+        expected = x[front:front + m * k].view(m, k).double() @ w[front:front + n * k].view(n, k).double().t()
+        within(y, expected, U * expected.abs() + TINY[F32])
+
+
 @pytest.mark.parametrize("m", [2, 300])
 @pytest.mark.parametrize("dtype", R.TYPES)
 def test_linear_small_results_of_silu(m, dtype):
