@@ -16,7 +16,7 @@
 // maxima and roundings for 32 keys, 64 rows and a map of 64. 8 heads of 64 over 8192 queries and keys in bfloat16: 382 us, 1.08 PFLOP/s of the 12 d operations that one
 // pass with two outputs takes for a pair, where a library product of 8192^3 reaches 1.15 to 1.51; causal 228. Two waves to a SIMD have 256
 // registers each, most of them accumulators: what else is kept from pass to pass decides whether those stay in place. float32: 3 x 333 queries and keys, 6 heads of 64, 21 us; 8 x 3 heads, 4016 x 6818: 2.8 ms, 180
-// TFLOP/s (float32 products reach 154). Few rows by the bytes: 8 x 1 of up to 8192 keys, 90 MB, 20 us (4.5 TB/s) and 6 for the second launch.
+// TFLOP/s (float32 products reach 154). Few rows by the bytes: 8 x 1 of up to 8192 keys, 90 MB, 20 us (4.5 TB/s) and 4 for the second launch.
 #include "mixed.h"
 #include "gemm_tile.h"
 
@@ -691,15 +691,16 @@ extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t S
     const int forced = tuning().diff_splits;
     if (forced > 0) return std::min(forced, 256);
     // By what a workgroup's stages take, what joining takes (a launch, and the sums written and read), and one round of workgroups at most. Measured, microseconds: 8 x 1 of
-    // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 97 in one part (FEW), 34 in 8, 30 in 16, 36 in 32 (SMALL); 1 x 1 of them 18.2 in 16, 16.1 in 32, 19.6 in 64; 16 x 1 of 1000 keys, 8 heads,
-    // float16: 20.7 in one part, 21.7 in 2, 20.0 in 4; 512 of 512, 8 heads: 11.0 and 18.4; float32, 8 heads of 128, 1024 of 1024: 159 and 104.
+    // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 100 in one part (FEW), 32 in 8, 28 in 16, 32 in 32 (SMALL); 1 x 1 of them 16.1 in 16, 13.0 in 32; 16 x 1 of 1000 keys, 8 heads,
+    // float16: 20.6 in one part, 19.7 in 2, 17.7 in 4; 512 of 512, 8 heads: 11.3 and 18.2; float32: 333 of 333, 6 heads of 64, 24.8 in one part, 21.7 in 2, 19.5 in 3; 8 heads
+    // of 128, 1024 of 1024: 162 and 109, 256 of 256 47, 36, 31.6 in 4.
     auto stage = [&](const DiffCut& c) { return type == MI355X_TYPE_FLOAT ? (size == 128 ? 4.5 : 2.3) : c.form == DIFF_SMALL ? 1.0 : 1.3; };   // us
     const double sums = 16.0 * (double)(batch * Sq * heads) * (double)(2 * size + 2) / 4e6;                                                  // of one part
     const int64_t room = (part.form == DIFF_SMALL ? 512 : 256) / part.workgroups;
     int64_t best = 1;
     double least = stage(whole) * (double)whole.stages;
     for (int64_t n = 2; n <= std::min({room, part.stages, (int64_t)256}); ++n) {
-        const double cost = stage(part) * (double)ceil_div(part.stages, n) + 7.0 + (double)n * (0.1 + sums);
+        const double cost = stage(part) * (double)ceil_div(part.stages, n) + 4.0 + (double)n * (0.1 + sums);
         if (cost < least) least = cost, best = n;
     }
     return best;
