@@ -496,7 +496,7 @@ int mi355x_rotary_positions(const void* Q, const void* K, const void* positions,
  * `scratch` has room for splits * batch * Sq * heads * (4 size + 4) floats, 16-byte aligned, and belongs to the
  * call until it is done. Of values that a row does not see, but another row of the entry does, an infinity or NaN
  * may still reach it; lengths keep them out. In float32 an infinite query, key or value that a row sees makes it not a
- * number (finite values are exact in the products' operands). */
+ * number, and values below 2^-110 lose digits (others are exact in the products' operands). */
 int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups,
                                              int64_t size, int type);
 int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1,
