@@ -321,13 +321,17 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
     }
 }
 
+// false: more workgroups than a launch has
 template <class T, int ACT>
-static void launch_qlin(QLinArgs p, hipStream_t st) {
+static bool launch_qlin(QLinArgs p, hipStream_t st) {
+    bool fits = true;
     const bool words = ((reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.W)) & 3) == 0;
     auto direct = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         p.tiles_n = ceil_div(p.N, (int64_t)16);
         p.tiles_m = ceil_div(p.M, (int64_t)(16 * MT));
+        fits = grid_fits(p.tiles_m * p.tiles_n, 512);
+        if (!fits) return;
         const dim3 grid((unsigned)(p.tiles_m * p.tiles_n)), block(512);
         if (words && p.K % 4) hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT, true>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((qlin_direct_kernel<T, ACT, MT, false>), grid, block, 0, st, p);
@@ -338,6 +342,8 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
         p.tiles_m = ceil_div(p.M, (int64_t)(32 * TM * WM));
         p.tiles_n = ceil_div(p.N, (int64_t)(32 * TN * WN));
         const int64_t nwg = p.tiles_m * p.tiles_n;
+        fits = grid_fits(nwg, 64 * WM * WN);
+        if (!fits) return;
         const int group_m = choose_group_m(p.tiles_m, ceil_div(nwg, (int64_t)NUM_XCD), (int64_t)per_cu * 32, 32 * TM * WM, 32 * TN * WN, p.K);
         const dim3 grid((unsigned)nwg), block(64 * WM * WN);
         if (aligned) hipLaunchKernelGGL((qlin_tile_kernel<T, ACT, WM, WN, TM, TN, NS, BK, true>), grid, block, 0, st, p, group_m);
@@ -366,6 +372,7 @@ static void launch_qlin(QLinArgs p, hipStream_t st) {
     else if (mt == 1) direct(Int<1>{});
     else if (mt == 2) direct(Int<2>{});
     else direct(Int<4>{});
+    return fits;
 }
 
 }  // namespace mi355x
@@ -382,15 +389,17 @@ extern "C" int mi355x_quantized_linear(const int8_t* X, const int8_t* W, const f
     MI355X_REQUIRE(w_scale_count == 1 || w_scale_count == N, "quantized_linear: w_scale holds %lld values, expected 1 or N=%lld", (long long)w_scale_count, (long long)N);
     if (M == 0 || N == 0) return MI355X_OK;
     MI355X_REQUIRE((K == 0 || (X && W)) && x_scale && w_scale && Y, "quantized_linear: null pointer");
-    MI355X_REQUIRE(M < (int64_t)1 << 31 && N < (int64_t)1 << 31 && grid_fits(ceil_div(M, (int64_t)16) * ceil_div(N, (int64_t)16), 512), "quantized_linear: too large");
+    MI355X_REQUIRE(M < (int64_t)1 << 31 && N < (int64_t)1 << 31, "quantized_linear: too large");
     QLinArgs p = {X, W, x_scale, w_scale, bias, residual, Y, M, N, K, x_scale_count != 1, w_scale_count != 1, activation, 0, 0};
+    bool fits = true;
     with_type(type, [&](auto t) {
         using T = decltype(t);
         hipStream_t st = static_cast<hipStream_t>(stream);
-        if (activation == MI355X_ACT_RELU) launch_qlin<T, MI355X_ACT_RELU>(p, st);
-        else if (activation == MI355X_ACT_GELU) launch_qlin<T, MI355X_ACT_GELU>(p, st);
-        else if (activation == MI355X_ACT_SILU) launch_qlin<T, MI355X_ACT_SILU>(p, st);
-        else launch_qlin<T, MI355X_ACT_NONE>(p, st);
+        if (activation == MI355X_ACT_RELU) fits = launch_qlin<T, MI355X_ACT_RELU>(p, st);
+        else if (activation == MI355X_ACT_GELU) fits = launch_qlin<T, MI355X_ACT_GELU>(p, st);
+        else if (activation == MI355X_ACT_SILU) fits = launch_qlin<T, MI355X_ACT_SILU>(p, st);
+        else fits = launch_qlin<T, MI355X_ACT_NONE>(p, st);
     });
+    MI355X_REQUIRE(fits, "quantized_linear: too large");
     return check_launch("quantized_linear");
 }

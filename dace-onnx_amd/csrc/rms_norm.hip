@@ -213,12 +213,16 @@ __global__ __launch_bounds__(1024) void rms_norm_long(RmsArgs p) {
     }
 }
 
+// false: more workgroups than a launch has
 template <class T>
-static void launch_rms_norm(const RmsArgs& p, hipStream_t st) {
+static bool launch_rms_norm(const RmsArgs& p, hipStream_t st) {
     constexpr int64_t E = 16 / sizeof(T);
+    bool fits = true;
     auto rows = [&](auto th, auto nv) {
-        constexpr int TH = decltype(th)::value, NV = decltype(nv)::value, ROWS = TH < 256 ? 256 / TH : 1;
-        hipLaunchKernelGGL((rms_norm_rows<T, TH, NV>), dim3((unsigned)ceil_div(p.rows, (int64_t)ROWS)), dim3(TH < 256 ? 256 : TH), 0, st, p);
+        constexpr int TH = decltype(th)::value, NV = decltype(nv)::value, ROWS = TH < 256 ? 256 / TH : 1, THREADS = TH < 256 ? 256 : TH;
+        const int64_t grid = ceil_div(p.rows, (int64_t)ROWS);
+        fits = grid_fits(grid, THREADS);
+        if (fits) hipLaunchKernelGGL((rms_norm_rows<T, TH, NV>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);
     };
     const int64_t vectors = ceil_div(p.cols, E);
     if (vectors <= 64) rows(Int<64>{}, Int<1>{});
@@ -228,7 +232,11 @@ static void launch_rms_norm(const RmsArgs& p, hipStream_t st) {
     else if (vectors <= 1024) rows(Int<256>{}, Int<4>{});
     else if (vectors <= 2048) rows(Int<1024>{}, Int<2>{});
     else if (vectors <= 4096) rows(Int<1024>{}, Int<4>{});
-    else hipLaunchKernelGGL(rms_norm_long<T>, dim3((unsigned)p.rows), dim3(1024), 0, st, p);
+    else {
+        fits = grid_fits(p.rows, 1024);
+        if (fits) hipLaunchKernelGGL(rms_norm_long<T>, dim3((unsigned)p.rows), dim3(1024), 0, st, p);
+    }
+    return fits;
 }
 
 }  // namespace mi355x
@@ -244,12 +252,14 @@ extern "C" int mi355x_skip_rms_norm(const void* X, const void* skip, const void*
     MI355X_REQUIRE(rows == 0 || cols > 0, "skip_rms_norm: rows without columns");
     if (rows == 0) return MI355X_OK;
     MI355X_REQUIRE(X && gain, "skip_rms_norm: null pointer (X and gain are required)");
-    MI355X_REQUIRE(cols < ((int64_t)1 << 31) - 65536 && grid_fits(rows, 1024), "skip_rms_norm: too many rows or columns");
+    MI355X_REQUIRE(cols < ((int64_t)1 << 31) - 65536 && rows < (int64_t)1 << 40, "skip_rms_norm: too many rows or columns");
     const bool over = Sum == X || Y == X || (skip && (Sum == skip || Y == skip));
     const int64_t vectors = ceil_div(cols, (int64_t)(type == MI355X_TYPE_FLOAT ? 4 : 8));
     MI355X_REQUIRE(!over || vectors <= 4096, "skip_rms_norm: rows of %lld columns cannot be written over the input", (long long)cols);
     MI355X_REQUIRE(Sum == nullptr || Sum != Y, "skip_rms_norm: Sum and Y are one array");
     const RmsArgs p = {X, skip, gain, Y, Sum, Q, q_scale, rows, cols, epsilon};
-    with_type(type, [&](auto t) { launch_rms_norm<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
+    bool fits = true;
+    with_type(type, [&](auto t) { fits = launch_rms_norm<decltype(t)>(p, static_cast<hipStream_t>(stream)); });
+    MI355X_REQUIRE(fits, "skip_rms_norm: too many rows");
     return check_launch("rms_norm_rows");
 }

@@ -102,9 +102,8 @@ __global__ __launch_bounds__(ROTARY_THREADS) void rotary_positions_kernel(Rotary
 }
 
 template <class T>
-static void launch_rotary(RotaryArgs p, bool interleaved, hipStream_t st) {
+static void launch_rotary(const RotaryArgs& p, bool interleaved, hipStream_t st) {
     const int pairs = p.rotated / 2;
-    p.tokens_per_wg = std::max(1, std::min(4, ROTARY_LDS_ANGLES / std::max(pairs, 1)));
     const dim3 grid((unsigned)ceil_div(p.tokens, (int64_t)p.tokens_per_wg)), block(ROTARY_THREADS);
     auto launch = [&](auto vec) {
         constexpr int VEC = decltype(vec)::value;
@@ -138,7 +137,8 @@ extern "C" int mi355x_rotary_positions(const void* Q, const void* K, const void*
     MI355X_REQUIRE(pairs == rotated / 2, "rotary_positions: sections of %lld pairs, %lld are turned", (long long)pairs, (long long)(rotated / 2));
     if (tokens == 0 || heads + kv_heads == 0 || size == 0) return MI355X_OK;
     MI355X_REQUIRE((heads == 0 || (Q && Q_out)) && (kv_heads == 0 || (K && K_out)) && (rotated == 0 || (positions && frequencies)), "rotary_positions: null pointer");
-    MI355X_REQUIRE(grid_fits(tokens, ROTARY_THREADS), "rotary_positions: too many tokens");
+    p.tokens_per_wg = std::max(1, std::min(4, ROTARY_LDS_ANGLES / std::max(p.rotated / 2, 1)));
+    MI355X_REQUIRE(tokens < (int64_t)1 << 40 && grid_fits(ceil_div(tokens, (int64_t)p.tokens_per_wg), ROTARY_THREADS), "rotary_positions: too many tokens");
     with_type(type, [&](auto t) { launch_rotary<decltype(t)>(p, interleaved != 0, static_cast<hipStream_t>(stream)); });
     return check_launch("rotary_positions_kernel");
 }

@@ -138,6 +138,8 @@ ATTENTION = dict(Q=P, K=P, V=P, q1=P, k1=P, q2=P, k2=P, lengths=P, O=P, scratch=
     ("mi355x_quantized_linear", LINEAR, dict(activation=4), "activation"), ("mi355x_quantized_linear", LINEAR, dict(type=3), "element type"),
     ("mi355x_quantized_linear", LINEAR, dict(M=-4, xc=1), "negative"), ("mi355x_quantized_linear", LINEAR, dict(W=None), "null"),
     ("mi355x_quantized_linear", LINEAR, dict(M=1 << 31, xc=1), "too large"),
+    ("mi355x_quantized_linear", LINEAR, dict(M=(1 << 31) - 1, N=(1 << 31) - 1, xc=1, wc=1), "too large"), ("mi355x_skip_rms_norm", NORM, dict(rows=1 << 26), "too many"),
+    ("mi355x_rotary_positions", ROTARY, dict(tokens=1 << 27), "too many"),
     ("mi355x_rotary_positions", ROTARY, dict(rotated=7), "values"), ("mi355x_rotary_positions", ROTARY, dict(rotated=10), "values"), ("mi355x_rotary_positions", ROTARY, dict(axes=9), "axes"),
     ("mi355x_rotary_positions", ROTARY, dict(sections=[2, 1]), "sections"), ("mi355x_rotary_positions", ROTARY, dict(sections=[5, -1]), "section"),
     ("mi355x_rotary_positions", ROTARY, dict(bytes=2), "positions of 2"), ("mi355x_rotary_positions", ROTARY, dict(K=None), "null"), ("mi355x_rotary_positions", ROTARY, dict(type=6), "element type"),

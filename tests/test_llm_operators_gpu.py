@@ -77,6 +77,14 @@ def test_norm_over_several_dimensions():
     check_norm(x.reshape(6, 40), gain.reshape(40), None, y.reshape(6, 40), None, q.reshape(6, 40), scale.reshape(6))
 
 
+def test_norm_of_many_rows():
+    """2^22 rows and more, as the heads of long prompts are."""
+    rows, columns = (1 << 22) + 5, 8
+    x, gain = normal(1, rows, columns, dtype=BF), normal(2, columns, dtype=BF)
+    check_norm(x, gain, None, *R.call("SkipRMSNormalization", [("x", x), ("g", gain), ("skip", None)], [("y", BF, x.shape), None, ("q", torch.int8, x.shape), ("qs", F32, (rows,))])[:1],
+               None, None, None)
+
+
 @pytest.mark.parametrize("columns", [40, 300, 40000])
 def test_norm_of_extreme_rows(columns):
     """Squares beyond float32, squares that vanish in it, rows of zeros, rows with an infinity or a NaN."""
@@ -193,6 +201,16 @@ def test_linear_straight_from_memory_of_odd_rows(m, n, k, tuning):
                    "linear")
         expected = x[front:front + m * k].view(m, k).double() @ w[front:front + n * k].view(n, k).double().t()
         within(y, expected, U * expected.abs() + TINY[F32])
+
+
+@pytest.mark.parametrize("k", [16, 17])
+def test_linear_of_more_than_32_bits_of_results(k):
+    m, n = (1 << 17) + 3, (1 << 14) + 24
+    x, w, xs, ws = eight(1, m, k), eight(2, n, k), normal(3, m).abs() / 74 + 1e-3, normal(4, n).abs() / 74
+    y, = R.call("QuantizedLinear", [("x", x), ("w", w), ("xs", xs), ("ws", ws)], [("y", F16, (m, n))], to=R.ELEMENT[F16])
+    for rows in (slice(0, 300), slice(m // 2, m // 2 + 300), slice(m - 300, m)):
+        expected, size = R.quantized_linear(x[rows], w, xs[rows], ws)
+        within(y[rows], expected, linear_bound(size, expected, F16))
 
 
 @pytest.mark.parametrize("m", [2, 300])
