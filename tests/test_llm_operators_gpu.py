@@ -607,3 +607,30 @@ def test_another_stream_and_recordings_of_the_caller():
         replayed = out.clone()
         assert torch.equal(replayed, m(*tensors))
         torch.cuda.synchronize()
+
+
+def test_attention_in_parts_as_a_recorded_graph_and_as_a_single_call():
+    """A graph that has the sums of its parts recorded with it, replayed between eager calls; a node called by itself on two streams in turn."""
+    q, k, v = normal(1, 2, 1, 8, 64, dtype=F16), normal(2, 2, 3000, 4, 64, dtype=F16), normal(3, 2, 3000, 2, 128, dtype=F16)
+    vectors, lengths = [normal(4 + i, 8, scale=0.3) for i in range(4)], torch.tensor([3000, 17], dtype=torch.int32).cuda()
+    assert _lib.library().mi355x_differential_attention_splits(2, 1, 3000, 4, 2, 64, 10) > 1
+    names = ["Q", "K", "V", "lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2", "lengths"]
+    tensors = [q, k, v, *vectors, lengths]
+    infos = [helper.make_tensor_value_info(n, R.ELEMENT[t.dtype], list(t.shape)) for n, t in zip(names, tensors)]
+    graph = helper.make_model(helper.make_graph([helper.make_node("DifferentialAttention", names, ["O"], name="node", causal=1, lambda_init=0.4)], "one", infos,
+                                                [helper.make_tensor_value_info("O", 10, [2, 1, 4, 128])]))
+    eager, recorded = donnx.ONNXModel("eager", graph), donnx.ONNXModel("recorded", graph, use_hip_graph=True)
+    out, side = torch.empty(2, 1, 4, 128, dtype=F16, device="cuda"), torch.cuda.Stream()
+    for n in ((3000, 17), (1, 0), (2000, 3000), (33, 64)):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        expected, size = R.differential_attention(q, k, v, vectors, 0.4, None, lengths, True)
+        o = eager(*tensors).clone()
+        within(o, expected, attention_bound(q, k, size, expected, 0.125, 8))
+        assert torch.equal(recorded(*tensors), o)
+        for stream in (torch.cuda.current_stream(), side):
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                donnx.ONNXDifferentialAttention(**dict(zip(names, tensors)), O=out, causal=1, lambda_init=0.4)
+            torch.cuda.default_stream().wait_stream(stream)
+            assert torch.equal(out, o)
+            out.zero_()
