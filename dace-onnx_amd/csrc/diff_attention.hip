@@ -626,14 +626,35 @@ struct DiffForm {
 
 // Which form. FEW: one block of rows and KW key waves to a workgroup, one workgroup to a CU; SMALL: half the key waves, two to a CU (small heads); WIDE: many rows by
 // two key waves, one to a CU, where the long and short blocks of a causal mask even out; TALL: by one, two to a CU. Microseconds FEW / SMALL / WIDE / TALL, bfloat16,
-// 8 heads of 64: 512 queries and keys 11.0 / 11.8 / 20.7 / 21.7; 1039 (264 blocks of rows) 34 / 23 / 35 / 41; 1500 43 / 31 / 45 / 54; 2048 49 / - / 54 / 68; 8192 699 / - /
-// 441 / 394, causal 348 / - / 232 / 277. Heads of 128, 1039: 75 / 59 / 40 / 50. float32, heads of 64: 3 x 333 24.8 / - / 29.9 / 32.8, 1039 117 / 102 / 79 / 93.
+// 8 heads of 64: 512 queries and keys 11.0 / 11.8 / 20.7 / 21.7; 1039 (264 blocks of rows) 34 / 23 / 35 / 41; 1500 41 / 30 / 45 / 55; 2048 49 / - / 54 / 68; 8192 699 / - /
+// 441 / 394. Heads of 128, 1039: 75 / 59 / 40 / 50; in three parts 1200 of 4000, 4 heads 97 / - / 59 / 72 (one part 121 / - / 112 / 162). float32, heads of 64: 3 x 333 24.8 / - /
+// 29.9 / 32.8, 1039 117 / 102 / 79 / 93.
 enum { DIFF_FEW, DIFF_TALL, DIFF_WIDE, DIFF_SMALL };
+
+// Of a causal mask, heads of at most 128 bytes: a form's time is that of the longest block, of all blocks, or, where there are more workgroups than places, of the two that
+// follow one another; long ones start first. `row`: us for a key and 32 rows where all places are taken, `block`: for a key and a workgroup, `start`: for each round.
+// 4 heads of 64, bfloat16: 4000 56 / 68 / 103; 8 heads: 1200 19.0 / 22.0 / 35.5, 2048 35.0 / 34.9 / 55.6, 2600 53 / 46.8 / 71.8, 8192 348 / - / 232; 4 x 600 26.6 / 15.9 / 25.4;
+// float32, heads of 32: 2 x 1644 86 / 74 / 104, 10 x 564 of 3435, 3 heads 215 / 214 / 200.
+static int diff_causal_form(int64_t few, int64_t wide, int64_t Sq, int64_t Sk) {
+    const double longest = (double)Sk, shortest = std::max(0.0, (double)(Sk - Sq)), mean = Sq <= Sk ? longest - 0.5 * (double)Sq : 0.5 * longest * longest / (double)Sq;
+    auto cost = [&](int64_t workgroups, int64_t places, double row, double block, double start) {
+        double most = std::max(longest * block, (double)few * mean * row / 256.0);
+        if (workgroups > places) most = std::max(most, 2.0 * block * (longest - (longest - shortest) * (double)places / (double)workgroups));
+        return most + start * (double)workgroups / (double)places;
+    };
+    const double as_few = cost(few, 256, 0.0102, 0.0102, 4.0), as_small = cost(few, 512, 0.0078, 0.0156, 2.0), as_wide = cost(wide, 256, 0.0067, 0.0269, 2.0);
+    return as_few <= as_small && as_few <= as_wide ? DIFF_FEW : as_small <= as_wide ? DIFF_SMALL : DIFF_WIDE;
+}
+
 struct DiffCut { int form; int64_t workgroups, stages; };
-static DiffCut diff_cut(int64_t rows, int64_t slices, int64_t Sk, int bytes, int causal, bool in_parts) {
+static DiffCut diff_cut(int64_t rows, int64_t slices, int64_t Sq, int64_t Sk, int bytes, int causal, bool in_parts) {
     const int forced = tuning().diff_form;
     const int64_t few = ceil_div(rows, (int64_t)32) * slices, wide = ceil_div(rows, (int64_t)(bytes <= 128 ? 128 : 64)) * slices;
-    const int form = forced >= 0 && forced <= DIFF_SMALL ? forced : rows <= 32 && in_parts && bytes <= 128 ? DIFF_SMALL : rows <= 32 || (few <= 256 && bytes <= 256) ? DIFF_FEW :
+    const int form = forced >= 0 && forced <= DIFF_SMALL ? forced :
+                     in_parts && bytes <= 128 && rows <= 32 ? DIFF_SMALL :
+                     in_parts && bytes == 256 && few > 128 ? DIFF_WIDE :   // (FEW has no room for parts)
+                     rows <= 32 || (few <= 256 && bytes <= 256) ? DIFF_FEW :
+                     causal && bytes <= 128 && !in_parts ? diff_causal_form(few, wide, Sq, Sk) :
                      few <= 512 && bytes <= 128 ? DIFF_SMALL :
                      causal || wide <= 256 ? DIFF_WIDE : DIFF_TALL;
     const bool one_block = form == DIFF_FEW || form == DIFF_SMALL;
@@ -659,7 +680,7 @@ static int launch_diff(DiffArgs p, hipStream_t st) {
         if (direct) hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, true>), g, block, 0, st, p);
         else hipLaunchKernelGGL((diff_attention_kernel<T, D, RB, RW, KW, SUB, false>), g, block, 0, st, p);
     };
-    const int form = diff_cut(rows, slices, p.Sk, F::BYTES, p.causal, p.splits > 1).form;
+    const int form = diff_cut(rows, slices, p.Sq, p.Sk, F::BYTES, p.causal, p.splits > 1).form;
     if (form == DIFF_FEW) launch(Int<1>{}, Int<1>{}, Int<F::KW>{}, Int<1>{});
     else if (form == DIFF_SMALL) launch(Int<1>{}, Int<1>{}, Int<(F::KW > 1 ? F::KW / 2 : 1)>{}, Int<1>{});
     else if (form == DIFF_WIDE) launch(Int<F::RB>{}, Int<F::RW>{}, Int<F::WIDE>{}, Int<1>{});
@@ -687,14 +708,18 @@ extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t S
     if (!is_mixed_type(type) || (size != 32 && size != 64 && size != 128) || groups < 1 || heads < 1 || heads % groups || batch < 1 || Sq < 1 || Sk < 1 || !diff_fits(batch, Sq, Sk, heads, groups)) return 1;
     const int64_t rows = Sq * (heads / groups), slices = batch * groups;
     const int bytes = (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2);
-    const DiffCut whole = diff_cut(rows, slices, Sk, bytes, 0, false), part = diff_cut(rows, slices, Sk, bytes, 0, true);
+    const DiffCut whole = diff_cut(rows, slices, Sq, Sk, bytes, 0, false), part = diff_cut(rows, slices, Sq, Sk, bytes, 0, true);
     const int forced = tuning().diff_splits;
     if (forced > 0) return std::min(forced, 256);
     // By what a workgroup's stages take, what joining takes (a launch, and the sums written and read), and one round of workgroups at most. Measured, microseconds: 8 x 1 of
     // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 100 in one part (FEW), 32 in 8, 28 in 16, 32 in 32 (SMALL); 1 x 1 of them 16.1 in 16, 13.0 in 32; 16 x 1 of 1000 keys, 8 heads,
     // float16: 20.6 in one part, 19.7 in 2, 17.7 in 4; 512 of 512, 8 heads: 11.3 and 18.2; float32: 333 of 333, 6 heads of 64, 24.8 in one part, 21.7 in 2, 19.5 in 3; 8 heads
-    // of 128, 1024 of 1024: 162 and 109, 256 of 256 47, 36, 31.6 in 4.
-    auto stage = [&](const DiffCut& c) { return type == MI355X_TYPE_FLOAT ? (size == 128 ? 4.5 : 2.3) : c.form == DIFF_SMALL ? 1.0 : 1.3; };   // us
+    // of 128, 1024 of 1024: 162 and 109, 256 of 256 47, 36, 31.6 in 4; 2 heads, 2228 of 2228: of 64, float32 119 and 71 in 3 (WIDE), of 128, bfloat16, causal 72 and 42.5, 3344 of 3344 101
+    // and 66 in 2.
+    auto stage = [&](const DiffCut& c) { 
+        const bool wide = c.form == DIFF_WIDE || c.form == DIFF_TALL;   // us
+        return type == MI355X_TYPE_FLOAT ? (size == 128 ? 4.5 : size == 64 ? (wide ? 4.2 : 3.2) : 2.3) : size == 128 ? (wide ? 1.8 : 1.9) : c.form == DIFF_SMALL ? 1.0 : 1.3;
+    };
     const double sums = 16.0 * (double)(batch * Sq * heads) * (double)(2 * size + 2) / 4e6;                                                  // of one part
     const int64_t room = (part.form == DIFF_SMALL ? 512 : 256) / part.workgroups;
     int64_t best = 1;
