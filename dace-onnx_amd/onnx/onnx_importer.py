@@ -257,6 +257,8 @@ class ONNXModel:
             else:
                 raise ValueError(f"Constant node attribute '{kind}' is not supported")
             extra.append(proto.numpy_helper.from_array(value, name=node.output[0]))
+            if kind == "value" and attr.value.data_type == TensorProto.BFLOAT16:   # (numpy holds its values in float32)
+                extra[-1].data_type = TensorProto.BFLOAT16
         model.graph.node = kept
         model.graph.initializer = list(model.graph.initializer) + extra
         return model
