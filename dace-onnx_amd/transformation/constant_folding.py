@@ -15,6 +15,8 @@ numpy, for the operators that exporters use in such constant subgraphs. Two deli
 * ``Transpose`` of a large weight (``nn.Linear`` exports its ``[out, in]`` weight behind one) is left in
   the graph: the fusion pass turns it into GEMM operand strides, which costs no copy and keeps the weight
   tied to the module parameter it came from.
+
+Of bfloat16, which numpy does not have, only ``Cast`` (to it with its rounding, and from it), ``ConstantOfShape`` and ``Shape`` are evaluated.
 """
 import copy
 import typing
@@ -22,7 +24,7 @@ import typing
 import numpy as np
 
 from ..onnx import proto
-from ..onnx.proto import ModelProto
+from ..onnx.proto import ModelProto, TensorProto
 
 #: a Transpose / Reshape / Identity result larger than this stays a node (see the module docstring)
 MAX_FOLDED_VIEW_ELEMENTS = 4096
@@ -39,6 +41,19 @@ def _axes(a, ins, idx):
     if len(ins) > idx and ins[idx] is not None:
         return [int(v) for v in np.asarray(ins[idx]).reshape(-1)]
     return None
+
+
+def _makes_bfloat16(node):
+    """Whether the node's result, which a rule below gives in float32, is one of bfloat16."""
+    a = _attrs(node)
+    if node.op_type == "Cast":
+        return int(a["to"]) == TensorProto.BFLOAT16
+    return node.op_type == "ConstantOfShape" and a.get("value") is not None and a["value"].data_type == TensorProto.BFLOAT16
+
+
+def _bfloat16(name, values, dims):
+    """The values, rounded, as a tensor of bfloat16; its array has them in float32."""
+    return proto.helper.make_tensor(name, TensorProto.BFLOAT16, dims, values)
 
 
 def _evaluate(node, ins: typing.List[typing.Optional[np.ndarray]]) -> typing.Optional[typing.List[np.ndarray]]:
@@ -103,8 +118,9 @@ def fold_constants(model: ModelProto) -> ModelProto:
     inputs (the module's parameters under ``keep_initializers_as_inputs``). The caller's model is not
     modified."""
     graph = model.graph
-    # (of bfloat16, which numpy does not have, nothing is computed here)
-    consts = {t.name: np.asarray(t.array).reshape(t.dims) for t in graph.initializer if t.data_type != proto.TensorProto.BFLOAT16}
+    consts = {t.name: np.asarray(t.array).reshape(t.dims) for t in graph.initializer if t.data_type != TensorProto.BFLOAT16}
+    # those of bfloat16, which numpy does not have: nothing but a Cast and a Shape looks at them here
+    halves = {t.name: t for t in graph.initializer if t.data_type == TensorProto.BFLOAT16}
     listed = {v.name for v in graph.input}
     static_shapes = {v.name: v.shape for v in list(graph.input) + list(graph.value_info) + list(graph.output)
                      if v.shape is not None and all(isinstance(d, int) for d in v.shape)}
@@ -113,13 +129,18 @@ def fold_constants(model: ModelProto) -> ModelProto:
         outs = None
         if node.op_type == "Shape" and len(node.input) == 1:
             src = node.input[0]
-            shape = consts[src].shape if src in consts else static_shapes.get(src)
+            shape = consts[src].shape if src in consts else halves[src].dims if src in halves else static_shapes.get(src)
             if shape is not None:
                 outs = [np.asarray(shape, dtype=np.int64)]
         elif node.input and all(name == "" or name in consts for name in node.input):
             outs = _evaluate(node, [consts[name] if name else None for name in node.input])
+        elif node.op_type == "Cast" and node.input[0] in halves:
+            outs = _evaluate(node, [_bfloat16(node.input[0], halves[node.input[0]].array, halves[node.input[0]].dims).array])
         if outs is None or len(outs) != len(node.output):
             kept.append(node)
+            continue
+        if _makes_bfloat16(node):
+            halves[node.output[0]] = folded[node.output[0]] = _bfloat16(node.output[0], outs[0], np.shape(outs[0]))
             continue
         for name, value in zip(node.output, outs):
             consts[name] = folded[name] = np.asarray(value)
@@ -130,7 +151,7 @@ def fold_constants(model: ModelProto) -> ModelProto:
     model.graph = copy.copy(graph)
     model.graph.node = kept
     model.graph.initializer = [t for t in graph.initializer if t.name in used or t.name in listed] + \
-        [proto.numpy_helper.from_array(v, name=k) for k, v in folded.items() if k in used]
+        [v if isinstance(v, TensorProto) else proto.numpy_helper.from_array(v, name=k) for k, v in folded.items() if k in used]
     # value_info of a folded value would contradict nothing, but is dead weight
     model.graph.value_info = [v for v in graph.value_info if v.name not in folded or v.name in used]
     return model
