@@ -79,7 +79,7 @@ struct DiffTile {
 __device__ __forceinline__ void diff_to_lds(const void* base, uint32_t offset, uint32_t lds) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint64_t uniform = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(uniform) : "memory", "m0");
 }
 
 // Eight values of an operand as the matrix unit takes them: one vector of 16-bit numbers, or a float32 as the sum of three bfloat16 numbers, its

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(512) void qlin_direct_kernel(QLinArgs p) {
 // 16 bytes to a lane from global memory, base + the lane's offset, into LDS at lds + 16 lane; base and lds are the same for the wave, all 16-byte aligned.
 // Written as assembly because the compiler waits for every builtin transfer before the next LDS read.
 __device__ __forceinline__ void qlin_to_lds(const int8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(base) : "memory", "m0");
 }
 
 // Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, NS stages. A row's 128 bytes of a step are eight
