@@ -154,6 +154,14 @@ __device__ __forceinline__ void qlin_to_lds(const int8_t* base, uint32_t offset,
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(base) : "memory", "m0");
 }
 
+// What the lanes of a wave wrote to LDS before is read by the others after it, and the other way round. LDS operations of a wave complete in order, so this takes no
+// instruction: it keeps the compiler, which sees the addresses of one lane, from moving one across the other.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // Tiles through LDS: WM x WN waves of 32 TM rows and 32 TN columns each, steps of 128 k, NS stages. A row's 128 bytes of a step are eight
 // pieces of 16; piece c of row r lies at c ^ (r / 2 % 8), so that the 16 rows whose
 // pieces are read at a time lie in 16 different places of the 256 bytes that the banks hold. DIRECT (rows at
@@ -295,6 +303,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
             for (int g = 0; g < 4; ++g)
                 *reinterpret_cast<f32x4*>(mine + at(l32, 32 * u + 8 * g + 4 * h)) =
                     f32x4{(float)acc[t][u][4 * g] * xs, (float)acc[t][u][4 * g + 1] * xs, (float)acc[t][u][4 * g + 2] * xs, (float)acc[t][u][4 * g + 3] * xs};
+        wave_lds_fence();   // lanes read what others wrote
 #pragma unroll
         for (int i0 = 0; i0 < COUNT; i0 += BATCH) {
             float res[BATCH][4];
@@ -318,6 +327,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qlin_tile_kernel(QLinArgs p, int
                 store_values(static_cast<T*>(p.Y) + (m + row) * p.N + n, v, m + row < p.M ? left : 0);
             }
         }
+        wave_lds_fence();   // the next 32 rows go where others have read
     }
 }
 

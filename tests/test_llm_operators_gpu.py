@@ -634,3 +634,17 @@ def test_attention_in_parts_as_a_recorded_graph_and_as_a_single_call():
             torch.cuda.default_stream().wait_stream(stream)
             assert torch.equal(out, o)
             out.zero_()
+
+
+@pytest.mark.parametrize("form", range(5))
+@pytest.mark.parametrize("m, n, k", [(512, 512, 64), (300, 270, 144), (257, 515, 33)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_results_of_a_tile_are_where_they_belong(form, m, n, k, residual, tuning):
+    """Whole numbers, equal to the last bit: no row of a tile has another's results, whichever lanes hand them round."""
+    tuning(MI355X_QLIN_FORM=form)
+    x, w, one = eight(1, m, k), eight(2, n, k), torch.ones(1, device="cuda")
+    r = eight(3, m, n).float() if residual else None
+    expected = (x.double() @ w.double().t() + (r.double() if residual else 0)).float()
+    for _ in range(3):
+        y, = R.call("QuantizedLinear", [("x", x), ("w", w), ("xs", one), ("ws", one), ("b", None), ("r", r)], [("y", F32, (m, n))])
+        assert torch.equal(y, expected)
