@@ -1,5 +1,7 @@
 """The nodes of quantised and differential transformers without a GPU: shapes, refusals of nodes and of the C interface, bfloat16 on the host,
 and the definitions in ``llm_operators`` against elementary sums."""
+import glob
+import os
 import re
 
 import numpy as np
@@ -245,3 +247,29 @@ def test_definitions_by_elementary_sums():
             expected = sum((p1[j] / sum(p1) - weight * p2[j] / sum(p2)) * v[0, j, 0] for j in range(2 + i))
             assert torch.allclose(out[0, i, h], expected)
     assert R.differential_attention(q, k, v, vectors, 0.2, lengths=torch.tensor([1]), causal=True)[0][0, 0].abs().max() == 0
+
+
+# ---------------------------------------------------------------------------------------------- the documented layer
+
+
+def test_the_documented_layer_can_be_built():
+    """The nodes that the documentation lists for a layer are a graph: every name is an input of the layer, one of its weights or another node's result."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    texts = [open(path).read() for path in glob.glob(os.path.join(root, "*.md"))]
+    block, = [b for text in texts for b in re.findall(r"```python\n(.*?)```", text, re.S) if 'node("DifferentialAttention"' in b]
+    nodes = []
+    exec(block, {"node": lambda op, inputs, outputs, **attributes: nodes.append(proto.helper.make_node(op, inputs, outputs, **attributes))})   # noqa: S102
+    B, S, H, G, d = 2, 5, 4, 2, 64
+    hidden, T, helper = 2 * H * d, proto.TensorProto, proto.helper
+    inputs = {"x": (T.BFLOAT16, [B, S, hidden]), "skip": (T.BFLOAT16, [B, S, hidden]), "positions": (T.INT64, [3, B, S]), "lengths": (T.INT32, [B])}
+    weights = {"gain": (T.BFLOAT16, [hidden]), "head_gain": (T.BFLOAT16, [2 * d]), "o_gain": (T.BFLOAT16, [hidden]), "frequencies": (T.FLOAT, [d // 2]),
+               **{"lambda_" + n: (T.FLOAT, [d]) for n in ("q1", "k1", "q2", "k2")}}
+    for name, columns in (("wq", 2 * H * d), ("wk", 2 * G * d), ("wv", 2 * G * d), ("wo", hidden)):
+        weights[name], weights[name + "_scale"] = (T.INT8, [columns, hidden]), (T.FLOAT, [columns])
+    shapes = {"q_shape": [B, S, 2 * H, d], "k_shape": [B, S, 2 * G, d], "v_shape": [B, S, G, 2 * d], "o_shape": [B, S, hidden]}
+    made = {name for n in nodes for name in n.output}
+    assert {name for n in nodes for name in n.input if name} - made == {*inputs, *weights, *shapes}
+    initializers = [helper.make_tensor(n, t, shape, np.ones(shape)) for n, (t, shape) in weights.items()] + [proto.numpy_helper.from_array(np.array(v), n) for n, v in shapes.items()]
+    graph = helper.make_graph(nodes, "layer", [helper.make_tensor_value_info(n, *v) for n, v in inputs.items()],
+                              [helper.make_tensor_value_info(n, T.BFLOAT16, [B, S, hidden]) for n in ("out", "stream")], initializer=initializers)
+    assert [c.function for c in _functions(donnx.ONNXModel("documented", helper.make_model(graph)))].count("mi355x_quantized_linear") == 4
