@@ -648,3 +648,11 @@ def test_linear_results_of_a_tile_are_where_they_belong(form, m, n, k, residual,
     for _ in range(3):
         y, = R.call("QuantizedLinear", [("x", x), ("w", w), ("xs", one), ("ws", one), ("b", None), ("r", r)], [("y", F32, (m, n))])
         assert torch.equal(y, expected)
+
+
+@pytest.mark.parametrize("dtype, d", [(BF, 128), (F16, 128), (F32, 64)])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_attention_of_many_rows_of_wide_heads_in_parts(dtype, d, causal):
+    """Heads of 256 bytes with more than 128 blocks of 32 rows: two row waves and two key waves to a workgroup, and the keys in parts."""
+    assert _lib.library().mi355x_differential_attention_splits(2, 2100, 2200, 1, 1, d, R.ELEMENT[dtype]) > 1
+    check_attention(2, 2100, 2200, 1, 1, d, dtype, causal=causal, lengths=[2200, 2101])
