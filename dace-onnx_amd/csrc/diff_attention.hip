@@ -10,7 +10,8 @@
 //     values V's operand comes from LDS by transposing reads, with float32 by 4-byte reads (and is split in three, see Operand). Every lane has one row: a running maximum that
 //     changes is one factor to a lane.
 //   * Keys and values are staged through LDS for all waves, 16-byte pieces permuted within a row so that reads of a column meet no bank twice.
-// P is rounded to the arrays' type for the second product, half a step of it; the sum is that of the rounded values.
+// P is rounded to the arrays' type for the second product, half a step of it, because the matrix unit takes it in no more than 16 bits at the rate of that type (errors of
+// bfloat16 results in the 2-norm 1.8e-3, where rounding the results alone gives 1.7e-3); the sum is that of the rounded values, so that the weights add up to one.
 // Few rows: the keys are dealt to `splits` workgroups, whose maxima, sums and outputs a second launch joins.
 // Bound by matrix and vector instructions one after the other (a vector instruction takes its time from the matrix pipe): 768 cycles of products and about 1000 of exponentials,
 // maxima and roundings for 32 keys, 64 rows and a map of 64. 8 heads of 64 over 8192 queries and keys in bfloat16: 382 us, 1.08 PFLOP/s of the 12 d operations that one
@@ -83,8 +84,9 @@ __device__ __forceinline__ void diff_to_lds(const void* base, uint32_t offset, u
 }
 
 // Eight values of an operand as the matrix unit takes them: one vector of 16-bit numbers, or a float32 as the sum of three bfloat16 numbers, its
-// first, middle and last eight bits. Of the nine partial products of two such values the six largest are taken; those left out are below 2^-23 of the
-// product. (An infinity is no such sum: it gives NaN.)
+// first, middle and last eight bits, cut off one after the other: all of its sign. Of the nine partial products of two such values the six largest are taken; those left out are
+// below 2^-21 of the product (both values 1 + 2^-7 - 2^-23: 2^-21.0; 2^-24.5 on average), always towards zero. Parts to the nearest would leave half of that and less to either
+// side, but the first part of values from 2^128 - 2^119 on would be infinite. (An infinity is no such sum: it gives NaN.)
 template <class T>
 struct Operand {
     typedef T Vector __attribute__((ext_vector_type(8)));
@@ -711,6 +713,7 @@ extern "C" int64_t mi355x_differential_attention_splits(int64_t batch, int64_t S
     const DiffCut whole = diff_cut(rows, slices, Sq, Sk, bytes, 0, false), part = diff_cut(rows, slices, Sq, Sk, bytes, 0, true);
     const int forced = tuning().diff_splits;
     if (forced > 0) return std::min(forced, 256);
+    // A causal call is priced as one without a mask: every row as if it saw all keys, and of one part the form that the call would take without the mask.
     // By what a workgroup's stages take, what joining takes (a launch, and the sums written and read), and one round of workgroups at most. Measured, microseconds: 8 x 1 of
     // 8192 keys, 16 heads in 4 groups, 64, bfloat16: 100 in one part (FEW), 32 in 8, 28 in 16, 32 in 32 (SMALL); 1 x 1 of them 16.1 in 16, 13.0 in 32; 16 x 1 of 1000 keys, 8 heads,
     // float16: 20.6 in one part, 19.7 in 2, 17.7 in 4; 512 of 512, 8 heads: 11.3 and 18.2; float32: 333 of 333, 6 heads of 64, 24.8 in one part, 21.7 in 2, 19.5 in 3; 8 heads

@@ -1,4 +1,4 @@
-// Arrays of float32, float16 or bfloat16 that are computed with in float32.
+// Arrays of float32, float16 or bfloat16 whose values are read as float32 and rounded when they are stored.
 #pragma once
 
 #include "common.h"

@@ -6,9 +6,10 @@
 // |y|; both are exchanged in the wave by DPP and between waves through LDS.
 //   rms_norm_rows<T, TH, NV>  TH threads to a row, NV vectors of 16 bytes to a thread: a wave while two vectors to a lane hold the row, then 256 threads, whose loads are in
 //                             flight together, then 1024, so that no thread holds more than 32 values and their residuals
-//   rms_norm_long             longer rows: one workgroup sweeps them three times
+//   rms_norm_long             longer rows: one workgroup sweeps them three times, element by element: 1024 x 40000 in float32 240 us, 0.49 GB at 2 TB/s
 // Bound by the bytes: 16384 x 4096 in bfloat16 with residual, sum and eight bits 84 us, 5.6 TB/s (a copy of 1 GiB 5.1); 1777 x 1001 in float32 7.1 us. Few rows by the
-// launch and three trips (memory, two exchanges): 4 x 2048 3.2 us, of which an empty launch is 1.6. Rows at any address: 16-byte accesses wherever they lie.
+// launch and three trips (memory, two exchanges): 4 x 2048 3.2 us, of which an empty launch is 1.6. Rows at any address: 16-byte accesses wherever they lie. Narrow rows leave lanes
+// idle: 128 values in bfloat16, a norm of each head, are 16 vectors for the 64 lanes of a wave: 65536 of them 20 us, 1.7 TB/s.
 #include "mixed.h"
 
 namespace mi355x {

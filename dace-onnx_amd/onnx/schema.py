@@ -75,7 +75,7 @@ _FLOATS = [dace.float16, dace.float32, dace.float64]
 _NUMERIC = _FLOATS + [dace.int32, dace.int64, dace.uint8, dace.int8, dace.int16]
 _ANY = _NUMERIC + [dace.bool_]
 _HELD = _ANY + [dace.bfloat16]   # of nodes that move values without looking at them
-_MIXED = [dace.float32, dace.float16, dace.bfloat16]   # of nodes that compute in float32 whatever their arrays hold
+_MIXED = [dace.float32, dace.float16, dace.bfloat16]   # of nodes that compute in float32 whatever their arrays hold, but for DifferentialAttention's probabilities
 
 
 def _unary(name, version, in_name, out_name, types=_FLOATS, attributes=(), doc=""):
@@ -176,8 +176,9 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "K [B, Sk, 2 G, d] hold the two maps of a head next to each other, V is [B, Sk, G, 2 d], O [B, Sq, H, 2 d]; H / G heads "
                "share keys and values. Keys from lengths[b] on do not exist; if `causal`, query i sees the keys up to i + lengths[b] - Sq. A row "
                "without keys is 0. `scale` is 1 / sqrt(d) if it is left out. Prompts padded behind their end need no lengths if `causal`: no valid "
-               "query sees the padding. In float32 an infinite query, key or value that a row sees makes it not a number, and so may, in any type, a value "
-               "that is not finite of a later key that a neighbouring row of a `causal` call sees."),
+               "query sees the padding. In float16 and bfloat16 the probabilities are rounded to that type for their product with V. "
+               "In float32 an infinite query, key or value that a row sees makes it not a number; in any type an infinite value that it sees makes it infinite or not a "
+               "number, and so may a value that is not finite of a later key that a neighbouring row of a `causal` call sees."),
     # Pad only ever runs folded into the Conv that reads it (transformation/fusion.py, the reference's PadConvFusion)
     ONNXSchema("Pad", 11,
                [ONNXParameter("data", "T"), ONNXParameter("pads", "tensor(int64)"), ONNXParameter("constant_value", "T", _O)],

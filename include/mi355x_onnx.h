@@ -452,8 +452,8 @@ int mi355x_cast(const void* X, int from_type, void* Y, int to_type, int64_t n,
 
 /* ---- quantised and differential transformers ------------------------------------------------------------
  * The reference has none of these nodes. Arrays of element type `type` (MI355X_TYPE_FLOAT, MI355X_TYPE_FLOAT16 or
- * MI355X_TYPE_BFLOAT16) are computed with in float32 and rounded once, to the nearest; all arrays are C-contiguous, at
- * any address of their element type. */
+ * MI355X_TYPE_BFLOAT16) are computed with in float32 and rounded once, to the nearest, but for what is said at
+ * mi355x_differential_attention; all arrays are C-contiguous, at any address of their element type. */
 #define MI355X_TYPE_FLOAT16 10
 #define MI355X_TYPE_BFLOAT16 16
 
@@ -480,7 +480,8 @@ int mi355x_quantized_linear(const int8_t* X, const int8_t* W, const float* x_sca
  * same launch, K [tokens, kv_heads, size] to K_out (either count may be 0). `rotated` values of a head are turned: pairs
  * are i and i + rotated / 2, neighbours 2 i and 2 i + 1 if `interleaved`; the others are copied. positions
  * [axes, tokens] are integers of position_bytes (4 or 8), frequencies [rotated / 2] float32; sections[axes] (host
- * memory) says how many pairs, in order, belong to each axis. axes <= 8. Q_out may be Q itself, K_out may be K. */
+ * memory) says how many pairs, in order, belong to each axis. axes <= 8. Q_out may be Q itself, K_out may be K. An angle
+ * is right to 2^-51 of its turns (positions of 2^40: 5e-4), and to 2e-7 besides. */
 int mi355x_rotary_positions(const void* Q, const void* K, const void* positions, const float* frequencies, void* Q_out,
                             void* K_out, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t rotated,
                             int64_t axes, const int64_t* sections, int interleaved, int position_bytes, int type,
@@ -494,9 +495,12 @@ int mi355x_rotary_positions(const void* Q, const void* K, const void* positions,
  * count as the nearer of the two. If `causal`, query i sees the keys up to i + length - Sq. A row that sees no key is 0.
  * `splits` workgroups share the keys of a row, 1 to 256; mi355x_differential_attention_splits says how many pay. From 2 on
  * `scratch` has room for splits * batch * Sq * heads * (4 size + 4) floats, 16-byte aligned, and belongs to the
- * call until it is done. Of values that a row does not see, but another row of the entry does, an infinity or NaN
- * may still reach it; lengths keep them out. In float32 an infinite query, key or value that a row sees makes it not a
- * number, and values below 2^-110 lose digits (others are exact in the products' operands). */
+ * call until it is done. With arrays of 16 bits the probabilities are rounded to `type` for their product with V, and their
+ * sum is that of the rounded ones; scores, maxima, sums and results stay in float32. Of values that a row does not see, but
+ * another row of the entry does, an infinity or NaN may still reach it; lengths keep them out. An infinite value that a row
+ * sees makes it infinite or not a number (the maps' shares are subtracted); in float32 an infinite query, key or value
+ * makes it not a number, and values below 2^-110 lose digits (others are exact in the products' operands; of a product
+ * less than 2^-21 is left out). A map all of whose scores are minus infinity counts as 0. */
 int64_t mi355x_differential_attention_splits(int64_t batch, int64_t Sq, int64_t Sk, int64_t heads, int64_t groups,
                                              int64_t size, int type);
 int mi355x_differential_attention(const void* Q, const void* K, const void* V, const float* lambda_q1,
