@@ -11,7 +11,7 @@
 //     changes is one factor to a lane.
 //   * Keys and values are staged through LDS for all waves, 16-byte pieces permuted within a row so that reads of a column meet no bank twice.
 // P is rounded to the arrays' type for the second product, half a step of it, because the matrix unit takes it in no more than 16 bits at the rate of that type (errors of
-// bfloat16 results in the 2-norm 1.8e-3, where rounding the results alone gives 1.7e-3); the sum is that of the rounded values, so that the weights add up to one.
+// bfloat16 results in the 2-norm 1.7e-3 to 2.0e-3, where rounding the results alone gives 1.7e-3); the sum is that of the rounded values, so that the weights add up to one.
 // Few rows: the keys are dealt to `splits` workgroups, whose maxima, sums and outputs a second launch joins.
 // Bound by matrix and vector instructions one after the other (a vector instruction takes its time from the matrix pipe): 768 cycles of products and about 1000 of exponentials,
 // maxima and roundings for 32 keys, 64 rows and a map of 64. 8 heads of 64 over 8192 queries and keys in bfloat16: 382 us, 1.08 PFLOP/s of the 12 d operations that one
