@@ -99,6 +99,11 @@ SIGNATURES: typing.Dict[str, typing.Tuple[typing.Any, typing.List[typing.Any]]] 
     "mi355x_differential_attention_splits": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
     "mi355x_differential_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                              _f32, _f32, _int, _i64, _int, _vp]),
+    "mi355x_paged_cache_append": (_int, [_vp] * 11 + [_i64] * 11 + [_c_i64_p, _int, _int, _int, _vp]),
+    "mi355x_tree_attention_scratch": (_i64, [_i64] * 7 + [_int]),
+    "mi355x_tree_attention": (_int, [_vp] * 8 + [_i64] * 9 + [_f32, _int, _vp]),
+    "mi355x_draft_acceptance_scratch": (_i64, [_i64, _i64, _i64, _int]),
+    "mi355x_draft_acceptance": (_int, [_vp] * 7 + [_i64] * 4 + [_int, _vp]),
     "mi355x_program_function": (_int, [ctypes.c_char_p]),
     "mi355x_program_run": (_i64, [_vp, _i64, _i64, _vp, _i64, _vp, _vp]),
 }

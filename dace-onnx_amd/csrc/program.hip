@@ -66,7 +66,8 @@ constexpr Function kFunctions[] = {
     MI355X_FUNCTION(mi355x_maxpool2d_f32), MI355X_FUNCTION(mi355x_batchnorm_f32), MI355X_FUNCTION(mi355x_eltwise_f32),
     MI355X_FUNCTION(mi355x_eltwise_program_f32), MI355X_FUNCTION(mi355x_permute_b32), MI355X_FUNCTION(mi355x_cast),
     MI355X_FUNCTION(mi355x_skip_rms_norm), MI355X_FUNCTION(mi355x_quantized_linear), MI355X_FUNCTION(mi355x_rotary_positions),
-    MI355X_FUNCTION(mi355x_differential_attention)};
+    MI355X_FUNCTION(mi355x_differential_attention), MI355X_FUNCTION(mi355x_paged_cache_append), MI355X_FUNCTION(mi355x_tree_attention),
+    MI355X_FUNCTION(mi355x_draft_acceptance)};
 #undef MI355X_FUNCTION
 constexpr int kNumFunctions = sizeof(kFunctions) / sizeof(kFunctions[0]);
 

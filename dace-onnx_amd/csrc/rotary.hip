@@ -2,21 +2,18 @@
 // height, width) a run of the pairs. Queries and keys in one launch, arrays in float32, float16 or bfloat16, computed in float32. The reference has
 // no such node.
 //
-// An angle is an integer position times a float32 frequency, in float64: exact for positions below 2^29, rounded from there on. It is counted in turns, by a rounded
-// factor, and brought into one turn there: off by less than 2^-51 of the turns in all (position 2^40 at frequency 1: 5e-4 radians). Positions far into a context
-// are thousands of turns, of which float32 would leave few right digits (position 100000: 0.004 radians). What is left is rounded to float32, pi 2^-24 of an angle at most, and its
-// cosine and sine are float32: float32 results are off by 4.9e-8 in the 2-norm, where cosine and sine taken in float64 give 3.6e-8.
 // A workgroup has a few tokens: their angles are computed once, into LDS, and then serve all heads. Four tokens keep enough loads of a thread in flight and leave the
 // angles' float64 hidden behind other workgroups' bytes. Bound by the bytes of the heads: 32768 tokens of 16 + 4 heads of 128 in bfloat16 61 us, 5.5 TB/s (a copy of 1
 // GiB 5.1); 4616 tokens of 12 heads of 64, 48 of them turned, in float32 7.6 us. One token to a request, 8 x 40 heads: 4.4 us by two workgroups of four
 // tokens, whose threads go through the heads in five rounds; few tokens are not dealt to more workgroups.
 #include "mixed.h"
+#include "rotary.h"
 
 #include <algorithm>
 
 namespace mi355x {
 
-constexpr int ROTARY_MAX_AXES = 8, ROTARY_THREADS = 256, ROTARY_LDS_ANGLES = 2048;
+constexpr int ROTARY_THREADS = 256;
 
 struct RotaryArgs {
     const void* q; const void* k; const void* positions; const float* frequencies;
@@ -41,10 +38,7 @@ __global__ __launch_bounds__(ROTARY_THREADS) void rotary_positions_kernel(Rotary
         while (axis + 1 < p.axes && pair >= p.end[axis]) ++axis;
         const int64_t at = axis * p.tokens + token0 + token;
         const int64_t position = p.wide_positions ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
-        const double turns = (double)position * (double)p.frequencies[pair] * 0.15915494309189533577;
-        float sine, cosine;
-        sincospif((float)(2.0 * (turns - rint(turns))), &sine, &cosine);
-        turn[i] = make_float2(cosine, sine);
+        turn[i] = rotary_turn(position, p.frequencies[pair]);
     }
     __syncthreads();
 

@@ -40,6 +40,14 @@ def call_onnx_op(cls, **kwargs):
     # constants of this one-node graph, as initializers are in an imported model
     sdfg._constant_inputs = {}
     for conn, value in list(inputs.items()) + list(outputs.items()):
+        if conn in schema.updates and conn in outputs:   # the array of an input, which the node updates
+            source = schema.updates[conn]
+            if value is not inputs.get(source):
+                raise ValueError(f"{conn} is {source}, updated: both have to be the same array")
+            arr = "__" + source
+            state.add_edge(node, conn, state.add_write(arr), None, sdfg.make_array_memlet(arr))
+            node.add_out_connector(conn)
+            continue
         arr = "__" + conn
         if conn in inputs and isinstance(value, np.ndarray) and np.issubdtype(value.dtype, np.integer) and value.size <= 64:
             sdfg._constant_inputs[arr] = value.copy()

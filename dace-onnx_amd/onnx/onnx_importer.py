@@ -124,6 +124,7 @@ class ONNXModel:
         for node in model.graph.node:
             if not has_onnx_node(node.op_type):
                 raise ValueError("Unsupported ONNX operator: '{}'".format(node.op_type))
+        self._updates = self._updated_inputs(model.graph)   # output (or value) -> the input whose array it is
         if infer_shapes:
             model = _infer_shapes(model)
         graph = model.graph
@@ -150,7 +151,8 @@ class ONNXModel:
                 continue
             (self.inputs if is_input else self.outputs).append(value.name)
             self.value_infos[value.name] = value
-            self._add_value_info(value, transient=False)
+            if value.name not in self._updates:
+                self._add_value_info(value, transient=False)
         for value in graph.value_info:
             if not value.name:
                 raise ValueError("Got input or output without name")
@@ -179,14 +181,15 @@ class ONNXModel:
                                                       enumerate(zip(node.output, repeat(False)))):
                 if vname == "":
                     continue  # omitted optional parameter
-                if clean_onnx_name(vname) not in self.sdfg.arrays:
+                array = clean_onnx_name(self._updates.get(vname, vname))
+                if array not in self.sdfg.arrays:
                     if vname not in self.value_infos:
                         raise ValueError("Could not find array with name '{}'".format(vname))
                     self._add_value_info(self.value_infos[vname], transient=True)
                 if vname in access_nodes:
                     access = access_nodes[vname]
                 else:
-                    access = AccessNode(clean_onnx_name(vname))
+                    access = AccessNode(array)
                     self.state.add_node(access)
                     access_nodes[vname] = access
                 params = op_node.schema.inputs if is_input else op_node.schema.outputs
@@ -202,7 +205,7 @@ class ONNXModel:
                     conn_name = params[param_idx].name + "__0"
                 else:
                     conn_name = params[param_idx].name
-                memlet = self.sdfg.make_array_memlet(clean_onnx_name(vname))
+                memlet = self.sdfg.make_array_memlet(array)
                 if is_input:
                     op_node.add_in_connector(conn_name)
                     self.state.add_edge(access, None, op_node, conn_name, memlet)
@@ -288,6 +291,30 @@ class ONNXModel:
             renamed.name = new_name
             graph.output[i] = renamed
         return model
+
+    @staticmethod
+    def _updated_inputs(graph) -> typing.Dict[str, str]:
+        """Value -> the graph input whose array it is, for the nodes of ``graph`` that update arrays (``ONNXSchema.updates``). Such an array is one that the
+        caller keeps, and what it held before the call is read by nobody but the node: after it, everybody reads the node's output."""
+        inputs, constants = {v.name for v in graph.input}, {t.name for t in graph.initializer}
+        reads = collections.Counter(name for node in graph.node for name in node.input)
+        returned = {o.name for o in graph.output}
+        updates = {}
+        for node in graph.node:
+            schema = get_onnx_node(node.op_type).schema
+            place = {p.name: i for i, p in enumerate(schema.inputs)}
+            for i, parameter in enumerate(schema.outputs):
+                name = node.output[i] if i < len(node.output) else ""
+                if parameter.name not in schema.updates or not name:
+                    continue
+                source = schema.updates[parameter.name]
+                value = node.input[place[source]] if place[source] < len(node.input) else ""
+                if value not in inputs or value in constants:
+                    raise ValueError(f"{node.op_type} '{node.name}' updates '{value}' ({source}), which has to be an input of the graph and no initializer")
+                if reads[value] > 1 or value in returned:
+                    raise ValueError(f"{node.op_type} '{node.name}' updates '{value}' ({source}): other readers of it take the node's output '{name}'")
+                updates[name] = value
+        return updates
 
     @staticmethod
     def _convert_attribute(attr):
@@ -455,12 +482,16 @@ class ONNXModel:
             raise TypeError(f"missing model inputs {missing}")
         return inputs
 
+    def _fresh_outputs(self):
+        """The outputs that are no arrays of the caller's."""
+        return [n for n in self.outputs if n not in self._updates] if self._updates else self.outputs
+
     def _host_plan(self):
         """What calls with tensors on the GPU take from the second on; False where there is no such way for this model."""
         if self._compiled._bound is None:
             return None
         clean = clean_onnx_name
-        return self._compiled.host_plan({clean(n): i for i, n in enumerate(self.inputs)}, {clean(n): i for i, n in enumerate(self.outputs)},
+        return self._compiled.host_plan({clean(n): i for i, n in enumerate(self.inputs)}, {clean(n): i for i, n in enumerate(self._fresh_outputs())},
                                         {clean(n): n for n in self.weights}, {c.array: i for i, c in enumerate(self._packed)}) or False
 
     def _call_by_plan(self, args):
@@ -471,13 +502,19 @@ class ONNXModel:
             self._plan = self._host_plan()
         if not self._plan:
             return None
-        return self._compiled.run_plan(self._plan, self.weights, self._packed, args)
+        results = self._compiled.run_plan(self._plan, self.weights, self._packed, args)
+        if results is None or not self._updates:
+            return results
+        fresh = iter(results)
+        return [args[self.inputs.index(self._updates[n])] if n in self._updates else next(fresh) for n in self.outputs]
 
     def __call__(self, *args, **kwargs):
         """Execute the model.
 
         Calls of one model share its intermediate arrays: they follow one another on one stream, or the caller makes one wait for the other. Calls
         of a model without any (no transient among ``sdfg.arrays`` once it is compiled) may overlap on several streams and threads.
+
+        An input that a node updates (a cache) is a contiguous tensor on the model's device; the output that it becomes is that tensor.
 
         :param args: positional arguments; the i-th is the i-th graph input.
         :param kwargs: named arguments matching the ONNX input names.
@@ -491,9 +528,13 @@ class ONNXModel:
         compiled = self.compile_and_init()
         inputs = self._call_args(args, kwargs)
         use_torch = any(isinstance(v, torch.Tensor) for v in inputs.values())
+        updated = {clean_onnx_name(n) for n in self._updates.values()}
         call = {}
         for n, v in inputs.items():
             desc = self.sdfg.arrays[clean_onnx_name(n)]
+            if n in self._updates.values() and not (isinstance(v, torch.Tensor) and v.device == self.device and v.is_contiguous() and tuple(v.shape) == desc.shape
+                                                    and v.dtype == desc.dtype.as_torch()):
+                raise TypeError(f"input '{n}' is updated where it lies: it has to be a contiguous tensor of {desc.dtype}{list(desc.shape)} on {self.device}")
             if isinstance(v, torch.Tensor):
                 v = v.to(self.device)
                 if not v.is_contiguous():
@@ -504,18 +545,21 @@ class ONNXModel:
         outputs = collections.OrderedDict()
         packed = self._packed_now() if self._packed else []
         if self.use_hip_graph:
+            if self._static_io is not None and any(self._static_io[0][k].data_ptr() != call[k].data_ptr() for k in updated):
+                self._static_io = self._recorded_packed = None   # another cache: the recording is made anew
             if self._static_io is None:
-                # private input/output buffers: the graph is bound to their addresses
-                s_in = {k: v.clone() for k, v in call.items()}
+                # private input/output buffers: the graph is bound to their addresses, and to those of the arrays that it updates
+                s_in = {k: v if k in updated else v.clone() for k, v in call.items()}
                 s_out = {}
-                for n in self.outputs:
+                for n in self._fresh_outputs():
                     desc = self.sdfg.arrays[clean_onnx_name(n)]
                     s_out[clean_onnx_name(n)] = torch.empty(desc.shape, dtype=desc.dtype.as_torch(), device=self.device)
                 self._static_io = (s_in, s_out, self._own_weights())
             else:
                 s_in, s_out, _ = self._static_io
                 for k, v in call.items():
-                    s_in[k].copy_(v)
+                    if k not in updated:
+                        s_in[k].copy_(v)
             if packed != self._recorded_packed:
                 # an eager run, which binds the launch list, for the recording. Weights are the tensors of the first call, written or
                 # not: a launch reads a weight that was written, or replaced, itself from here on.
@@ -524,12 +568,15 @@ class ONNXModel:
                 self._recorded_packed = packed
             else:
                 compiled.replay()
-            outputs = collections.OrderedDict((n, s_out[clean_onnx_name(n)].clone()) for n in self.outputs)
+            outputs = collections.OrderedDict((n, call[clean_onnx_name(self._updates[n])] if n in self._updates else s_out[clean_onnx_name(n)].clone()) for n in self.outputs)
         else:
             for n in self.outputs:
+                if n in self._updates:
+                    outputs[n] = call[clean_onnx_name(self._updates[n])]
+                    continue
                 desc = self.sdfg.arrays[clean_onnx_name(n)]
                 outputs[n] = torch.empty(desc.shape, dtype=desc.dtype.as_torch(), device=self.device)
-            out_kwargs = {clean_onnx_name(n): t for n, t in outputs.items()}
+            out_kwargs = {clean_onnx_name(n): t for n, t in outputs.items() if n not in self._updates}
             if self.save_transients is not None:
                 for k in self._saved:
                     desc = self.sdfg.arrays[k]

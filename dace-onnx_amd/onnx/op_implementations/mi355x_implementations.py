@@ -1027,6 +1027,151 @@ class MI355XDifferentialAttention(ONNXForward):
 
 
 # ------------------------------------------------------------------------------------
+# a cache in pages, and drafted tokens over it (no node of the reference's)
+
+
+def _updates_in_place(node, state):
+    """Whether each output that the node's schema says is an input's array is that array."""
+    data = {e.dst_conn: e.data.data for e in state.in_edges(node)}
+    return all(e.data.data == data.get(node.schema.updates[e.src_conn]) for e in state.out_edges(node) if e.src_conn in node.schema.updates)
+
+
+@op_implementation(op="PagedCacheAppend", name=IMPLEMENTATION_NAME)
+class MI355XPagedCacheAppend(ONNXForward):
+    """Keys and values to their pages, keys and queries turned on the way, in one launch."""
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        K, V, k_pages, v_pages, table, lengths, frequencies, positions, order, Q, Q_out = _descs(
+            node, state, sdfg, ("K", "V", "k_pages", "v_pages", "table", "lengths", "frequencies", "positions", "order", "Q"), ("Q_out", ))
+        if (Q is None) != (Q_out is None) or not _updates_in_place(node, state):
+            return None
+        heads = [d for d in (K, V, k_pages, v_pages, Q, Q_out) if d is not None]
+        kind = _mixed_type(*heads)
+        if kind is None or any(len(d.shape) != 4 for d in heads) or not _contig(*(d for d in (table, lengths, frequencies, positions, order, *heads) if d is not None)):
+            return None
+        (B, S, G, D), (pages, _, page, _) = K.shape, k_pages.shape
+        if tuple(V.shape) != (B, S, G, D) or tuple(k_pages.shape) != (pages, G, page, D) or tuple(v_pages.shape) != (pages, G, page, D) or page < 1:
+            return None
+        if table.dtype != dace.int32 or len(table.shape) != 2 or table.shape[0] != B or lengths.dtype != dace.int32 or tuple(lengths.shape) != (B, ):
+            return None
+        if order is not None and (order.dtype != dace.int32 or len(order.shape) != 2 or order.shape[0] != B):
+            return None
+        if Q is not None and (order is not None or frequencies is None or (Q.shape[0], Q.shape[1], Q.shape[3]) != (B, S, D) or tuple(Q_out.shape) != tuple(Q.shape)):
+            return None
+        pairs, axes, sections = 0, 1, [0]
+        if frequencies is not None:
+            if not _is_f32(frequencies) or len(frequencies.shape) != 1:
+                return None
+            pairs = frequencies.shape[0]
+            if positions is not None:
+                if positions.dtype not in (dace.int32, dace.int64) or len(positions.shape) != 3 or tuple(positions.shape[1:]) != (B, S):
+                    return None
+                axes = positions.shape[0]
+            sections = [int(n) for n in node.sections] if node.sections is not None else [pairs] + [0] * (axes - 1)
+        elif positions is not None or node.sections is not None:
+            return None
+        if not 1 <= axes <= MI355XRotaryPositions.MAX_AXES or len(sections) != axes or min(sections) < 0 or sum(sections) != pairs or 2 * pairs > D:
+            return None
+        if pairs > 2048 or D > 1 << 16 or max(G, Q.shape[2] if Q is not None else 0) > 1 << 12 or page >= 1 << 31 or table.shape[1] >= 1 << 31:
+            return None
+        taken = S if order is None else order.shape[1]
+        return (B, S, Q.shape[2] if Q is not None else 0, G, D, pages, page, table.shape[1], taken, 2 * pairs, axes, sections,
+                positions.dtype.bytes if positions is not None else 8, kind)
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XPagedCacheAppend._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        *sizes, axes, sections, position_bytes, kind = MI355XPagedCacheAppend._plan(node, state, sdfg)
+        optional = lambda name: Ptr(name if _has_input(node, state, name) else None)  # noqa: E731
+        return kernel_call_for_node(node, state, "mi355x_paged_cache_append", [
+            Ptr("K"), Ptr("V"), optional("Q"), Ptr("k_pages"), Ptr("v_pages"), Ptr("Q_out" if _has_output(node, state, "Q_out") else None), Ptr("table"), Ptr("lengths"),
+            optional("frequencies"), optional("positions"), optional("order"), *sizes, axes, I64Array(sections), int(bool(node.interleaved)), position_bytes, kind, Stream()])
+
+
+@op_implementation(op="TreeAttention", name=IMPLEMENTATION_NAME)
+class MI355XTreeAttention(ONNXForward):
+    """Softmax attention over a cache in pages, its last tokens a chain or a tree; with few queries the keys are dealt to several workgroups, and a second
+    launch joins their sums, which stand in a transient of the graph."""
+
+    HEAD_SIZES = (64, 128, 256)
+    MAX_TREE = 1024   # its parents stand in LDS
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        Q, k_pages, v_pages, table, lengths, parents, O = _descs(node, state, sdfg, ("Q", "k_pages", "v_pages", "table", "lengths", "parents"), ("O", ))
+        kind = _mixed_type(Q, k_pages, v_pages, O)
+        if kind is None or any(len(d.shape) != 4 for d in (Q, k_pages, v_pages, O)) or not _contig(*(d for d in (Q, k_pages, v_pages, table, lengths, parents, O) if d is not None)):
+            return None
+        (B, S, H, D), (pages, G, page, _) = Q.shape, k_pages.shape
+        if D not in MI355XTreeAttention.HEAD_SIZES or not G or H % G or page < 1 or pages < 1 or tuple(O.shape) != (B, S, H, D):
+            return None
+        if tuple(k_pages.shape) != (pages, G, page, D) or tuple(v_pages.shape) != (pages, G, page, D):
+            return None
+        if table.dtype != dace.int32 or len(table.shape) != 2 or table.shape[0] != B or lengths.dtype != dace.int32 or tuple(lengths.shape) != (B, ):
+            return None
+        if parents is not None and (parents.dtype != dace.int32 or tuple(parents.shape) != (B, S) or S > MI355XTreeAttention.MAX_TREE):
+            return None
+        scale = float(D) ** -0.5 if node.scale is None else float(node.scale)
+        if not 0 < scale < float("inf") or page * table.shape[1] >= (1 << 31) - 1024 or S >= 1 << 31 or pages >= 1 << 31:
+            return None
+        return B, S, H, G, D, pages, page, table.shape[1], scale, kind
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XTreeAttention._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        B, S, H, G, D, pages, page, columns, scale, kind = MI355XTreeAttention._plan(node, state, sdfg)
+        floats = _lib.library().mi355x_tree_attention_scratch(B, S, H, G, D, page, columns, kind)
+        if floats:
+            scratch = sdfg.free_name(node.label + "_scratch")
+            sdfg.add_transient(scratch, [floats], dace.float32)
+            state.add_edge(node, "_scratch", state.add_write(scratch), None, sdfg.make_array_memlet(scratch))
+        return kernel_call_for_node(node, state, "mi355x_tree_attention", [
+            *(Ptr(c) for c in ("Q", "k_pages", "v_pages", "table", "lengths")), Ptr("parents" if _has_input(node, state, "parents") else None), Ptr("O"),
+            Ptr("_scratch" if floats else None), floats, B, S, H, G, D, pages, page, columns, scale, kind, Stream()])
+
+
+@op_implementation(op="DraftAcceptance", name=IMPLEMENTATION_NAME)
+class MI355XDraftAcceptance(ONNXForward):
+    """The largest logit of every row by several workgroups, and the walk along each tree behind them; what the workgroups found stands in a transient of the graph."""
+
+    @staticmethod
+    def _plan(node, state, sdfg):
+        logits, tokens, parents, path, count, after = _descs(node, state, sdfg, ("logits", "tokens", "parents"), ("path", "count", "next"))
+        kind = _mixed_type(logits)
+        whole = [d for d in (tokens, parents, path, count, after) if d is not None]
+        if kind is None or len(logits.shape) != 3 or not _contig(logits, *whole) or any(d.dtype != dace.int32 for d in whole):
+            return None
+        B, S, vocabulary = logits.shape
+        if any(tuple(d.shape) != (B, S) for d in (tokens, path, *([parents] if parents is not None else []))) or any(tuple(d.shape) != (B, ) for d in (count, after)):
+            return None
+        if not 1 <= S <= MI355XTreeAttention.MAX_TREE or not 1 <= vocabulary < 1 << 31:
+            return None
+        return B, S, vocabulary, kind
+
+    @staticmethod
+    def forward_can_be_applied(node, state: SDFGState, sdfg: SDFG) -> bool:
+        return MI355XDraftAcceptance._plan(node, state, sdfg) is not None
+
+    @staticmethod
+    def forward(node, state: SDFGState, sdfg: SDFG):
+        B, S, vocabulary, kind = MI355XDraftAcceptance._plan(node, state, sdfg)
+        words = _lib.library().mi355x_draft_acceptance_scratch(B, S, vocabulary, kind)
+        scratch = sdfg.free_name(node.label + "_scratch")
+        sdfg.add_transient(scratch, [words], dace.int64)
+        state.add_edge(node, "_scratch", state.add_write(scratch), None, sdfg.make_array_memlet(scratch))
+        return kernel_call_for_node(node, state, "mi355x_draft_acceptance", [
+            Ptr("logits"), Ptr("tokens"), Ptr("parents" if _has_input(node, state, "parents") else None), Ptr("path"), Ptr("count"), Ptr("next"), Ptr("_scratch"), words,
+            B, S, vocabulary, kind, Stream()])
+
+
+# ------------------------------------------------------------------------------------
 # elementwise
 
 

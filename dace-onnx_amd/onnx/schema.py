@@ -47,7 +47,8 @@ class ONNXTypeConstraint:
 
 
 class ONNXSchema:
-    def __init__(self, name, since_version, inputs, outputs, attributes=(), type_constraints=(), doc=""):
+    def __init__(self, name, since_version, inputs, outputs, attributes=(), type_constraints=(), doc="", updates=None):
+        """:param updates: output -> the input whose array it is: the node writes there and leaves the rest of the array as it was."""
         self.name = name
         self.since_version = since_version
         self.inputs: typing.List[ONNXParameter] = list(inputs)
@@ -55,6 +56,7 @@ class ONNXSchema:
         self.attributes = {a.name: a for a in attributes}
         self.type_constraints = {c.type_str: c for c in type_constraints}
         self.doc = doc
+        self.updates: typing.Dict[str, str] = dict(updates or {})
 
     def non_variadic_inputs(self):
         return [i.name for i in self.inputs if i.param_type != ONNXParameterType.Variadic]
@@ -179,6 +181,40 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "query sees the padding. In float16 and bfloat16 the probabilities are rounded to that type for their product with V. "
                "In float32 an infinite query, key or value that a row sees makes it not a number; in any type an infinite value that it sees makes it infinite or not a "
                "number, and so may a value that is not finite of a later key that a neighbouring row of a `causal` call sees."),
+    # The three below are not ONNX operators either: a cache of keys and values in pages, and what verifies drafted tokens over it.
+    ONNXSchema("PagedCacheAppend", 1,
+               [ONNXParameter("K", "T"), ONNXParameter("V", "T"), ONNXParameter("k_pages", "T"), ONNXParameter("v_pages", "T"), ONNXParameter("table", "I32"),
+                ONNXParameter("lengths", "I32"), ONNXParameter("frequencies", "U", _O), ONNXParameter("positions", "I", _O), ONNXParameter("order", "I32", _O),
+                ONNXParameter("Q", "T", _O)],
+               [ONNXParameter("k_pages_out", "T"), ONNXParameter("v_pages_out", "T"), ONNXParameter("Q_out", "T", _O)],
+               [ONNXAttribute("sections", _A.Ints), ONNXAttribute("interleaved", _A.Int, 0)],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("I32", [dace.int32]), ONNXTypeConstraint("I", [dace.int64, dace.int32]),
+                ONNXTypeConstraint("U", [dace.float32])],
+               "Writes keys and values [B, S, G, D] into the pages [pages, G, page, D] of a cache, which the node updates where it lies: token i of entry b "
+               "becomes number lengths[b] + i of the entry, which is row (number % page) of page table[b, number / page] (table [B, columns]); with `order` [B, N] "
+               "it is token order[b, j] that becomes number lengths[b] + j, and where order[b, j] is none of 0 to S - 1 nothing is written. Nor is anything where the "
+               "table has no column for a number, or a value that is no page. Numbers that two tokens of a call would write to one row of one page are the "
+               "caller's error: it holds either. With `frequencies` keys are turned on the way, and Q [B, S, H, D] to Q_out with them, as RotaryPositions does, by "
+               "`positions` [axes, B, S] or, without, the token's number in the entry; Q is not taken with `order`. A length below 0 counts as 0.",
+               updates={"k_pages_out": "k_pages", "v_pages_out": "v_pages"}),
+    ONNXSchema("TreeAttention", 1,
+               [ONNXParameter("Q", "T"), ONNXParameter("k_pages", "T"), ONNXParameter("v_pages", "T"), ONNXParameter("table", "I32"), ONNXParameter("lengths", "I32"),
+                ONNXParameter("parents", "I32", _O)],
+               [ONNXParameter("O", "T")], [ONNXAttribute("scale", _A.Float)],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("I32", [dace.int32])],
+               "O = softmax(scale Q K^T) V for the S tokens of each entry that PagedCacheAppend has written behind its first lengths[b]; Q, O [B, S, H, D], pages and "
+               "table as there, H / G heads share keys and values. Token i sees the lengths[b] before the call, itself and its ancestors: parents[b, i] is the token "
+               "whose child it is, a lower number, anything else makes it a child of what is before the call. Without `parents` it sees the tokens up to itself. A table "
+               "value that is no page counts as the nearest one, keys for which the table has no column do not exist, a row without keys is 0. `scale` is 1 / sqrt(D) if "
+               "it is left out. In float16 and bfloat16 the probabilities are rounded to that type for their product with the values."),
+    ONNXSchema("DraftAcceptance", 1,
+               [ONNXParameter("logits", "T"), ONNXParameter("tokens", "I32"), ONNXParameter("parents", "I32", _O)],
+               [ONNXParameter("path", "I32"), ONNXParameter("count", "I32"), ONNXParameter("next", "I32")], [],
+               [ONNXTypeConstraint("T", _MIXED), ONNXTypeConstraint("I32", [dace.int32])],
+               "The path from token 0 of each entry's tree along which every token is what the model says after its parent: the place of the largest of its logits "
+               "[B, S, vocabulary], the first of equal ones, numbers only. path [B, S]: the tokens' places, then -1 (what PagedCacheAppend takes as `order`); "
+               "count [B]: how many; next [B]: what the model says after the last. tokens [B, S], parents as in TreeAttention (without: each token's parent is the one before "
+               "it); of two children with the same token the first is taken."),
     # Pad only ever runs folded into the Conv that reads it (transformation/fusion.py, the reference's PadConvFusion)
     ONNXSchema("Pad", 11,
                [ONNXParameter("data", "T"), ONNXParameter("pads", "tensor(int64)"), ONNXParameter("constant_value", "T", _O)],

@@ -77,6 +77,15 @@ def _infer_node(node, shapes, types, constants):
         if len(Q) != 4 or len(V) != 4 or Q[2] % 2:
             raise ShapeInferenceError(f"{op} '{node.name}': queries of {Q} and values of {V} (expected [B, S, 2 H, d] and [B, S, H, 2 d])")
         return [((Q[0], Q[1], Q[2] // 2, V[3]), tys[0])]
+    if op == "PagedCacheAppend":
+        Q = (ins[9], tys[9]) if len(ins) > 9 and ins[9] is not None else (ins[0], tys[0])
+        return [(ins[2], tys[2]), (ins[3], tys[3]), Q]
+    if op == "TreeAttention":
+        return [(ins[0], tys[0])]
+    if op == "DraftAcceptance":
+        if len(ins[0]) != 3:
+            raise ShapeInferenceError(f"{op} '{node.name}': logits of {ins[0]} (expected [B, S, vocabulary])")
+        return [(tuple(ins[0][:2]), TensorProto.INT32), (tuple(ins[0][:1]), TensorProto.INT32), (tuple(ins[0][:1]), TensorProto.INT32)]
     if op == "MatMul" or op == "MatMulInteger":
         A, B = ins[0], ins[1]
         if len(A) < 2 or len(B) < 2:

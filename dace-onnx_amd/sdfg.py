@@ -483,7 +483,8 @@ class SDFGState:
     def topological_nodes(self):
         """Nodes in dependency order. Two access nodes of the same array are
         ordered write-before-read, which is how DaCe sequences them across the
-        access-node chain of a state."""
+        access-node chain of a state, but for a node that updates an array: what it
+        reads is the array before."""
         indeg = {id(n): 0 for n in self._nodes}
         succ = collections.defaultdict(list)
         for e in self._edges:
@@ -496,6 +497,8 @@ class SDFGState:
         for data, ws in writers.items():
             for w in ws:
                 for r in readers.get(data, []):
+                    if any(e.dst is w for o in succ[id(r)] for e in self.out_edges(o)):
+                        continue
                     succ[id(w)].append(r)
                     indeg[id(r)] += 1
         ready = [n for n in self._nodes if indeg[id(n)] == 0]

@@ -509,6 +509,50 @@ int mi355x_differential_attention(const void* Q, const void* K, const void* V, c
                                   int64_t heads, int64_t groups, int64_t size, int64_t vector, float lambda_init,
                                   float scale, int causal, int64_t splits, int type, void* stream);
 
+/* ---- a cache in pages, and drafted tokens over it --------------------------------------------------------
+ * The reference has none of these nodes either. Types, rounding and layout as above; pages are [pages, kv_heads, page_size, size].
+ * Number n of batch entry b is row n % page_size of page table[b, n / page_size]; table [batch, columns], lengths [batch]. */
+
+/* K and V [batch, tokens, kv_heads, size] into the pages: token i of entry b becomes number lengths[b] + i, or, with order
+ * [batch, taken], token order[b, j] becomes number lengths[b] + j (taken is `tokens` without). Nothing is written where order
+ * holds none of 0 to tokens - 1, where the number has no column, or its table value is none of 0 to pages - 1; a length below 0
+ * counts as 0. K is turned on the way, and Q [batch, tokens, heads, size] to Q_out, as mi355x_rotary_positions does, by positions
+ * [axes, batch, tokens] or, if that is NULL, by the number itself (axes is 1 then; a taken token's is the number that it becomes).
+ * rotated may be 0. Q (with heads of 0) and order may be NULL, not both given. The pages are apart from each other and from
+ * everything else, as are the rows that a call writes; Q_out may be Q. */
+int mi355x_paged_cache_append(const void* K, const void* V, const void* Q, void* k_pages, void* v_pages, void* Q_out,
+                              const int32_t* table, const int32_t* lengths, const float* frequencies,
+                              const void* positions, const int32_t* order, int64_t batch, int64_t tokens, int64_t heads,
+                              int64_t kv_heads, int64_t size, int64_t pages, int64_t page_size, int64_t columns,
+                              int64_t taken, int64_t rotated, int64_t axes, const int64_t* sections, int interleaved,
+                              int position_bytes, int type, void* stream);
+
+/* O = softmax(scale Q K^T) V for tokens Q [batch, tokens, heads, size] that are numbers lengths[b] to lengths[b] + tokens - 1 of
+ * their entries: token i sees the numbers before lengths[b], itself and its ancestors. parents [batch, tokens] holds each token's
+ * parent, a lower place; anything else is none. Without (NULL) a token's parent is the one before it. size is 64, 128 or 256,
+ * heads / kv_heads heads share keys and values, tokens is 1024 at most with parents. Table values that are no page count as the
+ * nearest one, numbers without a column do not exist, a length below 0 counts as 0; a row without keys is 0. The pages stand at
+ * 16-byte boundaries. `scratch` has room for scratch_floats floats, 16-byte aligned (mi355x_tree_attention_scratch says how many,
+ * 0 with NULL: none needed), and belongs to the call until it is done.
+ * With arrays of 16 bits the probabilities are rounded to `type` for their product with V, and their sum is that of the rounded
+ * ones; scores, maxima, sums and results stay in float32. In float32 an infinite query, key or value that a row sees makes it not a
+ * number, and values below 2^-110 lose digits. What a row does not see does not reach it, whatever it holds. */
+int64_t mi355x_tree_attention_scratch(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size,
+                                      int64_t page_size, int64_t columns, int type);
+int mi355x_tree_attention(const void* Q, const void* k_pages, const void* v_pages, const int32_t* table,
+                          const int32_t* lengths, const int32_t* parents, void* O, float* scratch, int64_t scratch_floats,
+                          int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t pages,
+                          int64_t page_size, int64_t columns, float scale, int type, void* stream);
+
+/* The walk along a tree of drafted tokens [batch, tokens]: from token 0 to the first child whose token is the place of the
+ * largest of the parent's logits [batch, tokens, vocabulary] (the first of equal ones; a NaN is none, a row of NaN says 0), and so on.
+ * path [batch, tokens] the places of the tokens on it, then -1; count [batch]; next [batch] what the logits of the last one say.
+ * parents as above. tokens is 1024 at most. scratch: scratch_words words of 64 bits (mi355x_draft_acceptance_scratch). */
+int64_t mi355x_draft_acceptance_scratch(int64_t batch, int64_t tokens, int64_t vocabulary, int type);
+int mi355x_draft_acceptance(const void* logits, const int32_t* tokens, const int32_t* parents, int32_t* path,
+                            int32_t* count, int32_t* next, void* scratch, int64_t scratch_words, int64_t batch,
+                            int64_t token_count, int64_t vocabulary, int type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
