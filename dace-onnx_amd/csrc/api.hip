@@ -78,6 +78,8 @@ static void parse_tuning(Tuning& t) {
     t.qlin_form = env_int("MI355X_QLIN_FORM", -1);
     t.diff_splits = env_int("MI355X_DIFF_SPLITS", 0);
     t.diff_form = env_int("MI355X_DIFF_FORM", -1);
+    t.tree_splits = env_int("MI355X_TREE_SPLITS", 0);
+    t.tree_form = env_int("MI355X_TREE_FORM", -1);
 }
 
 Tuning tuning() {
