@@ -78,7 +78,8 @@ static void parse_tuning(Tuning& t) {
     t.qlin_form = env_int("MI355X_QLIN_FORM", -1);
     t.diff_splits = env_int("MI355X_DIFF_SPLITS", 0);
     t.diff_form = env_int("MI355X_DIFF_FORM", -1);
-    t.tree_splits = env_int("MI355X_TREE_SPLITS", 0);
+    t.tree_deal = env_int("MI355X_TREE_DEAL", -1);
+    t.accept_parts = env_int("MI355X_ACCEPT_PARTS", 0);
     t.tree_form = env_int("MI355X_TREE_FORM", -1);
 }
 

@@ -33,7 +33,7 @@ struct Tuning {
     bool mmi_generic = false;
     int mmi_wgs_per_cu = 0, mmi_tile = 0;
     int attn_waves = 0, attn_split = -1, attn_few = -1;
-    int qlin_form = -1, diff_splits = 0, diff_form = -1, tree_splits = 0, tree_form = -1;
+    int qlin_form = -1, diff_splits = 0, diff_form = -1, tree_form = -1, tree_deal = -1, accept_parts = 0;
 };
 Tuning tuning();   // a copy taken under the lock: a reload never changes what a launch in progress reads
 int device_cus();

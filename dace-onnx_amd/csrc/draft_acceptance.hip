@@ -1,6 +1,8 @@
 // DraftAcceptance: the largest of every row of logits, and the walk along each entry's tree of drafted tokens that follows them. The reference has no such node.
 #include "mixed.h"
 
+#include <algorithm>
+
 namespace mi355x {
 
 constexpr int ACCEPT_MOST = 1024;   // tokens of a tree
@@ -27,48 +29,96 @@ __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
     return v;
 }
 
+// A part of a row to a workgroup. A thread keeps the largest of its vectors and which it was, the first of equal ones, and looks for the place in it at the end.
 template <class T>
 __global__ __launch_bounds__(256) void accept_rows_kernel(AcceptArgs p) {
+    constexpr int E = 16 / sizeof(T), AHEAD = 4;
+    typedef typename Values<T, E>::vec Vector;
     __shared__ uint64_t found[4];
     const int64_t row = blockIdx.x / p.parts, first = blockIdx.x % p.parts * p.part;
     const int64_t last = first + p.part < p.vocabulary ? first + p.part : p.vocabulary;
     const T* x = static_cast<const T*>(p.logits) + row * p.vocabulary;
+    auto key = [](uint32_t order, int64_t place) { return (uint64_t)order << 32 | (uint32_t)~(uint32_t)place; };
+    // vectors begin at 16-byte boundaries; what stands before and behind them goes by single values
+    const int64_t gap = (int64_t)((16 - (reinterpret_cast<uintptr_t>(x + first) & 15)) & 15) / (int64_t)sizeof(T);
+    const int64_t begin = first + gap < last ? first + gap : last, vectors = (last - begin) / E, end = begin + vectors * E;
     uint64_t best = 0;
-    for (int64_t i = first + threadIdx.x; i < last; i += 256) best = larger(best, (uint64_t)order_of((float)x[i]) << 32 | (uint32_t)~(uint32_t)i);
+    const int64_t single = (int64_t)threadIdx.x < begin - first ? first + threadIdx.x : (int64_t)threadIdx.x - E < last - end && threadIdx.x >= E ? end + threadIdx.x - E : -1;
+    if (single >= 0) best = key(order_of((float)x[single]), single);
+    const Vector* v = reinterpret_cast<const Vector*>(x + begin);
+    uint32_t largest = 0;
+    int64_t which = threadIdx.x;
+    for (int64_t i0 = threadIdx.x; i0 < vectors; i0 += 256 * AHEAD) {
+        Vector held[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) held[u] = v[i0 + 256 * u < vectors ? i0 + 256 * u : i0];   // (again the first, where there is none: not larger than itself)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            float m = (float)held[u][0];
+#pragma unroll
+            for (int e = 1; e < E; ++e) m = fmaxf(m, (float)held[u][e]);
+            const uint32_t order = order_of(m);
+            if (order > largest) largest = order, which = i0 + 256 * u;
+        }
+    }
+    if ((int64_t)threadIdx.x < vectors) {
+        const Vector again = v[which];
+        int place = 0;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+            if (order_of((float)again[e]) == largest) place = e;
+        best = larger(best, key(largest, begin + which * E + place));
+    }
     best = wave_largest(best);
     if (threadIdx.x % WAVE == 0) found[threadIdx.x / WAVE] = best;
     __syncthreads();
     if (threadIdx.x == 0) p.best[blockIdx.x] = larger(larger(found[0], found[1]), larger(found[2], found[3]));
 }
 
-// A workgroup to an entry. A token's children stand behind it, so one pass over the tokens finds the whole path.
+// A workgroup to an entry. A token's children stand behind it: each step looks at the tokens from its own 64 on.
 __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptArgs p) {
     __shared__ int32_t said[ACCEPT_MOST], tokens[ACCEPT_MOST], parents[ACCEPT_MOST];
     const int S = p.batch_tokens;
     const int64_t row0 = (int64_t)blockIdx.x * S;
     for (int i = threadIdx.x; i < S; i += 256) {
+        const int32_t token = p.tokens[row0 + i], parent = p.parents ? p.parents[row0 + i] : i - 1;
         uint64_t best = 0;
+#pragma unroll 8
         for (int c = 0; c < p.parts; ++c) best = larger(best, p.best[(row0 + i) * p.parts + c]);
         said[i] = (int32_t)~(uint32_t)best;
-        tokens[i] = p.tokens[row0 + i];
-        parents[i] = p.parents ? p.parents[row0 + i] : i - 1;
+        tokens[i] = token;
+        parents[i] = parent;
     }
     __syncthreads();
-    if (threadIdx.x) return;
-    int node = 0, length = 1;
-    p.path[row0] = 0;
-    for (int i = 1; i < S; ++i)
-        if (parents[i] == node && tokens[i] == said[node]) p.path[row0 + length++] = node = i;
-    for (int i = length; i < S; ++i) p.path[row0 + i] = -1;
-    p.count[blockIdx.x] = length;
-    p.next[blockIdx.x] = said[node];
+    if (threadIdx.x >= WAVE) return;
+    int node = 0, length = 0;
+    while (true) {
+        if (threadIdx.x == 0) p.path[row0 + length] = node;
+        ++length;
+        const int32_t wanted = said[node];
+        int child = S;
+        for (int i0 = node / WAVE * WAVE; i0 < S && child == S; i0 += WAVE) {
+            const int i = i0 + threadIdx.x;
+            const uint64_t fits = __ballot(i < S && i > node && parents[i] == node && tokens[i] == wanted);
+            if (fits) child = i0 + __builtin_ctzll(fits);
+        }
+        if (child == S) break;
+        node = child;
+    }
+    for (int i = length + threadIdx.x; i < S; i += WAVE) p.path[row0 + i] = -1;
+    if (threadIdx.x == 0) p.count[blockIdx.x] = length, p.next[blockIdx.x] = said[node];
 }
 
 static bool accept_fits(int64_t batch, int64_t tokens, int64_t vocabulary) {
     return batch >= 0 && tokens >= 1 && tokens <= ACCEPT_MOST && vocabulary >= 1 && vocabulary < (int64_t)1 << 31 && batch < (int64_t)1 << 31 && (double)batch * tokens * vocabulary < 0x1p45;
 }
 
-static int64_t accept_parts(int64_t rows, int64_t vocabulary) { return rows ? 1 : 1; }
+// Workgroups to a row: enough for all CUs several times, none with less than two vectors to a thread
+static int64_t accept_parts(int64_t rows, int64_t vocabulary) {
+    const int forced = tuning().accept_parts;
+    if (forced > 0) return std::min<int64_t>(forced, vocabulary);
+    return std::max<int64_t>(1, std::min({ceil_div((int64_t)2048, std::max<int64_t>(rows, 1)), vocabulary / 4096, (int64_t)64}));
+}
 
 }  // namespace mi355x
 

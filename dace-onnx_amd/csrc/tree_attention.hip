@@ -9,21 +9,205 @@ constexpr int TREE_MOST = 1024;   // tokens of a tree
 
 struct TreeArgs {
     const void* q; const void* k_pages; const void* v_pages; const int32_t* table; const int32_t* lengths; const int32_t* parents; void* o;
-    float* partial_o; float* partial_ml;   // of splits; [split][slice][row][D], [split][slice][row][2]
+    float* partial_o; float* partial_ml;   // of parts: [workgroup][row of the block][D], [workgroup][row of the block][2]
     int64_t batch, tokens, columns, row_blocks;
     int pages, page_size, capacity;        // capacity = page_size * columns
-    int heads, kv_heads, share, splits;    // share = heads / kv_heads
+    int heads, kv_heads, share;            // share = heads / kv_heads
+    int block_rows;                        // of a workgroup's part
+    int dealt;                             // workgroups that the parts of all blocks are dealt to; 0: one workgroup to a block
+    int order;                             // of those: see tree_block
     uint32_t page_magic; int page_shift;   // n / page_size for n below 2^31
     float scale_log2;
 };
 
 __device__ __forceinline__ int tree_column(const TreeArgs& p, int n) { return (int)(__umulhi(2u * (uint32_t)n, p.page_magic) >> p.page_shift); }
 
+struct TreeEntry { int length, total; };   // keys before the call, and with it
+__device__ __forceinline__ TreeEntry tree_entry(const TreeArgs& p, int64_t b) {
+    const int given = p.lengths[b], length = given < 0 ? 0 : given > p.capacity ? p.capacity : given;
+    return {length, (int)std::min<int64_t>(length + p.tokens, p.capacity)};
+}
+
+// f over the lanes of a wave, four of a row at a time, then the rows; every lane gets it
+template <class F>
+__device__ __forceinline__ uint32_t wave_uint(uint32_t v, F&& f) {
+    auto across = [&](auto control) { v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(control)::value, 0xf, 0xf, false)); };
+    across(Int<DPP_QUAD_XOR1>{}), across(Int<DPP_QUAD_XOR2>{}), across(Int<DPP_ROW_HALF_MIRROR>{}), across(Int<DPP_ROW_MIRROR>{});
+    auto row = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
+    return f(f(row(0), row(16)), f(row(32), row(48)));
+}
+
+// The keys of every block of an entry, in stages of KT, cut into as many parts as it takes for none to have more than `most` stages, which is as few as leave enough workgroups for all
+// parts; an entry's `items` blocks count alike. Workgroups go by entry, block and part. A lane of each wave looks at entries lane, lane + 64, ...
+constexpr int DEAL_ENTRIES = 256;
+template <int KT>
+struct TreeDeal {
+    static constexpr int EACH = DEAL_ENTRIES / WAVE;
+    int64_t items;   // blocks of an entry
+    uint32_t most, stages[EACH];
+    __device__ __forceinline__ uint32_t parts(uint32_t stages) const { return (stages + most - 1) / most; }
+    __device__ __forceinline__ int64_t sum(const TreeArgs& p, int64_t before) const {   // parts of the entries before that one
+        int64_t all = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (i * WAVE >= before) break;
+            all += wave_uint(i * WAVE + (int)(threadIdx.x % WAVE) < before ? parts(stages[i]) : 0u, [](uint32_t x, uint32_t y) { return x + y; });
+        }
+        return all;
+    }
+    __device__ __forceinline__ TreeDeal(const TreeArgs& p) : items(p.kv_heads * p.row_blocks) {
+        int64_t all = 0;
+        uint32_t longest = 1;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int64_t b = i * WAVE + threadIdx.x % WAVE;
+            stages[i] = b < p.batch ? std::max(1, (tree_entry(p, b).total + KT - 1) / KT) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (i * WAVE >= p.batch) break;
+            all += wave_uint(stages[i], [](uint32_t x, uint32_t y) { return x + y; });
+            longest = std::max(longest, wave_uint(stages[i], [](uint32_t x, uint32_t y) { return x > y ? x : y; }));
+        }
+        // (enough are all stages of a block: there are no more blocks than workgroups)
+        uint32_t low = (uint32_t)((all * items + p.dealt - 1) / p.dealt);
+        most = longest;
+        while (low < most) {
+            const uint32_t enough = most;
+            most = low + (enough - low) / 2;
+            if (sum(p, p.batch) * items <= p.dealt) continue;
+            low = most + 1;
+            most = enough;
+        }
+    }
+    // the entry that workgroup w is of, which of the entry's it is, and how many parts the entry's blocks have; false: of none
+    __device__ __forceinline__ bool find(const TreeArgs& p, int64_t w, int64_t& b, int64_t& of_entry, int& own) const {
+        int64_t passed = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (i * WAVE >= p.batch) break;
+            const int mine = (int)parts(stages[i]);
+            int with = mine;
+#pragma unroll
+            for (int d = 1; d < WAVE; d *= 2) {
+                const int other = __shfl_up(with, d);
+                with += (int)(threadIdx.x % WAVE) >= d ? other : 0;
+            }
+            const uint64_t beyond = __ballot((passed + with) * items > w);
+            if (beyond) {
+                const int lane = __builtin_ctzll(beyond);
+                own = __builtin_amdgcn_readlane(mine, lane);
+                b = i * WAVE + lane;
+                of_entry = w - (passed + __builtin_amdgcn_readlane(with, lane) - own) * items;
+                return true;
+            }
+            passed += __builtin_amdgcn_readlane(with, WAVE - 1);
+        }
+        return false;
+    }
+    __device__ __forceinline__ int parts_of(int64_t b) const {
+        int own = 1;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (b / WAVE == i) own = (int)__shfl((int)parts(stages[i]), (int)(b % WAVE));
+        return own;
+    }
+};
+
+// Which block of a call that is not dealt out workgroup blockIdx.x has. The hardware deals workgroups to the XCDs in turn, and those of an XCD to its CUs in turn: slices (an
+// entry's group) stay on one XCD or few, whose L2 their keys then pass once, and every XCD has blocks of all lengths.
+// order 0: the long ones first; 1: of up to two workgroups to a CU, a long one and a short one.
+__device__ __forceinline__ void tree_block(const TreeArgs& p, int64_t& slice, int64_t& block) {
+    const int64_t slices = p.batch * p.kv_heads, grid = slices * p.row_blocks;
+    const uint32_t w = blockIdx.x;
+    int64_t turn;
+    if (slices % NUM_XCD == 0) {
+        const uint32_t each = (uint32_t)(slices / NUM_XCD), local = w / NUM_XCD;
+        slice = w % NUM_XCD * (int64_t)each + local % each;
+        turn = local / each;
+    } else {
+        slice = w % slices;
+        turn = w / slices;
+    }
+    if (p.order && turn * slices >= grid / 2) turn = p.row_blocks - 1 - (turn - (grid / 2 + slices - 1) / slices);
+    block = p.row_blocks - 1 - turn;
+}
+
 // the lowest n of 32 bits
 __device__ __forceinline__ uint32_t lowest_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
 
-// Waves: RW blocks of 32 RB rows, KW shares of a stage's keys, 32 SUB each; NS stages.
-template <class T, int D, int RB, int RW, int KW, int SUB, int NS, int PER_SIMD>
+// N KB of keys or values that lie one behind the other, to LDS likewise: the offset of an instruction counts on both sides
+template <int N>
+__device__ __forceinline__ void run_to_lds(const void* base, const uint32_t* lane_offset, uint32_t lds) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint64_t uniform = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    const int to = __builtin_amdgcn_readfirstlane((int)lds);
+    static_assert(N == 1 || N == 2 || N == 4, "offsets of 12 bits");
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_offset[0]), "s"(uniform) : "memory", "m0");
+    else if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(to), "v"(lane_offset[0]),
+                     "v"(lane_offset[1]), "s"(uniform) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+                     "global_load_lds_dwordx4 %4, %5 offset:3072" ::"s"(to), "v"(lane_offset[0]), "v"(lane_offset[1]), "v"(lane_offset[2]), "v"(lane_offset[3]), "s"(uniform) : "memory", "m0");
+}
+
+// S^T of 32 keys and 32 rows, the keys' operands on their way from LDS all at once: one after the other each product waits for its own.
+template <class T, int D, int RB>
+__device__ __forceinline__ void tree_scores(uint32_t lds_k, const Operand<T> (&q)[RB][D / 16], f32x16 (&acc)[RB]) {
+    using Wave = AttentionWave<T, D, D>;
+    typename Values<T, 8>::vec k[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) k[s] = Wave::template read<typename Values<T, 8>::vec>(lds_k ^ (32 * s), 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) acc[b] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) Operand<T>::product({{k[s]}}, q[b][s], acc[b]);
+}
+
+// The values' operands of 32 keys: in registers by the time the probabilities are
+template <class T, int D>
+__device__ __forceinline__ void tree_read_values(uint32_t lds_v, typename Values<T, 8>::vec (&v)[2 * D / 32]) {
+    constexpr int ROW = AttentionTile<T, D>::ROW;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            s16x4 half[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                half[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(reinterpret_cast<__attribute__((address_space(3))) char*>(
+                    lds_v ^ (16 * (4 * c ^ 2 * i))) + (16 * t + 8 * i) * ROW));
+            v[t * (D / 32) + c] = __builtin_bit_cast(typename Values<T, 8>::vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+}
+
+template <class T, int D, int RB>
+__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * D / 32], const f32x16 (&prob)[RB], f32x16 (&out)[RB][D / 32], float (&sum)[RB]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        Operand<T> pr[RB];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            T x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (T)prob[b][8 * t + e];
+            pr[b].set(x);
+            pr[b].add_to(sum[b], x);
+        }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) Operand<T>::product({{v[t * (D / 32) + c]}}, pr[b], out[b][c]);
+    }
+}
+
+// Waves: RW blocks of 32 RB rows, KW shares of a stage's keys, 32 SUB each; NS stages. WHOLE: no transfer's keys lie in two pages.
+template <class T, int D, int RB, int RW, int KW, int SUB, int NS, int PER_SIMD, bool WHOLE>
 __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(TreeArgs p) {
     using Tile = AttentionTile<T, D>;
     using Wave = AttentionWave<T, D, D>;
@@ -34,34 +218,127 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
     constexpr int PER_T = KT * Tile::PIECES / NT, KPT = WAVE / Tile::PIECES;   // transfers of a wave's keys in a stage, keys to a transfer
     static_assert(KT * Tile::PIECES % NT == 0 && Tile::PIECES <= WAVE && NS >= 2 && (NS - 2) * 2 * PER_T < 64, "whole pieces to a thread, whole keys to a transfer");
     constexpr int EXCHANGE = 32 * D;   // floats of a row block's output
+    constexpr bool AHEAD = sizeof(T) == 2 && D <= 128;   // operands are read from LDS all at once, before they are needed
     __shared__ __attribute__((aligned(1024))) unsigned char lds[std::max(NS * STAGE, KW == 1 ? 0 : 4 * EXCHANGE * (KW / 2) * RW * RB)];
     __shared__ int16_t parents[TREE_MOST];
     __shared__ uint32_t odd_keys[2][KT / 32];   // of the stage and the one before
 
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int n = lane % 32, h = lane / 32, row_wave = wave % RW, key_wave = wave / RW;
-    const int64_t logical = xcd_remap(blockIdx.x, (int64_t)gridDim.x);
-    const int64_t turn = logical % p.row_blocks, rest = logical / p.row_blocks, slice = rest / p.splits;
-    const int split = (int)(rest % p.splits);
-    const int64_t b = slice / p.kv_heads;
-    const int group = (int)(slice % p.kv_heads);
-    const int64_t rows = p.tokens * p.share, block = p.row_blocks - 1 - turn;   // long ones first
-    const int given = p.lengths[b];
-    const int length = given < 0 ? 0 : given > p.capacity ? p.capacity : given;
-    const int total = (int)std::min<int64_t>(length + p.tokens, p.capacity);
+    const int64_t rows = p.tokens * p.share;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+    const uint32_t key_at = Wave::key_address(0, n, h), value_at = Wave::value_address(lane, n, h);
+    if (tid < KT / 32) odd_keys[0][tid] = odd_keys[1][tid] = 0;
+
+    // Piece `lane` of transfer j of a wave, whose keys are one behind the other: where it is, counted from the transfer's first key
+    uint32_t offset[PER_T];
+#pragma unroll
+    for (int j = 0; j < PER_T; ++j) {
+        const int key = (wave * PER_T + j) * KPT + lane / Tile::PIECES;
+        offset[j] = (uint32_t)(lane / Tile::PIECES * Tile::ROW + (lane % Tile::PIECES ^ Tile::place(key)) * 16);
+    }
+
+    int64_t b, block, of_entry;
+    int group, part = 0, parts = 1;
+    if (p.dealt) {
+        const TreeDeal<KT> deal(p);
+        if (!deal.find(p, blockIdx.x, b, of_entry, parts)) return;
+        part = (int)(of_entry % parts);
+        group = (int)(of_entry / parts / p.row_blocks);
+        block = of_entry / parts % p.row_blocks;
+    } else {
+        int64_t slice;
+        tree_block(p, slice, block);
+        b = slice / p.kv_heads;
+        group = (int)(slice % p.kv_heads);
+    }
+    const TreeEntry entry = tree_entry(p, b);
+    const int length = __builtin_amdgcn_readfirstlane(entry.length), total = __builtin_amdgcn_readfirstlane(entry.total);
     // keys up to and with token `row / share`
     auto up_to = [&](int64_t row) { return (int)std::min<int64_t>(total, length + row / p.share + 1); };
-
-    if (tid < KT / 32) odd_keys[0][tid] = odd_keys[1][tid] = 0;
     if (p.parents) {
         for (int i = tid; i < (int)p.tokens; i += NT) {
             const int parent = p.parents[b * p.tokens + i];
             parents[i] = (int16_t)(parent >= 0 && parent < i ? parent : -1);
         }
     }
-
-    // ---- queries: row r of a slice is head r % share of token r / share ------------------------------------
+    // keys that any row of the workgroup sees, and that all of them see; the same of the wave
     const int64_t row0 = block * ROWS + row_wave * RB * 32;   // of the wave
+    const int end = up_to(std::min(rows, (block + 1) * ROWS) - 1), all = p.parents ? length : up_to(block * ROWS);
+    const int wave_end = row0 < rows ? __builtin_amdgcn_readfirstlane(up_to(std::min(rows, row0 + 32 * RB) - 1)) : 0;
+    const int wave_all = p.parents ? length : __builtin_amdgcn_readfirstlane(up_to(std::min(rows - 1, row0)));
+    const int stages = (end + KT - 1) / KT, first = (int)((int64_t)part * stages / parts), last = (int)((int64_t)(part + 1) * stages / parts), count = last - first;
+
+    // ---- keys and values -------------------------------------------------------------------------------
+    typedef const __attribute__((address_space(4))) int32_t Uniform;   // (read by scalar loads, which the transfers' counter does not count)
+    const int32_t* const columns = p.table + b * p.columns;
+    Uniform* const table = (Uniform*)(uintptr_t)columns;
+    const int64_t page_bytes = (int64_t)p.kv_heads * p.page_size * Tile::ROW;
+    const char* K = static_cast<const char*>(p.k_pages) + (int64_t)group * p.page_size * Tile::ROW;
+    const char* V = static_cast<const char*>(p.v_pages) + (int64_t)group * p.page_size * Tile::ROW;
+    auto from_page = [&](int page, int row) { return std::min(std::max(page, 0), p.pages - 1) * page_bytes + (int64_t)row * Tile::ROW; };
+    int next_page[PER_T];
+    // f(transfers of a wave that are sure to lie in one page, one behind the other)
+    auto by_runs = [&](auto&& f) __attribute__((always_inline)) {
+        if constexpr (PER_T >= 8) { if (p.page_size % (8 * KPT) == 0) { f(Int<8>{}); return; } }
+        if constexpr (PER_T >= 4) { if (p.page_size % (4 * KPT) == 0) { f(Int<4>{}); return; } }
+        if constexpr (PER_T >= 2) { if (p.page_size % (2 * KPT) == 0) { f(Int<2>{}); return; } }
+        f(Int<1>{});
+    };
+    // (of keys that do not exist: some that can be read)
+    auto number = [&](int stage, int j, int keys) { return std::min(stage * KT + (wave * PER_T + j) * KPT, p.capacity - keys); };
+    auto find = [&](int stage) __attribute__((always_inline)) {
+        if constexpr (WHOLE)
+            by_runs([&](auto run) __attribute__((always_inline)) {
+                constexpr int R = decltype(run)::value;
+#pragma unroll
+                for (int j = 0; j < PER_T; j += R) next_page[j] = table[tree_column(p, number(stage, j, R * KPT))];
+            });
+    };
+    auto load = [&](int stage, int buffer) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
+            by_runs([&](auto run) __attribute__((always_inline)) {
+                constexpr int R = decltype(run)::value, N = R < 4 ? R : 4;
+#pragma unroll
+                for (int j = 0; j < PER_T; j += R) {
+                    const int first_key = number(stage, j, R * KPT);
+                    const int64_t from = from_page(next_page[j], first_key - tree_column(p, first_key) * p.page_size);
+                    const uint32_t to = lds0 + (uint32_t)(buffer * STAGE + (wave * PER_T + j) * 1024);
+#pragma unroll
+                    for (int i = 0; i < R; i += N) {
+                        run_to_lds<N>(K + from + i * 1024, offset + j + i, to + i * 1024);
+                        run_to_lds<N>(V + from + i * 1024, offset + j + i, to + i * 1024 + HALF);
+                    }
+                }
+            });
+        } else {
+            int page[PER_T], row[PER_T];
+#pragma unroll
+            for (int j = 0; j < PER_T; ++j) {
+                const int key = std::min(stage * KT + (wave * PER_T + j) * KPT + lane / Tile::PIECES, p.capacity - 1), column = tree_column(p, key);
+                page[j] = columns[column];
+                row[j] = key - column * p.page_size;
+            }
+            char* to = reinterpret_cast<char*>(lds) + buffer * STAGE + wave * PER_T * 1024 + lane * 16;
+#pragma unroll
+            for (int j = 0; j < PER_T; ++j) {
+                const int64_t from = from_page(page[j], row[j]) + (offset[j] - lane / Tile::PIECES * Tile::ROW);
+                const Piece k = *reinterpret_cast<const Piece*>(K + from), v = *reinterpret_cast<const Piece*>(V + from);
+                *reinterpret_cast<Piece*>(to + j * 1024) = k;
+                *reinterpret_cast<Piece*>(to + j * 1024 + HALF) = v;
+            }
+        }
+    };
+
+    if (count > 0) find(last - 1);
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+        if (s < count) {
+            load(last - 1 - s, s);
+            if (s + 1 < count) find(last - 2 - s);
+        }
+
+    // ---- queries: row r of a slice is head r % share of token r / share --------------------------------
     int token[RB], ancestor[RB];
     Operand<T> q[RB][Wave::QP];
 #pragma unroll
@@ -82,67 +359,6 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             q[i][s].set(v);
         }
     }
-    // keys that any row of the workgroup sees, and that all of them see; the same of the wave
-    const int end = up_to(std::min(rows, (block + 1) * ROWS) - 1), all = p.parents ? length : up_to(block * ROWS);
-    const int wave_end = row0 < rows ? __builtin_amdgcn_readfirstlane(up_to(std::min(rows, row0 + 32 * RB) - 1)) : 0;
-    const int wave_all = p.parents ? length : __builtin_amdgcn_readfirstlane(up_to(std::min(rows - 1, row0)));
-    const int stages = (end + KT - 1) / KT, per_split = (stages + p.splits - 1) / p.splits;
-    const int first = split * per_split, count = std::max(0, std::min(stages, first + per_split) - first), last = first + count;
-
-    // ---- keys and values -----------------------------------------------------------------------------------
-    const T* K = static_cast<const T*>(p.k_pages);
-    const T* V = static_cast<const T*>(p.v_pages);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
-    typedef const __attribute__((address_space(4))) int32_t Uniform;   // (read by scalar loads, which the transfers' counter does not count)
-    Uniform* const table = (Uniform*)(uintptr_t)(p.table + b * p.columns);
-    auto page_at = [&](int column) { return std::min(std::max((int)table[column], 0), p.pages - 1); };
-    auto row_at = [&](int page, int row) { return (((int64_t)page * p.kv_heads + group) * p.page_size + row) * D; };
-    const bool whole = p.page_size % KPT == 0;   // no transfer's keys lie in two pages
-    // piece tid + j NT of a stage's keys, or values: what of a transfer this lane fetches, counted from the transfer's first key
-    uint32_t offset[PER_T];
-    int at_key[PER_T], next_page[PER_T];
-#pragma unroll
-    for (int j = 0; j < PER_T; ++j) {
-        const int key = (tid + j * NT) / Tile::PIECES, piece = (tid + j * NT) % Tile::PIECES ^ Tile::place(key);
-        offset[j] = (uint32_t)(((whole ? lane / Tile::PIECES : 0) * D + piece * E) * sizeof(T));
-        at_key[j] = whole ? __builtin_amdgcn_readfirstlane(key) : key;
-    }
-    auto number = [&](int stage, int j) { return std::min(stage * KT + at_key[j], p.capacity - (whole ? KPT : 1)); };   // (keys that do not exist: some that can be read)
-    auto find = [&](int stage) __attribute__((always_inline)) {
-        if (!whole) return;
-#pragma unroll
-        for (int j = 0; j < PER_T; ++j) next_page[j] = page_at(__builtin_amdgcn_readfirstlane(tree_column(p, number(stage, j))));
-    };
-    auto load = [&](int stage, int buffer) __attribute__((always_inline)) {
-        if (whole) {
-#pragma unroll
-            for (int j = 0; j < PER_T; ++j) {
-                const int at = number(stage, j), row = at - tree_column(p, at) * p.page_size;
-                const int64_t from = row_at(next_page[j], row);
-                const uint32_t to = lds0 + (uint32_t)(buffer * STAGE + (wave * WAVE + j * NT) * 16);
-                attention_to_lds(K + from, offset[j], to);
-                attention_to_lds(V + from, offset[j], to + HALF);
-            }
-        } else {
-            int page[PER_T], row[PER_T];
-#pragma unroll
-            for (int j = 0; j < PER_T; ++j) {
-                const int at = number(stage, j), column = tree_column(p, at);
-                page[j] = p.table[b * p.columns + column];
-                row[j] = at - column * p.page_size;
-            }
-            T* to = reinterpret_cast<T*>(lds + buffer * STAGE) + tid * E;
-#pragma unroll
-            for (int j = 0; j < PER_T; ++j) {
-                const int64_t from = row_at(std::min(std::max(page[j], 0), p.pages - 1), row[j]) + offset[j] / sizeof(T);
-                const Piece k = *reinterpret_cast<const Piece*>(K + from), v = *reinterpret_cast<const Piece*>(V + from);
-                *reinterpret_cast<Piece*>(to + j * NT * E) = k;
-                *reinterpret_cast<Piece*>(to + j * NT * E + HALF / (int)sizeof(T)) = v;
-            }
-        }
-    };
-
-    const uint32_t key_at = Wave::key_address(0, n, h), value_at = Wave::value_address(lane, n, h);
     f32x16 out[RB][VT];
     float base[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
 #pragma unroll
@@ -153,13 +369,6 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
         for (int c = 0; c < VT; ++c) out[i][c] = f32x16{};
     }
 
-    if (count > 0) find(last - 1);
-#pragma unroll
-    for (int s = 0; s < NS - 1; ++s)
-        if (s < count) {
-            load(last - 1 - s, s);
-            if (s + 1 < count) find(last - 2 - s);
-        }
     int buffer = 0;
     for (int turn = 0; turn < count; ++turn, buffer = buffer + 1 == NS ? 0 : buffer + 1) {
         const int stage = last - 1 - turn;   // from the end on: a row's ancestors are met in falling order
@@ -178,7 +387,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             if (tid < KT / 32) odd_keys[(turn + 1) % 2][tid] = 0;
 #pragma unroll 1
             for (int j = 0; j < PER_T; ++j) {
-                const int at = tid + j * NT, key = at / Tile::PIECES;
+                const int at = tid + j * NT, key = at / Tile::PIECES;   // (any share of the stage)
                 if (stage * KT + key < all) continue;
                 Piece v = *reinterpret_cast<const Piece*>(values + at * E);
                 bool finite = true;
@@ -203,8 +412,15 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             lds_k += key_at;
             asm volatile("" : "+v"(lds_k), "+v"(lds_v));   // (nothing made of them is kept from one pass to the next)
             f32x16 s[RB];
+            typename Values<T, 8>::vec held[AHEAD ? 2 * VT : 1];
             __builtin_amdgcn_s_setprio(1);
-            Wave::scores(lds_k, q, s);
+            if constexpr (AHEAD) {
+                tree_scores<T, D>(lds_k, q, s);
+                tree_read_values<T, D>(lds_v, held);
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                Wave::scores(lds_k, q, s);
+            }
             __builtin_amdgcn_s_setprio(0);
             uint32_t seen[RB];   // of the 32 keys
 #pragma unroll
@@ -259,12 +475,13 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
                 for (int r = 0; r < 16; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from));
             }
             __builtin_amdgcn_s_setprio(1);
-            Wave::values(lds_v, s, out, sum);
+            if constexpr (AHEAD) tree_values<T, D>(held, s, out, sum);
+            else Wave::values(lds_v, s, out, sum);
             __builtin_amdgcn_s_setprio(0);
             if (!odd) continue;
             for (uint32_t left = __builtin_amdgcn_readfirstlane(odd[local / 32]); left; left &= left - 1) {
                 const int key = __builtin_ctz(left), at = key0 + key, column = tree_column(p, at);
-                const T* value = V + row_at(page_at(__builtin_amdgcn_readfirstlane(column)), at - column * p.page_size);
+                const T* value = reinterpret_cast<const T*>(V + from_page(columns[column], at - column * p.page_size));
 #pragma unroll
                 for (int i = 0; i < RB; ++i) {
                     float weight = 0.0f;
@@ -334,15 +551,14 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             }
             __syncthreads();
         }
-        if (key_wave) return;
     }
 
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
         const int64_t row = row0 + 32 * i + n;
-        if (row >= rows) continue;
-        if (p.splits > 1) {
-            const int64_t at = (split * p.batch * p.kv_heads + slice) * rows + row;
+        if (key_wave || row >= rows) continue;
+        if (parts > 1) {
+            const int64_t at = (int64_t)blockIdx.x * p.block_rows + (row - block * ROWS);
             if (h == 0) {
                 p.partial_ml[2 * at] = base[i];
                 p.partial_ml[2 * at + 1] = sum[i];
@@ -369,66 +585,117 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
     }
 }
 
-// The splits of a row joined: a wave to a row, its lanes the D values.
-template <class T, int D>
+// The parts of a row joined: WAVES waves to a row share its parts, the lanes of each are the D values. A block of one part is done.
+template <class T, int D, int KT, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs p) {
-    constexpr int PER_LANE = D / WAVE;
-    const int64_t rows = p.tokens * p.share, all = p.batch * p.kv_heads * rows;
-    const int lane = threadIdx.x % WAVE;
-    const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;   // of a slice's row
-    if (at >= all) return;
+    constexpr int PER_LANE = D / WAVE, ROWS = 4 / WAVES, BATCH = 8;
+    __shared__ float sums[4][D + 2];
+    const int64_t rows = p.tokens * p.share;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), share = wave % WAVES;
+    const int64_t at = (int64_t)blockIdx.x * ROWS + wave / WAVES;   // of a slice's row
+    if (at >= p.batch * p.kv_heads * rows) return;   // (of waves that share a row: all)
+    const int64_t slice = at / rows, row = at % rows, b = slice / p.kv_heads, block = row / p.block_rows;
+    const int group = (int)(slice % p.kv_heads);
+    const TreeDeal<KT> deal(p);
+    const int parts = __builtin_amdgcn_readfirstlane(deal.parts_of(b));
+    if (parts == 1) return;
+    T* to = static_cast<T*>(p.o) + ((b * p.tokens + row / p.share) * p.heads + group * p.share + (int)(row % p.share)) * D + lane * PER_LANE;
     float top = -__builtin_inff(), sum = 0.0f, o[PER_LANE] = {};
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.partial_ml[2 * (s * all + at)]);
-    const float from = top == -__builtin_inff() ? 0.0f : top;
-    for (int s = 0; s < p.splits; ++s) {
-        const float factor = __builtin_amdgcn_exp2f(p.partial_ml[2 * (s * all + at)] - from);
-        float part[PER_LANE];
-        load_values(part, p.partial_o + (s * all + at) * D + lane * PER_LANE, PER_LANE);
-        sum = fmaf(p.partial_ml[2 * (s * all + at) + 1], factor, sum);
+    const int64_t first = deal.sum(p, b) * deal.items + (group * p.row_blocks + block) * parts;   // workgroup
+    for (int part = share; part < parts; part += BATCH * WAVES) {
+        float base[BATCH], weight[BATCH], values[BATCH][PER_LANE], now = top;
 #pragma unroll
-        for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(part[e], factor, o[e]);
+        for (int i = 0; i < BATCH; ++i) {
+            const bool real = part + i * WAVES < parts;
+            const int64_t from = (first + (real ? part + i * WAVES : part)) * p.block_rows + (row - block * p.block_rows);
+            base[i] = real ? p.partial_ml[2 * from] : -__builtin_inff();
+            weight[i] = real ? p.partial_ml[2 * from + 1] : 0.0f;
+            load_values(values[i], p.partial_o + from * D + lane * PER_LANE, PER_LANE);
+            if (!real)
+#pragma unroll
+                for (int e = 0; e < PER_LANE; ++e) values[i][e] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) now = fmaxf(now, base[i]);
+        const float from = now == -__builtin_inff() ? 0.0f : now, factor = __builtin_amdgcn_exp2f(top - from);
+        sum *= factor;
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) o[e] *= factor;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const float f = __builtin_amdgcn_exp2f(base[i] - from);
+            sum = fmaf(weight[i], f, sum);
+#pragma unroll
+            for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(values[i][e], f, o[e]);
+        }
+        top = now;
+    }
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) sums[wave][lane * PER_LANE + e] = o[e];
+        if (lane == 0) sums[wave][D] = top, sums[wave][D + 1] = sum;
+        __syncthreads();
+        if (share) return;
+        float all = top;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) all = fmaxf(all, sums[wave + w][D]);
+        const float from = all == -__builtin_inff() ? 0.0f : all, factor = __builtin_amdgcn_exp2f(top - from);
+        sum *= factor;
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) o[e] *= factor;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sums[wave + w][D] - from);
+            sum = fmaf(sums[wave + w][D + 1], f, sum);
+#pragma unroll
+            for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(sums[wave + w][lane * PER_LANE + e], f, o[e]);
+        }
     }
 #pragma unroll
     for (int e = 0; e < PER_LANE; ++e) o[e] *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t slice = at / rows, row = at % rows, b = slice / p.kv_heads;
-    const int head = (int)(slice % p.kv_heads) * p.share + (int)(row % p.share);
-    store_values(static_cast<T*>(p.o) + ((b * p.tokens + row / p.share) * p.heads + head) * D + lane * PER_LANE, o, PER_LANE);
+    store_values(to, o, PER_LANE);
 }
 
 enum { TREE_FEW, TREE_MID, TREE_TALL };
 
-struct TreeCut { int form; int64_t row_blocks, workgroups, stages; };
-static TreeCut tree_cut(int64_t rows, int64_t slices, int64_t keys, int bytes) {
-    const int forced = tuning().tree_form;
+// How a call is cut: which form, and how many workgroups the stages of its blocks are dealt to (0: one to a block).
+struct TreeCut { int form, block_rows, dealt; int64_t row_blocks; };
+static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int bytes) {
+    const int64_t rows = tokens * (heads / kv_heads);
+    const int forced = tuning().tree_form, wanted = tuning().tree_deal;
     const int form = forced >= 0 && forced <= TREE_TALL ? forced : rows <= 32 ? TREE_FEW : rows <= 64 ? TREE_MID : TREE_TALL;
-    const int64_t blocks = ceil_div(rows, (int64_t)(form == TREE_FEW ? 32 : form == TREE_MID ? 64 : 128));
-    return {form, blocks, blocks * slices, ceil_div(keys, (int64_t)(form == TREE_FEW && bytes <= 256 ? 128 : 64))};
+    const int block = form == TREE_FEW ? 32 : form == TREE_MID ? 64 : 128;
+    const int64_t blocks = ceil_div(rows, (int64_t)block);
+    const int64_t items = blocks * batch * kv_heads, most = wanted >= 0 ? wanted : form == TREE_FEW && bytes <= 256 ? 512 : 256;
+    const int dealt = items <= most && batch <= DEAL_ENTRIES ? (int)most : 0;
+    return {form, (int)std::min<int64_t>(block, rows), dealt, blocks};
 }
 
-static int64_t tree_splits(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t keys, int type) {
-    const int forced = tuning().tree_splits;
-    if (forced > 0) return std::min(forced, 256);
-    if (!batch || !tokens || !heads) return 1;
-    const TreeCut cut = tree_cut(tokens * (heads / kv_heads), batch * kv_heads, keys, (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2));
-    return std::max<int64_t>(1, std::min({256 / cut.workgroups, cut.stages, (int64_t)256}));
-}
+static int tree_bytes(int64_t size, int type) { return (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2); }   // of a head's row
+static int64_t tree_scratch(const TreeCut& cut, int64_t size) { return (int64_t)cut.dealt * cut.block_rows * (size + 2); }
 
 template <class T, int D>
-static int launch_tree(TreeArgs p, hipStream_t st) {
+static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
     constexpr int BYTES = D * (int)sizeof(T);
     const int64_t rows = p.tokens * p.share, slices = p.batch * p.kv_heads;
-    const TreeCut cut = tree_cut(rows, slices, p.capacity, BYTES);
     bool fits = true;
     auto launch = [&](auto rb, auto rw, auto kw, auto sub, auto ns, auto per_simd) {
         constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
-        p.row_blocks = ceil_div(rows, (int64_t)(32 * RB * RW));
-        const int64_t grid = p.row_blocks * p.splits * slices;
-        fits = grid_fits(grid, 64 * RW * KW) && (p.splits == 1 || grid_fits(ceil_div(slices * rows, (int64_t)4), 256));
+        constexpr int KT = 32 * KW * SUB, PER_SIMD = decltype(per_simd)::value;
+        const int64_t grid = p.dealt ? p.dealt : p.row_blocks * slices;
+        const bool many_parts = p.dealt > 16 * p.row_blocks * slices;
+        const int64_t joins = p.dealt ? ceil_div(slices * rows, (int64_t)(many_parts ? 1 : 4)) : 0;
+        fits = grid_fits(grid, 64 * RW * KW) && grid_fits(joins, 256);
         if (!fits) return;
-        hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, decltype(per_simd)::value>), dim3((unsigned)grid), dim3(64 * RW * KW), 0, st, p);
+        const dim3 g((unsigned)grid), threads(64 * RW * KW);
+        if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
+        else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
+        if (!joins) return;
+        if (many_parts) hipLaunchKernelGGL((tree_join_kernel<T, D, KT, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((tree_join_kernel<T, D, KT, 1>), dim3((unsigned)joins), dim3(256), 0, st, p);
     };
     if constexpr (BYTES <= 256) {
-        if (cut.form == TREE_FEW) launch(Int<1>{}, Int<1>{}, Int<4>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<1>{});
+        if (cut.form == TREE_FEW) launch(Int<1>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<1>{}, Int<2>{}, Int<1>{});
         else if (cut.form == TREE_MID) launch(Int<1>{}, Int<2>{}, Int<2>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
         else launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<2>{}, Int<2>{}, Int<2>{});
     } else if constexpr (BYTES == 512) {
@@ -441,7 +708,6 @@ static int launch_tree(TreeArgs p, hipStream_t st) {
         else launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<1>{}, Int<2>{}, Int<1>{});
     }
     MI355X_REQUIRE(fits, "tree_attention: too large");
-    if (p.splits > 1) hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3((unsigned)ceil_div(slices * rows, (int64_t)4)), dim3(256), 0, st, p);
     return check_launch("tree_attention_kernel");
 }
 
@@ -456,8 +722,7 @@ static bool tree_fits(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_h
 extern "C" int64_t mi355x_tree_attention_scratch(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t page_size, int64_t columns, int type) {
     using namespace mi355x;
     if (!is_mixed_type(type) || !tree_fits(batch, tokens, heads, kv_heads, size, page_size, columns)) return 0;
-    const int64_t splits = tree_splits(batch, tokens, heads, kv_heads, size, page_size * columns, type);
-    return splits > 1 ? splits * batch * tokens * heads * (size + 2) : 0;
+    return batch && tokens && heads ? tree_scratch(tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type)), size) : 0;
 }
 
 extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const void* v_pages, const int32_t* table, const int32_t* lengths, const int32_t* parents, void* O,
@@ -474,16 +739,18 @@ extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const v
     if (batch == 0 || tokens == 0 || heads == 0) return MI355X_OK;
     MI355X_REQUIRE(Q && O && k_pages && v_pages && lengths && (columns == 0 || table), "tree_attention: null pointer");
     MI355X_REQUIRE(((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0, "tree_attention: pages have to stand at 16-byte boundaries");
-    const int64_t splits = tree_splits(batch, tokens, heads, kv_heads, size, page_size * columns, type), floats = splits > 1 ? splits * batch * tokens * heads * (size + 2) : 0;
+    const TreeCut cut = tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type));
+    const int64_t floats = tree_scratch(cut, size);
     MI355X_REQUIRE(floats == 0 || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 && scratch_floats >= floats), "tree_attention: scratch memory for %lld floats, 16-byte aligned",
                    (long long)floats);
     TreeArgs p = {};
     p.q = Q; p.k_pages = k_pages; p.v_pages = v_pages; p.table = table; p.lengths = lengths; p.parents = parents; p.o = O;
     p.partial_o = scratch;
-    p.partial_ml = scratch ? scratch + splits * batch * tokens * heads * size : nullptr;
-    p.batch = batch; p.tokens = tokens; p.columns = columns;
+    p.partial_ml = scratch ? scratch + (int64_t)cut.dealt * cut.block_rows * size : nullptr;
+    p.batch = batch; p.tokens = tokens; p.columns = columns; p.row_blocks = cut.row_blocks; p.block_rows = cut.block_rows; p.dealt = cut.dealt;
+    p.order = cut.row_blocks * batch * kv_heads <= 512;
     p.pages = (int)pages; p.page_size = (int)page_size; p.capacity = (int)(page_size * columns);
-    p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.share = (int)(heads / kv_heads); p.splits = (int)splits;
+    p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.share = (int)(heads / kv_heads);
     while (((int64_t)1 << p.page_shift) < page_size) ++p.page_shift;
     p.page_magic = (uint32_t)((((uint64_t)1 << (31 + p.page_shift)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
     p.scale_log2 = scale * 1.44269504088896340736f;
@@ -491,7 +758,7 @@ extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const v
     with_type(type, [&](auto t) {
         using T = decltype(t);
         hipStream_t st = static_cast<hipStream_t>(stream);
-        status = size == 64 ? launch_tree<T, 64>(p, st) : size == 128 ? launch_tree<T, 128>(p, st) : launch_tree<T, 256>(p, st);
+        status = size == 64 ? launch_tree<T, 64>(p, cut, st) : size == 128 ? launch_tree<T, 128>(p, cut, st) : launch_tree<T, 256>(p, cut, st);
     });
     return status;
 }
