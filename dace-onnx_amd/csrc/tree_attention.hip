@@ -10,6 +10,7 @@ constexpr int TREE_MOST = 1024;   // tokens of a tree
 struct TreeArgs {
     const void* q; const void* k_pages; const void* v_pages; const int32_t* table; const int32_t* lengths; const int32_t* parents; void* o;
     float* partial_o; float* partial_ml;   // of parts: [workgroup][row of the block][D], [workgroup][row of the block][2]
+    int32_t* plan;                         // [entry][2]: its first workgroup, the parts of its blocks
     int64_t batch, tokens, columns, row_blocks;
     int pages, page_size, capacity;        // capacity = page_size * columns
     int heads, kv_heads, share;            // share = heads / kv_heads
@@ -46,12 +47,12 @@ struct TreeDeal {
     int64_t items;   // blocks of an entry
     uint32_t most, stages[EACH];
     __device__ __forceinline__ uint32_t parts(uint32_t stages) const { return (stages + most - 1) / most; }
-    __device__ __forceinline__ int64_t sum(const TreeArgs& p, int64_t before) const {   // parts of the entries before that one
+    __device__ __forceinline__ int64_t all_parts(const TreeArgs& p) const {
         int64_t all = 0;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            if (i * WAVE >= before) break;
-            all += wave_uint(i * WAVE + (int)(threadIdx.x % WAVE) < before ? parts(stages[i]) : 0u, [](uint32_t x, uint32_t y) { return x + y; });
+            if (i * WAVE >= p.batch) break;
+            all += wave_uint(parts(stages[i]), [](uint32_t x, uint32_t y) { return x + y; });
         }
         return all;
     }
@@ -75,7 +76,7 @@ struct TreeDeal {
         while (low < most) {
             const uint32_t enough = most;
             most = low + (enough - low) / 2;
-            if (sum(p, p.batch) * items <= p.dealt) continue;
+            if (all_parts(p) * items <= p.dealt) continue;
             low = most + 1;
             most = enough;
         }
@@ -104,13 +105,6 @@ struct TreeDeal {
             passed += __builtin_amdgcn_readlane(with, WAVE - 1);
         }
         return false;
-    }
-    __device__ __forceinline__ int parts_of(int64_t b) const {
-        int own = 1;
-#pragma unroll
-        for (int i = 0; i < EACH; ++i)
-            if (b / WAVE == i) own = (int)__shfl((int)parts(stages[i]), (int)(b % WAVE));
-        return own;
     }
 };
 
@@ -243,6 +237,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
     if (p.dealt) {
         const TreeDeal<KT> deal(p);
         if (!deal.find(p, blockIdx.x, b, of_entry, parts)) return;
+        if (of_entry == 0 && tid == 0) p.plan[2 * b] = (int32_t)blockIdx.x, p.plan[2 * b + 1] = parts;
         part = (int)(of_entry % parts);
         group = (int)(of_entry / parts / p.row_blocks);
         block = of_entry / parts % p.row_blocks;
@@ -359,6 +354,12 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             q[i][s].set(v);
         }
     }
+    // The queries are here before the loop begins: the compiler would wait for them in it, each time, and so for all transfers, which count with them.
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int s = 0; s < Wave::QP; ++s)
+            if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(q[i][s].part[0]));
     f32x16 out[RB][VT];
     float base[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
 #pragma unroll
@@ -404,23 +405,31 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             __syncthreads();
             odd = odd_keys[turn % 2];
         }
+        if (stage * KT + key_wave * SUB * 32 >= wave_end) continue;   // (the same for the wave)
+        // Scores of the next 32 keys are on the matrix unit while the vector unit is at the probabilities of these.
+        f32x16 scores[SUB][RB];
+        const uint32_t keys0 = lds0 + (uint32_t)(buffer * STAGE + key_wave * SUB * 32 * Tile::ROW);
+        auto score = [&](int u) __attribute__((always_inline)) {
+            uint32_t lds_k = keys0 + (uint32_t)(u * 32 * Tile::ROW) + key_at;
+            asm volatile("" : "+v"(lds_k));   // (nothing made of it is kept from one pass to the next)
+            if constexpr (AHEAD) tree_scores<T, D>(lds_k, q, scores[u]);
+            else Wave::scores(lds_k, q, scores[u]);
+        };
+        __builtin_amdgcn_s_setprio(1);
+        score(SUB - 1);
 #pragma unroll
         for (int u = SUB - 1; u >= 0; --u) {
             const int local = (key_wave * SUB + u) * 32, key0 = stage * KT + local;
-            if (key0 >= wave_end) continue;   // (the same for the wave)
-            uint32_t lds_k = lds0 + (uint32_t)(buffer * STAGE + local * Tile::ROW), lds_v = lds_k + HALF + value_at;
-            lds_k += key_at;
-            asm volatile("" : "+v"(lds_k), "+v"(lds_v));   // (nothing made of them is kept from one pass to the next)
-            f32x16 s[RB];
+            uint32_t lds_v = keys0 + (uint32_t)(u * 32 * Tile::ROW) + HALF + value_at;
+            asm volatile("" : "+v"(lds_v));
             typename Values<T, 8>::vec held[AHEAD ? 2 * VT : 1];
+            f32x16 (&s)[RB] = scores[u];
             __builtin_amdgcn_s_setprio(1);
             if constexpr (AHEAD) {
-                tree_scores<T, D>(lds_k, q, s);
                 tree_read_values<T, D>(lds_v, held);
                 __builtin_amdgcn_sched_barrier(0);
-            } else {
-                Wave::scores(lds_k, q, s);
             }
+            if (u > 0) score(u - 1);
             __builtin_amdgcn_s_setprio(0);
             uint32_t seen[RB];   // of the 32 keys
 #pragma unroll
@@ -586,7 +595,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
 }
 
 // The parts of a row joined: WAVES waves to a row share its parts, the lanes of each are the D values. A block of one part is done.
-template <class T, int D, int KT, int WAVES>
+template <class T, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs p) {
     constexpr int PER_LANE = D / WAVE, ROWS = 4 / WAVES, BATCH = 8;
     __shared__ float sums[4][D + 2];
@@ -596,12 +605,11 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs p) {
     if (at >= p.batch * p.kv_heads * rows) return;   // (of waves that share a row: all)
     const int64_t slice = at / rows, row = at % rows, b = slice / p.kv_heads, block = row / p.block_rows;
     const int group = (int)(slice % p.kv_heads);
-    const TreeDeal<KT> deal(p);
-    const int parts = __builtin_amdgcn_readfirstlane(deal.parts_of(b));
+    const int parts = __builtin_amdgcn_readfirstlane(p.plan[2 * b + 1]);
     if (parts == 1) return;
     T* to = static_cast<T*>(p.o) + ((b * p.tokens + row / p.share) * p.heads + group * p.share + (int)(row % p.share)) * D + lane * PER_LANE;
     float top = -__builtin_inff(), sum = 0.0f, o[PER_LANE] = {};
-    const int64_t first = deal.sum(p, b) * deal.items + (group * p.row_blocks + block) * parts;   // workgroup
+    const int64_t first = p.plan[2 * b] + (group * p.row_blocks + block) * parts;   // workgroup
     for (int part = share; part < parts; part += BATCH * WAVES) {
         float base[BATCH], weight[BATCH], values[BATCH][PER_LANE], now = top;
 #pragma unroll
@@ -672,7 +680,7 @@ static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv
 }
 
 static int tree_bytes(int64_t size, int type) { return (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2); }   // of a head's row
-static int64_t tree_scratch(const TreeCut& cut, int64_t size) { return (int64_t)cut.dealt * cut.block_rows * (size + 2); }
+static int64_t tree_scratch(const TreeCut& cut, int64_t batch, int64_t size) { return cut.dealt ? (int64_t)cut.dealt * cut.block_rows * (size + 2) + 2 * batch : 0; }
 
 template <class T, int D>
 static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
@@ -681,7 +689,7 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
     bool fits = true;
     auto launch = [&](auto rb, auto rw, auto kw, auto sub, auto ns, auto per_simd) {
         constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
-        constexpr int KT = 32 * KW * SUB, PER_SIMD = decltype(per_simd)::value;
+        constexpr int PER_SIMD = decltype(per_simd)::value;
         const int64_t grid = p.dealt ? p.dealt : p.row_blocks * slices;
         const bool many_parts = p.dealt > 16 * p.row_blocks * slices;
         const int64_t joins = p.dealt ? ceil_div(slices * rows, (int64_t)(many_parts ? 1 : 4)) : 0;
@@ -691,8 +699,8 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
         if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
         else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
         if (!joins) return;
-        if (many_parts) hipLaunchKernelGGL((tree_join_kernel<T, D, KT, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((tree_join_kernel<T, D, KT, 1>), dim3((unsigned)joins), dim3(256), 0, st, p);
+        if (many_parts) hipLaunchKernelGGL((tree_join_kernel<T, D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((tree_join_kernel<T, D, 1>), dim3((unsigned)joins), dim3(256), 0, st, p);
     };
     if constexpr (BYTES <= 256) {
         if (cut.form == TREE_FEW) launch(Int<1>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<1>{}, Int<2>{}, Int<1>{});
@@ -722,7 +730,7 @@ static bool tree_fits(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_h
 extern "C" int64_t mi355x_tree_attention_scratch(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t page_size, int64_t columns, int type) {
     using namespace mi355x;
     if (!is_mixed_type(type) || !tree_fits(batch, tokens, heads, kv_heads, size, page_size, columns)) return 0;
-    return batch && tokens && heads ? tree_scratch(tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type)), size) : 0;
+    return batch && tokens && heads ? tree_scratch(tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type)), batch, size) : 0;
 }
 
 extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const void* v_pages, const int32_t* table, const int32_t* lengths, const int32_t* parents, void* O,
@@ -740,13 +748,14 @@ extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const v
     MI355X_REQUIRE(Q && O && k_pages && v_pages && lengths && (columns == 0 || table), "tree_attention: null pointer");
     MI355X_REQUIRE(((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0, "tree_attention: pages have to stand at 16-byte boundaries");
     const TreeCut cut = tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type));
-    const int64_t floats = tree_scratch(cut, size);
+    const int64_t floats = tree_scratch(cut, batch, size);
     MI355X_REQUIRE(floats == 0 || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 && scratch_floats >= floats), "tree_attention: scratch memory for %lld floats, 16-byte aligned",
                    (long long)floats);
     TreeArgs p = {};
     p.q = Q; p.k_pages = k_pages; p.v_pages = v_pages; p.table = table; p.lengths = lengths; p.parents = parents; p.o = O;
     p.partial_o = scratch;
     p.partial_ml = scratch ? scratch + (int64_t)cut.dealt * cut.block_rows * size : nullptr;
+    p.plan = scratch ? reinterpret_cast<int32_t*>(p.partial_ml + (int64_t)2 * cut.dealt * cut.block_rows) : nullptr;
     p.batch = batch; p.tokens = tokens; p.columns = columns; p.row_blocks = cut.row_blocks; p.block_rows = cut.block_rows; p.dealt = cut.dealt;
     p.order = cut.row_blocks * batch * kv_heads <= 512;
     p.pages = (int)pages; p.page_size = (int)page_size; p.capacity = (int)(page_size * columns);
