@@ -664,22 +664,62 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs p) {
     store_values(to, o, PER_LANE);
 }
 
-enum { TREE_FEW, TREE_MID, TREE_TALL };
+// PAIR: 64 rows by two row and two key waves, two workgroups to a CU; DEEP: 64 rows by two and four, one to a CU; TALL: 128 rows by four row waves, two to a CU, where each SIMD has two waves
+// and the matrix unit is busy, but with one to a CU it has one. Heads of more than 256 bytes: one to a CU, no DEEP. (32 rows by two waves were behind PAIR with few rows too:
+// two waves are not enough to get the transfers out.)
+enum { TREE_PAIR, TREE_DEEP, TREE_TALL, TREE_FORMS };
 
-// How a call is cut: which form, and how many workgroups the stages of its blocks are dealt to (0: one to a block).
-struct TreeCut { int form, block_rows, dealt; int64_t row_blocks; };
-static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int bytes) {
-    const int64_t rows = tokens * (heads / kv_heads);
-    const int forced = tuning().tree_form, wanted = tuning().tree_deal;
-    const int form = forced >= 0 && forced <= TREE_TALL ? forced : rows <= 32 ? TREE_FEW : rows <= 64 ? TREE_MID : TREE_TALL;
-    const int block = form == TREE_FEW ? 32 : form == TREE_MID ? 64 : 128;
-    const int64_t blocks = ceil_div(rows, (int64_t)block);
-    const int64_t items = blocks * batch * kv_heads, most = wanted >= 0 ? wanted : form == TREE_FEW && bytes <= 256 ? 512 : 256;
-    const int dealt = items <= most && batch <= DEAL_ENTRIES ? (int)most : 0;
-    return {form, (int)std::min<int64_t>(block, rows), dealt, blocks};
+// us: of 64 keys where a workgroup has its CU alone, and where another shares it; of a round of workgroups besides
+struct TreeForm { int rows, places; double alone, shared, start; };
+static TreeForm tree_form(int form, int bytes, bool f32) {
+    const int size = bytes / (f32 ? 4 : 2);
+    // by 8 x 64 and 8 x 8 tokens behind 4096, 1 to 16 heads of 1 to 4 groups, and prompts of 512 to 4096 tokens
+    const double rates[6][TREE_FORMS][2] = {{{0.65, 1.0}, {0.57, 0.57}, {1.12, 1.45}},   // 16 bits, heads of 64
+                                            {{1.05, 1.75}, {0.82, 0.82}, {1.55, 2.2}},    // 128
+                                            {{2.1, 2.1}, {}, {3.2, 3.2}},                 // 256
+                                            {{2.2, 3.0}, {1.6, 1.6}, {3.7, 5.0}},         // float32, 64
+                                            {{3.9, 3.9}, {}, {6.7, 6.7}},
+                                            {{14.5, 14.5}, {}, {13.5, 13.5}}};
+    const double(&rate)[2] = rates[(f32 ? 3 : 0) + (size == 64 ? 0 : size == 128 ? 1 : 2)][form];
+    return {form == TREE_TALL ? 128 : 64, form == TREE_DEEP || bytes > 256 ? 256 : 512, rate[0], rate[1], form == TREE_DEEP ? 10.0 : 8.0};
 }
 
-static int tree_bytes(int64_t size, int type) { return (int)size * (type == MI355X_TYPE_FLOAT ? 4 : 2); }   // of a head's row
+// How a call is cut: which form, and how many workgroups the parts of its blocks are dealt to (0: one to a block), by what the forms take if the longest of the entries fills its table and they do
+// by two thirds. Measured, us, at heads of 128 in 16 bits (PAIR / DEEP / TALL, one workgroup to a block; the best in parts): 16 x 1 token of up to 8192, 32 heads in 8 groups 146 / 118 / 185, 73;
+// 32 x 1 159 / 140 / 180, 128; 8 trees of 64 behind 4000 69 / 54 / 97, 55; 2 of 256 57 / 45 / 80, 51; 4 of 32 67 / 51 / 98, 29; a prompt of 512 17.4 / 17.5 / 22, 22; of 1024 28 / 39 / 35, 38; of 2048
+// 65 / 84 / 63, 92; 4096 behind 4096, 16 heads in 4 groups 259 / 292 / 241, 300.
+struct TreeCut { int form, block_rows, dealt; int64_t row_blocks; };
+static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, int64_t size, int type) {
+    const bool f32 = type == MI355X_TYPE_FLOAT;
+    const int bytes = (int)size * (f32 ? 4 : 2), forced = tuning().tree_form, wanted = tuning().tree_deal;
+    const int64_t rows = tokens * (heads / kv_heads), slices = batch * kv_heads;
+    const double most = std::max(1.0, (double)capacity / 64), mean = std::max(1.0, ((double)capacity - 0.5 * (double)std::min(tokens, capacity)) / 64);
+    const double full = batch > 1 ? 0.67 : 1.0, least_memory = full * (double)slices * (double)capacity * 2 * bytes / 5e6;
+    TreeCut best = {};
+    double least = __builtin_inf();
+    for (int form = 0; form < TREE_FORMS; ++form) {
+        if ((forced >= 0 && forced < TREE_FORMS && form != forced) || (form == TREE_DEEP && bytes > 256)) continue;
+        const TreeForm f = tree_form(form, bytes, f32);
+        const int64_t blocks = ceil_div(rows, (int64_t)f.rows), items = blocks * slices;
+        const int block_rows = (int)std::min<int64_t>(f.rows, rows);
+        // what the bytes take goes by how many workgroups ask for them; with one to a block the longest entry's are the last
+        const double memory = least_memory * (form == TREE_PAIR ? 1.0 : form == TREE_DEEP ? 1.1 : 1.3), uneven = batch > 1 ? 1.25 : 1.0, rounds = (double)items / f.places;
+        const double whole = f.start + std::max(memory * uneven, items <= 256 ? most * f.alone : items <= f.places ? std::max(most * f.alone, full * mean * f.shared) :
+                                                                  rounds * full * mean * (f.places > 256 ? f.shared : f.alone) + (rounds - 1) * f.start);
+        if (wanted <= 0 && whole < least) least = whole, best = {form, block_rows, 0, blocks};
+        const int64_t places = wanted > 0 ? wanted : form == TREE_TALL ? 256 : f.places;
+        if (wanted == 0 || items > places || batch > DEAL_ENTRIES) continue;
+        const double used = std::min((double)places, (double)items * most);   // parts are whole stages, and no block has less than one: a quarter more than even ones
+        const double parts = 3 + f.start + std::max(memory, 1.25 * (double)items * full * most / used * (used > 256 ? f.shared : f.alone)) + 4.5 + used * block_rows * (double)size * 8 / 4.5e6;
+        if (parts < least) least = parts, best = {form, block_rows, (int)places, blocks};
+    }
+    if (!best.row_blocks) {   // (forced, and not possible so)
+        const TreeForm f = tree_form(TREE_PAIR, bytes, f32);
+        best = {TREE_PAIR, (int)std::min<int64_t>(f.rows, rows), 0, ceil_div(rows, (int64_t)f.rows)};
+    }
+    return best;
+}
+
 static int64_t tree_scratch(const TreeCut& cut, int64_t batch, int64_t size) { return cut.dealt ? (int64_t)cut.dealt * cut.block_rows * (size + 2) + 2 * batch : 0; }
 
 template <class T, int D>
@@ -702,19 +742,10 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
         if (many_parts) hipLaunchKernelGGL((tree_join_kernel<T, D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
         else hipLaunchKernelGGL((tree_join_kernel<T, D, 1>), dim3((unsigned)joins), dim3(256), 0, st, p);
     };
-    if constexpr (BYTES <= 256) {
-        if (cut.form == TREE_FEW) launch(Int<1>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<1>{}, Int<2>{}, Int<1>{});
-        else if (cut.form == TREE_MID) launch(Int<1>{}, Int<2>{}, Int<2>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
-        else launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<2>{}, Int<2>{}, Int<2>{});
-    } else if constexpr (BYTES == 512) {
-        if (cut.form == TREE_FEW) launch(Int<1>{}, Int<1>{}, Int<2>{}, Int<1>{}, Int<2>{}, Int<1>{});
-        else if (cut.form == TREE_MID) launch(Int<1>{}, Int<2>{}, Int<2>{}, Int<1>{}, Int<2>{}, Int<1>{});
-        else launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<1>{}, Int<2>{}, Int<1>{});
-    } else {
-        if (cut.form == TREE_FEW) launch(Int<1>{}, Int<1>{}, Int<1>{}, Int<1>{}, Int<2>{}, Int<1>{});
-        else if (cut.form == TREE_MID) launch(Int<1>{}, Int<2>{}, Int<1>{}, Int<1>{}, Int<2>{}, Int<1>{});
-        else launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<1>{}, Int<2>{}, Int<1>{});
-    }
+    constexpr bool WIDE = BYTES > 256, WIDEST = BYTES > 512;
+    if (cut.form == TREE_PAIR) launch(Int<1>{}, Int<2>{}, Int<(WIDEST ? 1 : 2)>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<(WIDE ? 1 : 2)>{});
+    else if (cut.form == TREE_TALL) launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<(WIDE ? 1 : 2)>{}, Int<2>{}, Int<(WIDE ? 1 : 2)>{});
+    else if constexpr (!WIDE) launch(Int<1>{}, Int<2>{}, Int<4>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
     MI355X_REQUIRE(fits, "tree_attention: too large");
     return check_launch("tree_attention_kernel");
 }
@@ -730,7 +761,7 @@ static bool tree_fits(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_h
 extern "C" int64_t mi355x_tree_attention_scratch(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size, int64_t page_size, int64_t columns, int type) {
     using namespace mi355x;
     if (!is_mixed_type(type) || !tree_fits(batch, tokens, heads, kv_heads, size, page_size, columns)) return 0;
-    return batch && tokens && heads ? tree_scratch(tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type)), batch, size) : 0;
+    return batch && tokens && heads ? tree_scratch(tree_cut(batch, tokens, heads, kv_heads, page_size * columns, size, type), batch, size) : 0;
 }
 
 extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const void* v_pages, const int32_t* table, const int32_t* lengths, const int32_t* parents, void* O,
@@ -747,7 +778,7 @@ extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const v
     if (batch == 0 || tokens == 0 || heads == 0) return MI355X_OK;
     MI355X_REQUIRE(Q && O && k_pages && v_pages && lengths && (columns == 0 || table), "tree_attention: null pointer");
     MI355X_REQUIRE(((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0, "tree_attention: pages have to stand at 16-byte boundaries");
-    const TreeCut cut = tree_cut(batch, tokens, heads, kv_heads, tree_bytes(size, type));
+    const TreeCut cut = tree_cut(batch, tokens, heads, kv_heads, page_size * columns, size, type);
     const int64_t floats = tree_scratch(cut, batch, size);
     MI355X_REQUIRE(floats == 0 || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 && scratch_floats >= floats), "tree_attention: scratch memory for %lld floats, 16-byte aligned",
                    (long long)floats);

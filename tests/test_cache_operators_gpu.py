@@ -242,6 +242,32 @@ def test_attention_of_prompts(dtype, d, tokens, heads, groups, page, context):
     check_attention(2, tokens, heads, groups, d, page, context, dtype)
 
 
+@pytest.mark.parametrize("form", range(3))
+@pytest.mark.parametrize("dealt", [0, 5, 64, 512])
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("batch, tokens, heads, groups, page, context, tree", [(1, 3, 2, 1, 16, 300, True), (2, 150, 2, 2, 4, 129, False), (3, 70, 4, 1, 7, 260, True), (1, 300, 1, 1, 64, 0, False)])
+def test_attention_by_every_kernel(form, dealt, dtype, d, batch, tokens, heads, groups, page, context, tree, tuning):
+    """One workgroup to a block of rows, and its keys in parts: fewer workgroups than blocks (which have one each then), about as many, and more than there are stages."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    check_attention(batch, tokens, heads, groups, d, page, context, dtype, tree)
+
+
+@pytest.mark.parametrize("dealt", [0, 300, 512])
+@pytest.mark.parametrize("batch", [63, 64, 65, 130, 256, 257])
+def test_attention_of_many_entries(batch, dealt, tuning):
+    """Entries of all lengths, more of them than a wave has lanes, and than parts are dealt for."""
+    tuning(MI355X_TREE_DEAL=dealt)
+    lengths = [(37 * b * b) % 700 if b % 5 else 0 for b in range(batch)]
+    check_attention(batch, 2, 2, 1, 64, 16, 700, BF, lengths=lengths)
+
+
+def test_attention_of_one_long_entry_among_short_ones(tuning):
+    for dealt in (-1, 64, 256):
+        tuning(MI355X_TREE_DEAL=dealt)
+        check_attention(8, 1, 4, 2, 128, 16, 20000, BF, lengths=[0, 3, 20000, 1, 0, 64, 127, 128])
+
+
 @pytest.mark.parametrize("dtype", R.TYPES)
 def test_attention_of_large_trees(dtype):
     check_attention(1, 1024, 2, 1, 64, 16, 50, dtype, True)
@@ -391,9 +417,20 @@ def test_acceptance(dtype, tree, batch, tokens, vocabulary):
         check_acceptance(logits, drafts(3, logits, parents, hit), parents)
 
 
+@pytest.mark.parametrize("parts", [1, 2, 7, 64])
 @pytest.mark.parametrize("dtype", R.TYPES)
-def test_acceptance_of_equal_logits_and_of_none(dtype):
+@pytest.mark.parametrize("vocabulary", [1, 5, 63, 1025, 40001])
+def test_acceptance_in_any_number_of_parts(parts, dtype, vocabulary, tuning):
+    tuning(MI355X_ACCEPT_PARTS=parts)
+    logits = normal(1, 2, 5, vocabulary, scale=2.0, dtype=dtype)
+    check_acceptance(logits, drafts(3, logits, None, 0.8))
+
+
+@pytest.mark.parametrize("parts", [None, 5])
+@pytest.mark.parametrize("dtype", R.TYPES)
+def test_acceptance_of_equal_logits_and_of_none(dtype, parts, tuning):
     """The first of equal ones wherever they stand, 0 and -0 alike; rows of infinities and of NaN; a NaN next to numbers."""
+    tuning(MI355X_ACCEPT_PARTS=parts)
     inf, nan, V = float("inf"), float("nan"), 3001
     rows = torch.full((1, 12, V), -1.0)
     rows[0, 0, [17, 16, 2999]] = 5.0
