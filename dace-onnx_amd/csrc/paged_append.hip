@@ -1,8 +1,10 @@
 // PagedCacheAppend: the keys and values of a call's tokens to their rows of a cache in pages; keys, and the call's queries, turned by the tokens' positions on the way.
 // Arrays in float32, float16 or bfloat16, turned in float32. The reference has no such node.
 //
-// Token j of entry b becomes number n = lengths[b] + j of the entry: row n % page of page table[b, n / page], whatever order the pages were handed out in. Everything else is
-// as in RotaryPositions: a workgroup has a few tokens, whose places and angles are found once, into LDS, and then serve all heads.
+// Token j of entry b becomes number n = lengths[b] + j of the entry: row n % page of page table[b, n / page], whatever order the pages were handed out in. Pair i of a head is turned
+// by position * frequencies[i] (rotary.h). A workgroup has a few tokens, whose places and angles are found once, into LDS, and then serve their heads.
+// Bound by the bytes of the heads: 16384 tokens of 32 + 2 x 8 heads of 128 in bfloat16 79 us, 5.1 TB/s (a copy of 1 GiB 5.1); with few tokens by three reads that need each other (a
+// length, the page, the values) and the launch: 16 tokens 4.2 us, 225 tokens of 2 x 6 heads of 64 in float32 4.4.
 #include "mixed.h"
 #include "rotary.h"
 
@@ -17,7 +19,7 @@ struct AppendArgs {
     const int32_t* table; const int32_t* lengths; const float* frequencies; const void* positions; const int32_t* order;
     int64_t all, tokens, taken, pages, page_size, columns;   // all = batch * taken
     int64_t per_axis;                                        // batch * tokens
-    int heads, kv_heads, size, rotated, axes, tokens_per_wg;
+    int heads, kv_heads, size, rotated, axes, tokens_per_wg, heads_per_wg;
     int end[ROTARY_MAX_AXES];   // one past the last pair of each axis
     int wide_positions;         // 64 bits, not 32
 };
@@ -28,18 +30,16 @@ struct AppendPlace {
     int32_t page, row;
 };
 
+__device__ __forceinline__ AppendPlace append_source(const AppendArgs& p, int64_t at) {
+    const int64_t b = at / p.taken, j = at % p.taken, length = p.lengths[b], i = p.order ? p.order[at] : j;
+    return {i >= 0 && i < p.tokens ? b * p.tokens + i : -1, (length < 0 ? 0 : length) + j, -1, 0};
+}
+
 __device__ __forceinline__ AppendPlace append_place(const AppendArgs& p, int64_t at) {
-    const int64_t b = at / p.taken, j = at % p.taken, length = p.lengths[b];
-    AppendPlace place = {j, (length < 0 ? 0 : length) + j, -1, 0};
-    if (p.order) place.source = p.order[at];
+    AppendPlace place = append_source(p, at);
     const int64_t column = place.number / p.page_size;
-    if (place.source < 0 || place.source >= p.tokens) {
-        place.source = -1;
-        return place;
-    }
-    place.source += b * p.tokens;
     if (column < p.columns) {
-        const int32_t page = p.table[b * p.columns + column];
+        const int32_t page = p.table[at / p.taken * p.columns + column];
         if (page >= 0 && page < p.pages) place.page = page;
         place.row = (int32_t)(place.number - column * p.page_size);
     }
@@ -71,11 +71,12 @@ __global__ __launch_bounds__(APPEND_THREADS) void paged_append_kernel(AppendArgs
     const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_wg;
     const int tokens = (int)(p.all - token0 < p.tokens_per_wg ? p.all - token0 : p.tokens_per_wg);
     const int pairs = p.rotated / 2;
+    // Places and angles at once: a thread that takes an angle looks for the token's number itself rather than wait for the one that looks into the table.
     if ((int)threadIdx.x < tokens) places[threadIdx.x] = append_place(p, token0 + threadIdx.x);
-    __syncthreads();
     for (int i = threadIdx.x; i < tokens * pairs; i += APPEND_THREADS) {
         const int token = i / pairs, pair = i % pairs;
-        const AppendPlace& place = places[token];
+        const float frequency = p.frequencies[pair];
+        const AppendPlace place = append_source(p, token0 + token);
         if (place.source < 0) continue;
         int64_t position = place.number;
         if (p.positions) {
@@ -84,15 +85,15 @@ __global__ __launch_bounds__(APPEND_THREADS) void paged_append_kernel(AppendArgs
             const int64_t at = axis * p.per_axis + place.source;
             position = p.wide_positions ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
         }
-        turn[i] = rotary_turn(position, p.frequencies[pair]);
+        turn[i] = rotary_turn(position, frequency);
     }
     __syncthreads();
 
     const int copied = p.size - p.rotated;
     const int turning = pairs / VEC, steps = turning + (copied + 2 * VEC - 1) / (2 * VEC);   // of a head; of one that is copied whole no more
-    const int all_heads = p.heads + 2 * p.kv_heads;
-    for (int i = threadIdx.x; i < tokens * all_heads * steps; i += APPEND_THREADS) {
-        const int step = i % steps, head = i / steps % all_heads, token = i / steps / all_heads;
+    const int all_heads = p.heads + 2 * p.kv_heads, head0 = blockIdx.y * p.heads_per_wg, my_heads = min(p.heads_per_wg, all_heads - head0);
+    for (int i = threadIdx.x; i < tokens * my_heads * steps; i += APPEND_THREADS) {
+        const int step = i % steps, head = head0 + i / steps % my_heads, token = i / steps / my_heads;
         const AppendPlace& place = places[token];
         if (place.source < 0 || (head >= p.heads && place.page < 0)) continue;
         const T* x;
@@ -143,11 +144,21 @@ __global__ __launch_bounds__(APPEND_THREADS) void paged_append_kernel(AppendArgs
 }
 
 template <class T>
-static void launch_append(const AppendArgs& p, bool interleaved, hipStream_t st) {
+static void launch_append(AppendArgs p, bool interleaved, hipStream_t st) {
     const int pairs = p.rotated / 2;
-    const dim3 grid((unsigned)ceil_div(p.all, (int64_t)p.tokens_per_wg)), block(APPEND_THREADS);
+    const dim3 block(APPEND_THREADS);
     auto launch = [&](auto vec) {
         constexpr int VEC = decltype(vec)::value;
+        // Few tokens: one to a workgroup, and no more of its heads than its threads have a step of. Otherwise four tokens share what is found out about pages and angles. us, tokens of
+        // 32 + 2 x 8 heads of 128, four whole ones / shares of one: 16 in bfloat16 6.4 / 4.2 (the kernel alone); with the call around it: 512 in float32 12.2 / 7.8, 1024 in bfloat16 9.6 / 8.4,
+        // 2048 11.4 / 13.0, 4096 17.9 / 21.2.
+        const int all_heads = p.heads + 2 * p.kv_heads, steps = (p.size + 2 * VEC - 1) / (2 * VEC);
+        p.heads_per_wg = all_heads;
+        if (p.all <= 1024) {
+            p.tokens_per_wg = 1;
+            p.heads_per_wg = std::min(all_heads, std::max(1, APPEND_THREADS / std::max(steps, 1)));
+        }
+        const dim3 grid((unsigned)ceil_div(p.all, (int64_t)p.tokens_per_wg), (unsigned)ceil_div((int64_t)all_heads, (int64_t)p.heads_per_wg));
         if (interleaved) hipLaunchKernelGGL((paged_append_kernel<T, VEC, true>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((paged_append_kernel<T, VEC, false>), grid, block, 0, st, p);
     };
@@ -178,7 +189,7 @@ extern "C" int mi355x_paged_cache_append(const void* K, const void* V, const voi
     MI355X_REQUIRE(batch < (int64_t)1 << 31 && tokens < (int64_t)1 << 31 && taken < (int64_t)1 << 31 && pages < (int64_t)1 << 31 && page_size < (int64_t)1 << 31 &&
                        columns < (int64_t)1 << 31, "paged_cache_append: too large");
     AppendArgs p = {K, V, Q, k_pages, v_pages, Q_out, table, lengths, frequencies, positions, order, batch * taken, tokens, taken, pages, page_size, columns, batch * tokens,
-                    (int)heads, (int)kv_heads, (int)size, (int)rotated, (int)axes, 1, {}, position_bytes == 8};
+                    (int)heads, (int)kv_heads, (int)size, (int)rotated, (int)axes, 1, 1, {}, position_bytes == 8};
     int64_t pairs = 0;
     for (int64_t a = 0; a < axes; ++a) {
         MI355X_REQUIRE(sections[a] >= 0 && sections[a] <= rotated / 2, "paged_cache_append: section of %lld pairs", (long long)sections[a]);
