@@ -91,11 +91,11 @@ struct Operand<float> {
     }
 };
 
-// Queries and keys of D values, of which a row of W holds W / D (maps); values of W
-template <class T, int W, int D>
+// Queries and keys of D values, of which a row of W holds W / D (maps); values of W, of which the wave has COLUMNS
+template <class T, int W, int D, int COLUMNS = W>
 struct AttentionWave {
     using Tile = AttentionTile<T, W>;
-    static constexpr int E = Tile::E, QP = D / 16, VT = W / 32;   // operands of a map's query or key, tiles of 32 value columns
+    static constexpr int E = Tile::E, QP = D / 16, VT = COLUMNS / 32;   // operands of a map's query or key, tiles of 32 value columns
 
     typedef T Piece __attribute__((ext_vector_type(E)));
     typedef Piece UnalignedPiece __attribute__((aligned(sizeof(T))));

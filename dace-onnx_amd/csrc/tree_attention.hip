@@ -150,38 +150,41 @@ __device__ __forceinline__ void run_to_lds(const void* base, const uint32_t* lan
 // S^T of 32 keys and 32 rows, the keys' operands on their way from LDS all at once: one after the other each product waits for its own.
 template <class T, int D, int RB>
 __device__ __forceinline__ void tree_scores(uint32_t lds_k, const Operand<T> (&q)[RB][D / 16], f32x16 (&acc)[RB]) {
-    using Wave = AttentionWave<T, D, D>;
-    typename Values<T, 8>::vec k[D / 16];
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) k[s] = Wave::template read<typename Values<T, 8>::vec>(lds_k ^ (32 * s), 0);
-    __builtin_amdgcn_sched_barrier(0);
+    constexpr int BATCH = D / 16 < 8 ? D / 16 : 8;
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f32x16{};
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s)
+    for (int s0 = 0; s0 < D / 16; s0 += BATCH) {
+        typename Values<T, 8>::vec k[BATCH];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) Operand<T>::product({{k[s]}}, q[b][s], acc[b]);
+        for (int s = 0; s < BATCH; ++s) k[s] = AttentionWave<T, D, D>::template read<typename Values<T, 8>::vec>(lds_k ^ (32 * (s0 + s)), 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) Operand<T>::product({{k[s]}}, q[b][s0 + s], acc[b]);
+    }
 }
 
 // The values' operands of 32 keys: in registers by the time the probabilities are
-template <class T, int D>
-__device__ __forceinline__ void tree_read_values(uint32_t lds_v, typename Values<T, 8>::vec (&v)[2 * D / 32]) {
+template <class T, int D, int VT>
+__device__ __forceinline__ void tree_read_values(uint32_t lds_v, typename Values<T, 8>::vec (&v)[2 * VT]) {
     constexpr int ROW = AttentionTile<T, D>::ROW;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < VT; ++c) {
             s16x4 half[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 half[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(reinterpret_cast<__attribute__((address_space(3))) char*>(
                     lds_v ^ (16 * (4 * c ^ 2 * i))) + (16 * t + 8 * i) * ROW));
-            v[t * (D / 32) + c] = __builtin_bit_cast(typename Values<T, 8>::vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            v[t * VT + c] = __builtin_bit_cast(typename Values<T, 8>::vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
         }
 }
 
-template <class T, int D, int RB>
-__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * D / 32], const f32x16 (&prob)[RB], f32x16 (&out)[RB][D / 32], float (&sum)[RB]) {
+template <class T, int VT, int RB>
+__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * VT], const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         Operand<T> pr[RB];
@@ -194,34 +197,35 @@ __device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v
             pr[b].add_to(sum[b], x);
         }
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)
+        for (int c = 0; c < VT; ++c)
 #pragma unroll
-            for (int b = 0; b < RB; ++b) Operand<T>::product({{v[t * (D / 32) + c]}}, pr[b], out[b][c]);
+            for (int b = 0; b < RB; ++b) Operand<T>::product({{v[t * VT + c]}}, pr[b], out[b][c]);
     }
 }
 
-// Waves: RW blocks of 32 RB rows, KW shares of a stage's keys, 32 SUB each; NS stages. WHOLE: no transfer's keys lie in two pages.
-template <class T, int D, int RB, int RW, int KW, int SUB, int NS, int PER_SIMD, bool WHOLE>
-__global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(TreeArgs p) {
+// Waves: RW blocks of 32 RB rows, CW shares of the value columns (each takes the scores for itself), KW shares of a stage's keys, 32 SUB each; NS stages. WHOLE: no transfer's keys lie in
+// two pages.
+template <class T, int D, int RB, int RW, int CW, int KW, int SUB, int NS, int PER_SIMD, bool WHOLE>
+__global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_kernel(TreeArgs p) {
     using Tile = AttentionTile<T, D>;
-    using Wave = AttentionWave<T, D, D>;
+    using Wave = AttentionWave<T, D, D, D / CW>;
     using Piece = typename Wave::Piece;
     using UnalignedPiece = typename Wave::UnalignedPiece;
-    constexpr int KT = 32 * KW * SUB, E = Tile::E, NT = 64 * RW * KW, VT = Wave::VT, ROWS = 32 * RB * RW;
+    constexpr int KT = 32 * KW * SUB, E = Tile::E, NT = 64 * RW * CW * KW, VT = Wave::VT, ROWS = 32 * RB * RW;
     constexpr int HALF = KT * Tile::ROW, STAGE = 2 * HALF;            // keys, then values
     constexpr int PER_T = KT * Tile::PIECES / NT, KPT = WAVE / Tile::PIECES;   // transfers of a wave's keys in a stage, keys to a transfer
     static_assert(KT * Tile::PIECES % NT == 0 && Tile::PIECES <= WAVE && NS >= 2 && (NS - 2) * 2 * PER_T < 64, "whole pieces to a thread, whole keys to a transfer");
-    constexpr int EXCHANGE = 32 * D;   // floats of a row block's output
-    constexpr bool AHEAD = sizeof(T) == 2 && D <= 128;   // operands are read from LDS all at once, before they are needed
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[std::max(NS * STAGE, KW == 1 ? 0 : 4 * EXCHANGE * (KW / 2) * RW * RB)];
+    constexpr int EXCHANGE = 32 * D / CW;   // floats of a wave's output
+    constexpr bool AHEAD = sizeof(T) == 2;   // operands are read from LDS all at once, before they are needed
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[std::max(NS * STAGE, KW == 1 ? 0 : 4 * EXCHANGE * (KW / 2) * RW * CW * RB)];
     __shared__ int16_t parents[TREE_MOST];
     __shared__ uint32_t odd_keys[2][KT / 32];   // of the stage and the one before
 
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    const int n = lane % 32, h = lane / 32, row_wave = wave % RW, key_wave = wave / RW;
+    const int n = lane % 32, h = lane / 32, row_wave = wave % RW, column_wave = wave / RW % CW, key_wave = wave / (RW * CW);
     const int64_t rows = p.tokens * p.share;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
-    const uint32_t key_at = Wave::key_address(0, n, h), value_at = Wave::value_address(lane, n, h);
+    const uint32_t key_at = Wave::key_address(0, n, h), value_at = Wave::value_address(lane, n, h) ^ (uint32_t)(column_wave * VT * 32 * sizeof(T));
     if (tid < KT / 32) odd_keys[0][tid] = odd_keys[1][tid] = 0;
 
     // Piece `lane` of transfer j of a wave, whose keys are one behind the other: where it is, counted from the transfer's first key
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             f32x16 (&s)[RB] = scores[u];
             __builtin_amdgcn_s_setprio(1);
             if constexpr (AHEAD) {
-                tree_read_values<T, D>(lds_v, held);
+                tree_read_values<T, D, VT>(lds_v, held);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (u > 0) score(u - 1);
@@ -484,7 +488,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
                 for (int r = 0; r < 16; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from));
             }
             __builtin_amdgcn_s_setprio(1);
-            if constexpr (AHEAD) tree_values<T, D>(held, s, out, sum);
+            if constexpr (AHEAD) tree_values<T, VT>(held, s, out, sum);
             else Wave::values(lds_v, s, out, sum);
             __builtin_amdgcn_s_setprio(0);
             if (!odd) continue;
@@ -502,7 +506,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
                     for (int c = 0; c < VT; ++c)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const float v = (float)value[32 * c + 8 * (r / 4) + 4 * h + r % 4];
+                            const float v = (float)value[32 * (column_wave * VT + c) + 8 * (r / 4) + 4 * h + r % 4];
                             if (!(__builtin_fabsf(v) < __builtin_inff())) out[i][c][r] += weight * v;
                         }
                 }
@@ -517,7 +521,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
         float* exchange = reinterpret_cast<float*>(lds);
         __shared__ float base_sum[KW][RW][RB][2][32];
         __syncthreads();   // nobody reads the stages any more
-        if (h == 0) {
+        if (h == 0 && column_wave == 0) {   // (the others have the same)
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
                 base_sum[key_wave][row_wave][i][0][n] = base[i];
@@ -540,7 +544,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
         }
 #pragma unroll
         for (int step = KW / 2; step >= 1; step /= 2) {
-            const int slot = (key_wave % step) * RW + row_wave;
+            const int slot = ((key_wave % step) * CW + column_wave) * RW + row_wave;
             if (key_wave >= step && key_wave < 2 * step) {
 #pragma unroll
                 for (int i = 0; i < RB; ++i)
@@ -568,7 +572,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
         if (key_wave || row >= rows) continue;
         if (parts > 1) {
             const int64_t at = (int64_t)blockIdx.x * p.block_rows + (row - block * ROWS);
-            if (h == 0) {
+            if (h == 0 && column_wave == 0) {
                 p.partial_ml[2 * at] = base[i];
                 p.partial_ml[2 * at + 1] = sum[i];
             }
@@ -576,7 +580,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
             for (int c = 0; c < VT; ++c)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(p.partial_o + at * D + 32 * c + 8 * g + 4 * h) =
+                    *reinterpret_cast<f32x4*>(p.partial_o + at * D + 32 * (column_wave * VT + c) + 8 * g + 4 * h) =
                         f32x4{out[i][c][4 * g], out[i][c][4 * g + 1], out[i][c][4 * g + 2], out[i][c][4 * g + 3]};
             continue;
         }
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void tree_attention_kernel(
                 float o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = out[i][c][4 * g + e] * factor;
-                store_values(to + 32 * c + 8 * g + 4 * h, o, 4);
+                store_values(to + 32 * (column_wave * VT + c) + 8 * g + 4 * h, o, 4);
             }
     }
 }
@@ -676,10 +680,10 @@ static TreeForm tree_form(int form, int bytes, bool f32) {
     // by 8 x 64 and 8 x 8 tokens behind 4096, 1 to 16 heads of 1 to 4 groups, and prompts of 512 to 4096 tokens
     const double rates[6][TREE_FORMS][2] = {{{0.65, 1.0}, {0.57, 0.57}, {1.12, 1.45}},   // 16 bits, heads of 64
                                             {{1.05, 1.75}, {0.82, 0.82}, {1.55, 2.2}},    // 128
-                                            {{2.1, 2.1}, {}, {3.2, 3.2}},                 // 256
+                                            {{1.8, 1.8}, {}, {2.6, 2.6}},                 // 256
                                             {{2.2, 3.0}, {1.6, 1.6}, {3.7, 5.0}},         // float32, 64
                                             {{3.9, 3.9}, {}, {6.7, 6.7}},
-                                            {{14.5, 14.5}, {}, {13.5, 13.5}}};
+                                            {{10.8, 10.8}, {}, {13.5, 13.5}}};
     const double(&rate)[2] = rates[(f32 ? 3 : 0) + (size == 64 ? 0 : size == 128 ? 1 : 2)][form];
     return {form == TREE_TALL ? 128 : 64, form == TREE_DEEP || bytes > 256 ? 256 : 512, rate[0], rate[1], form == TREE_DEEP ? 10.0 : 8.0};
 }
@@ -727,25 +731,28 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
     constexpr int BYTES = D * (int)sizeof(T);
     const int64_t rows = p.tokens * p.share, slices = p.batch * p.kv_heads;
     bool fits = true;
-    auto launch = [&](auto rb, auto rw, auto kw, auto sub, auto ns, auto per_simd) {
-        constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
+    auto launch = [&](auto rb, auto rw, auto cw, auto kw, auto sub, auto ns, auto per_simd) {
+        constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, CW = decltype(cw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
         constexpr int PER_SIMD = decltype(per_simd)::value;
         const int64_t grid = p.dealt ? p.dealt : p.row_blocks * slices;
         const bool many_parts = p.dealt > 16 * p.row_blocks * slices;
         const int64_t joins = p.dealt ? ceil_div(slices * rows, (int64_t)(many_parts ? 1 : 4)) : 0;
-        fits = grid_fits(grid, 64 * RW * KW) && grid_fits(joins, 256);
+        fits = grid_fits(grid, 64 * RW * CW * KW) && grid_fits(joins, 256);
         if (!fits) return;
-        const dim3 g((unsigned)grid), threads(64 * RW * KW);
-        if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
-        else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
+        const dim3 g((unsigned)grid), threads(64 * RW * CW * KW);
+        if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, CW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
+        else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, CW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
         if (!joins) return;
         if (many_parts) hipLaunchKernelGGL((tree_join_kernel<T, D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
         else hipLaunchKernelGGL((tree_join_kernel<T, D, 1>), dim3((unsigned)joins), dim3(256), 0, st, p);
     };
+    // Heads of 256: a wave with all of their columns has no room for its sums beside the queries (they move between two register files for every 32 keys), two with half of them each have it,
+    // and take the scores twice. us, 4 x 64 tokens behind 4096, 16 heads in 4 groups: bfloat16 128 -> 109, 128 rows a workgroup 214 -> 178, float32 939 -> 693; float32 heads of 128 are behind so.
     constexpr bool WIDE = BYTES > 256, WIDEST = BYTES > 512;
-    if (cut.form == TREE_PAIR) launch(Int<1>{}, Int<2>{}, Int<(WIDEST ? 1 : 2)>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<(WIDE ? 1 : 2)>{});
-    else if (cut.form == TREE_TALL) launch(Int<1>{}, Int<4>{}, Int<1>{}, Int<(WIDE ? 1 : 2)>{}, Int<2>{}, Int<(WIDE ? 1 : 2)>{});
-    else if constexpr (!WIDE) launch(Int<1>{}, Int<2>{}, Int<4>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
+    constexpr int CW = D == 256 ? 2 : 1, PER_SIMD = WIDE && (D != 256 || WIDEST) ? 1 : 2;
+    if (cut.form == TREE_PAIR) launch(Int<1>{}, Int<2>{}, Int<CW>{}, Int<(WIDEST ? 1 : 2)>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<PER_SIMD>{});
+    else if (cut.form == TREE_TALL) launch(Int<1>{}, Int<4>{}, Int<(WIDEST ? 1 : CW)>{}, Int<1>{}, Int<(WIDE ? 1 : 2)>{}, Int<2>{}, Int<PER_SIMD>{});
+    else if constexpr (!WIDE) launch(Int<1>{}, Int<2>{}, Int<1>{}, Int<4>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
     MI355X_REQUIRE(fits, "tree_attention: too large");
     return check_launch("tree_attention_kernel");
 }
