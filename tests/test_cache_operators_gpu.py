@@ -325,6 +325,25 @@ def test_attention_of_values_that_some_rows_do_not_see(dtype, d, bad):
         assert bool(torch.isfinite(o[0, i]).all()) == (not below[i, 3])
 
 
+@pytest.mark.parametrize("form", range(3))
+@pytest.mark.parametrize("dealt", [0, 40])
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 11])
+def test_attention_of_values_that_some_rows_do_not_see_by_every_kernel(form, dealt, dtype, d, page, tuning):
+    """Of a chain: what later tokens hold, in several columns and of both halves of a wave, behind and across the ends of stages."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    tokens, context = 150, 100
+    bad = {30: (0, float("inf")), 61: (d - 1, float("nan")), 62: (d // 2 + 5, float("-inf")), 149: (7, float("inf"))}
+
+    def change(kp, vp, table):
+        for n, (column, value) in bad.items():
+            vp[int(table[0, (context + n) // page]), :, (context + n) % page, column] = value
+    o = check_attention(1, tokens, 4, 2, d, page, context, dtype, change=change)
+    for n, (column, value) in bad.items():
+        assert torch.isfinite(o[0, :n, :, column]).all() and not torch.isfinite(o[0, n:, :, column]).any()
+
+
 @pytest.mark.parametrize("dtype", R.TYPES)
 def test_attention_of_a_padded_prompt(dtype):
     """The tokens behind a prompt's end hold anything: those before them do not see it."""
