@@ -1,4 +1,10 @@
 // DraftAcceptance: the largest of every row of logits, and the walk along each entry's tree of drafted tokens that follows them. The reference has no such node.
+//
+// Every row is looked at, also those that the walk does not come to: which they are is known only once the largest of the rows before are, and reading all at once is one pass over memory. A
+// row's largest is that of its parts' keys, in 64 bits: the value's order, then how far its place is from the row's end, so the first of equal ones wins in any order of the parts, and nothing
+// has to be cleared or added to by atomics. Values are compared as they are; nothing is rounded.
+// Bound by the bytes of the logits: 16 trees of 32 over 131072 in bfloat16 25.4 us, 5.3 TB/s, and 4.6 for the walk. 8 rows of 32000: 3.4 and 2.5 us, less than the host takes for
+// the call (11).
 #include "mixed.h"
 
 #include <algorithm>
@@ -113,7 +119,7 @@ static bool accept_fits(int64_t batch, int64_t tokens, int64_t vocabulary) {
     return batch >= 0 && tokens >= 1 && tokens <= ACCEPT_MOST && vocabulary >= 1 && vocabulary < (int64_t)1 << 31 && batch < (int64_t)1 << 31 && (double)batch * tokens * vocabulary < 0x1p45;
 }
 
-// Workgroups to a row: enough for all CUs several times, none with less than two vectors to a thread
+// Workgroups to a row: enough for all CUs several times, none with less than two vectors to a thread (16 bits).
 static int64_t accept_parts(int64_t rows, int64_t vocabulary) {
     const int forced = tuning().accept_parts;
     if (forced > 0) return std::min<int64_t>(forced, vocabulary);

@@ -202,6 +202,8 @@ extern "C" int mi355x_paged_cache_append(const void* K, const void* V, const voi
     p.tokens_per_wg = std::max(1, std::min(APPEND_TOKENS, ROTARY_LDS_ANGLES / std::max(p.rotated / 2, 1)));
     MI355X_REQUIRE(p.all < (int64_t)1 << 40 && p.per_axis < (int64_t)1 << 40 && (double)pages * page_size * kv_heads < 0x1p46 &&
                        grid_fits(ceil_div(p.all, (int64_t)p.tokens_per_wg), APPEND_THREADS), "paged_cache_append: too many tokens");
+    const uint64_t at_k = reinterpret_cast<uint64_t>(k_pages), at_v = reinterpret_cast<uint64_t>(v_pages), apart = (at_k < at_v ? at_v - at_k : at_k - at_v) / (type == MI355X_TYPE_FLOAT ? 4 : 2);
+    MI355X_REQUIRE(apart >= (uint64_t)(pages * kv_heads * page_size * size), "paged_cache_append: keys and values share pages");
     with_type(type, [&](auto t) { launch_append<decltype(t)>(p, interleaved != 0, static_cast<hipStream_t>(stream)); });
     return check_launch("paged_append_kernel");
 }

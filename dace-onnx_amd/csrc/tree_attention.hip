@@ -1,4 +1,24 @@
 // TreeAttention: O = softmax(c Q K^T) V over a cache in pages, whose last tokens are a chain or a tree. The reference has no such node.
+//
+// Rows: a slice (an entry's group of keys and values) has tokens * share of them, the heads that share it side by side, so a page is read once for all of them. A workgroup has 64 or 128
+// rows and walks the keys in stages of 64 or 128, from the end on: S^T = K Q^T and O^T = V^T P^T by products of 32 x 32 x 16, in which a lane has a row of its own, its maximum and sum
+// included; P goes from one product to the next in registers. Softmax runs in powers of two: a row has a base b, P = 2^(c' s - b) with c' = c log2 e, and sums and outputs take a factor where
+// the base moves. Scores, bases, sums and outputs are float32; with arrays of 16 bits P is rounded to their type for its product, by half a step of it, and its sum is taken of the rounded
+// values, so that weights add up to 1. float32 goes by three bfloat16 parts of each operand and the six products of them above 2^-24.
+// Whom a row sees: of the keys in front of the call all, of the call's its ancestors. Those fall, so a row walking back through the keys holds the next one and looks each up once in
+// a table of parents in LDS: a mask of 32 bits for 32 keys, taken where a block holds keys that some row does not see, nowhere else. Values that are not finite become 0 there, as 0 times
+// one is not a number, and the rows that do see them add them one by one.
+// Keys and values come from their pages into a ring of stages in LDS by transfers of 1 KB that no register waits for; a wave's transfer knows its page by a scalar load, and where pages are long
+// enough two to eight transfers share one. (Pages that are no whole number of transfers: through registers.)
+// Few rows and long caches leave CUs without work: the keys of all blocks are then cut into parts that are dealt to a fixed number of workgroups, by the lengths that the kernel finds, not by
+// the table's room, and a second kernel joins the parts' outputs by their bases and sums. What the first says about the cut stands in scratch memory. No atomics: results repeat.
+//
+// Bound, at heads of 128 in bfloat16 (a copy 5.1 TB/s, a product of 8192^3 1570 TFLOP/s):
+// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 68 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 57 us, 4.7 TB/s, the join 6 of them.
+// - a prompt of 4096 behind 4096, 16 heads in 4 groups: the products, 220 to 240 us, 860 to 940 TFLOP/s. The vector unit (a power, a fused multiply-add and a conversion for each score)
+//   is about as long as they are: scores of the next 32 keys are under way while these are taken, and the four waves of a CU's two workgroups fill what is left.
+// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 29 us where bytes are 9. A workgroup has five stages: 2.7 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6 for the parts' sums, and the
+//   second kernel 5.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -6,6 +26,7 @@
 namespace mi355x {
 
 constexpr int TREE_MOST = 1024;   // tokens of a tree
+constexpr float LOG2_E = 1.44269504088896340736f;
 
 struct TreeArgs {
     const void* q; const void* k_pages; const void* v_pages; const int32_t* table; const int32_t* lengths; const int32_t* parents; void* o;
@@ -16,7 +37,7 @@ struct TreeArgs {
     int heads, kv_heads, share;            // share = heads / kv_heads
     int block_rows;                        // of a workgroup's part
     int dealt;                             // workgroups that the parts of all blocks are dealt to; 0: one workgroup to a block
-    int order;                             // of those: see tree_block
+    int order;                             // with one workgroup to a block: see tree_block
     uint32_t page_magic; int page_shift;   // n / page_size for n below 2^31
     float scale_log2;
 };
@@ -144,7 +165,7 @@ __device__ __forceinline__ void run_to_lds(const void* base, const uint32_t* lan
                      "v"(lane_offset[1]), "s"(uniform) : "memory", "m0");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-                     "global_load_lds_dwordx4 %4, %5 offset:3072" ::"s"(to), "v"(lane_offset[0]), "v"(lane_offset[1]), "v"(lane_offset[2]), "v"(lane_offset[3]), "s"(uniform) : "memory", "m0");
+                     "global_load_lds_dwordx4 %4, %5 offset:%6" ::"s"(to), "v"(lane_offset[0]), "v"(lane_offset[1]), "v"(lane_offset[2]), "v"(lane_offset[3]), "s"(uniform), "n"(3 * 1024) : "memory", "m0");
 }
 
 // S^T of 32 keys and 32 rows, the keys' operands on their way from LDS all at once: one after the other each product waits for its own.
@@ -778,7 +799,7 @@ extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const v
     MI355X_REQUIRE(is_mixed_type(type), "tree_attention: element type %d", type);
     MI355X_REQUIRE(size == 64 || size == 128 || size == 256, "tree_attention: head size %lld (64, 128 and 256 are supported)", (long long)size);
     MI355X_REQUIRE(heads >= 0 && kv_heads >= 1 && heads % kv_heads == 0, "tree_attention: %lld heads share keys and values in %lld groups", (long long)heads, (long long)kv_heads);
-    MI355X_REQUIRE(scale > 0.0f && scale < __builtin_inff(), "tree_attention: scale %g (a positive number is needed)", (double)scale);
+    MI355X_REQUIRE(scale > 0.0f && scale * LOG2_E < __builtin_inff(), "tree_attention: scale %g (a positive number is needed)", (double)scale);
     MI355X_REQUIRE(!parents || tokens <= TREE_MOST, "tree_attention: a tree of %lld tokens (%d at most)", (long long)tokens, TREE_MOST);
     MI355X_REQUIRE(tree_fits(batch, tokens, heads, kv_heads, size, page_size, columns) && pages >= 1 && pages < (int64_t)1 << 31 &&
                        (double)pages * page_size * kv_heads < 0x1p46, "tree_attention: negative, empty or too large an extent");
@@ -800,7 +821,7 @@ extern "C" int mi355x_tree_attention(const void* Q, const void* k_pages, const v
     p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.share = (int)(heads / kv_heads);
     while (((int64_t)1 << p.page_shift) < page_size) ++p.page_shift;
     p.page_magic = (uint32_t)((((uint64_t)1 << (31 + p.page_shift)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
-    p.scale_log2 = scale * 1.44269504088896340736f;
+    p.scale_log2 = scale * LOG2_E;
     int status = MI355X_OK;
     with_type(type, [&](auto t) {
         using T = decltype(t);

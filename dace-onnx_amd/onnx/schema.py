@@ -194,7 +194,7 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "becomes number lengths[b] + i of the entry, which is row (number % page) of page table[b, number / page] (table [B, columns]); with `order` [B, N] "
                "it is token order[b, j] that becomes number lengths[b] + j, and where order[b, j] is none of 0 to S - 1 nothing is written. Nor is anything where the "
                "table has no column for a number, or a value that is no page. Numbers that two tokens of a call would write to one row of one page are the "
-               "caller's error: it holds either. With `frequencies` keys are turned on the way, and Q [B, S, H, D] to Q_out with them, as RotaryPositions does, by "
+               "caller's error: it holds either; keys and values have pages of their own. With `frequencies` keys are turned on the way, and Q [B, S, H, D] to Q_out with them, as RotaryPositions does, by "
                "`positions` [axes, B, S] or, without, the token's number in the entry; Q is not taken with `order`. A length below 0 counts as 0.",
                updates={"k_pages_out": "k_pages", "v_pages_out": "v_pages"}),
     ONNXSchema("TreeAttention", 1,
@@ -206,7 +206,8 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "table as there, H / G heads share keys and values. Token i sees the lengths[b] before the call, itself and its ancestors: parents[b, i] is the token "
                "whose child it is, a lower number, anything else makes it a child of what is before the call. Without `parents` it sees the tokens up to itself. A table "
                "value that is no page counts as the nearest one, keys for which the table has no column do not exist, a row without keys is 0. `scale` is 1 / sqrt(D) if "
-               "it is left out. In float16 and bfloat16 the probabilities are rounded to that type for their product with the values."),
+               "it is left out. In float16 and bfloat16 the probabilities are rounded to that type for their product with the values. What a row does not see does not reach "
+               "it, whatever it holds; an infinite value that it sees makes it infinite or not a number, in float32 not a number, as an infinite query or key does."),
     ONNXSchema("DraftAcceptance", 1,
                [ONNXParameter("logits", "T"), ONNXParameter("tokens", "I32"), ONNXParameter("parents", "I32", _O)],
                [ONNXParameter("path", "I32"), ONNXParameter("count", "I32"), ONNXParameter("next", "I32")], [],

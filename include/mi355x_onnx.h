@@ -518,8 +518,8 @@ int mi355x_differential_attention(const void* Q, const void* K, const void* V, c
  * holds none of 0 to tokens - 1, where the number has no column, or its table value is none of 0 to pages - 1; a length below 0
  * counts as 0. K is turned on the way, and Q [batch, tokens, heads, size] to Q_out, as mi355x_rotary_positions does, by positions
  * [axes, batch, tokens] or, if that is NULL, by the number itself (axes is 1 then; a taken token's is the number that it becomes).
- * rotated may be 0. Q (with heads of 0) and order may be NULL, not both given. The pages are apart from each other and from
- * everything else, as are the rows that a call writes; Q_out may be Q. */
+ * rotated may be 0. Q (with heads of 0) and order may be NULL, not both given. The pages are apart from each other (this is checked) and
+ * from everything else, as are the rows that a call writes; Q_out may be Q. */
 int mi355x_paged_cache_append(const void* K, const void* V, const void* Q, void* k_pages, void* v_pages, void* Q_out,
                               const int32_t* table, const int32_t* lengths, const float* frequencies,
                               const void* positions, const int32_t* order, int64_t batch, int64_t tokens, int64_t heads,
@@ -536,7 +536,8 @@ int mi355x_paged_cache_append(const void* K, const void* V, const void* Q, void*
  * 0 with NULL: none needed), and belongs to the call until it is done.
  * With arrays of 16 bits the probabilities are rounded to `type` for their product with V, and their sum is that of the rounded
  * ones; scores, maxima, sums and results stay in float32. In float32 an infinite query, key or value that a row sees makes it not a
- * number, and values below 2^-110 lose digits. What a row does not see does not reach it, whatever it holds. */
+ * number, and values below 2^-110 lose digits; with arrays of 16 bits an infinite value that it sees makes it infinite or not a
+ * number. What a row does not see does not reach it, whatever it holds. */
 int64_t mi355x_tree_attention_scratch(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size,
                                       int64_t page_size, int64_t columns, int type);
 int mi355x_tree_attention(const void* Q, const void* k_pages, const void* v_pages, const int32_t* table,

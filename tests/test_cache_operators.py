@@ -253,3 +253,14 @@ def test_the_small_transformer_has_clear_largest_logits():
     for prompt in ([5, 17, 3, 200, 44, 9, 101], [77, 8]):
         _, least = C.greedy(weights, prompt, 24)
         assert least > 2e-3
+
+
+@pytest.mark.parametrize("apart", [0, 16, 4 * 9 * 2 * 5 * 8 - 16])
+def test_keys_and_values_in_the_same_pages(apart):
+    first = (ctypes.c_int64 * 1)(4)
+    for k, v in ((1 << 20, (1 << 20) + apart), ((1 << 20) + apart, 1 << 20)):
+        assert "share pages" in _refused("mi355x_paged_cache_append", *{**APPEND, "kp": k, "vp": v, "sections": first}.values(), None)
+
+
+def test_a_scale_that_leaves_float32():
+    assert "scale" in _refused("mi355x_tree_attention", *{**ATTENTION, "scale": 3e38}.values(), None)

@@ -597,6 +597,21 @@ def test_another_cache_in_a_recorded_graph_and_tensors_that_cannot_be_updated():
                 m(k, v, bad, vp, table, lengths)
 
 
+def test_keys_and_values_side_by_side_and_in_one_array():
+    """Pages of one allocation, one half behind the other; the same half twice is refused, on the first call and on those by the plan."""
+    k, v, table, lengths = normal(1, 2, 3, 2, 64), normal(2, 2, 3, 2, 64), whole([[4, 1], [0, 2]]), whole([3, 0])
+    cache = normal(3, 2, 5, 2, 4, 64)
+    m = donnx.ONNXModel("m", _append_proto(k, cache[0], table))
+    for turn in range(3):
+        ek, ev, *_ = C.append(k, v, cache[0].clone(), cache[1].clone(), table, lengths)
+        m(k, v, cache[0], cache[1], table, lengths)
+        assert torch.equal(cache[0].double(), ek) and torch.equal(cache[1].double(), ev)
+        before = cache.clone()
+        with pytest.raises(Exception, match="share pages"):
+            m(k, v, cache[0], cache[0], table, lengths)
+        assert torch.equal(cache, before)
+
+
 def _append_proto(k, kp, table):
     from dace_onnx_amd.onnx.proto import helper
     info = lambda n, t, s: helper.make_tensor_value_info(n, t, list(s))   # noqa: E731
