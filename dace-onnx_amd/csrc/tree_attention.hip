@@ -15,8 +15,10 @@
 //
 // Bound, at heads of 128 in bfloat16 (a copy 5.1 TB/s, a product of 8192^3 1570 TFLOP/s):
 // - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 68 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 57 us, 4.7 TB/s, the join 6 of them.
-// - a prompt of 4096 behind 4096, 16 heads in 4 groups: the products, 220 to 240 us, 860 to 940 TFLOP/s. The vector unit (a power, a fused multiply-add and a conversion for each score)
-//   is about as long as they are: scores of the next 32 keys are under way while these are taken, and the four waves of a CU's two workgroups fill what is left.
+// - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 228 us, 900 to 960 TFLOP/s. Of a wave's cycles 38 % issue, 38 % wait for a unit, 24 % for LDS and barriers;
+//   the matrix unit is busy for 45 %. The vector instructions of 32 keys (a power, a multiply-add, half a conversion and half a product of pairs for each score) take about as long as
+//   their products, and the products of a wave's own are where they hide best (below). With 256 rows to a workgroup, one to a CU, calls whose blocks are all as long take 5 % less, but causal
+//   ones 8 % more: no short block stands next to a long one.
 // - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 29 us where bytes are 9. A workgroup has five stages: 2.7 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6 for the parts' sums, and the
 //   second kernel 5.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
 #include "attention_tile.h"
@@ -168,22 +170,26 @@ __device__ __forceinline__ void run_to_lds(const void* base, const uint32_t* lan
                      "global_load_lds_dwordx4 %4, %5 offset:%6" ::"s"(to), "v"(lane_offset[0]), "v"(lane_offset[1]), "v"(lane_offset[2]), "v"(lane_offset[3]), "s"(uniform), "n"(3 * 1024) : "memory", "m0");
 }
 
-// S^T of 32 keys and 32 rows, the keys' operands on their way from LDS all at once: one after the other each product waits for its own.
-template <class T, int D, int RB>
-__device__ __forceinline__ void tree_scores(uint32_t lds_k, const Operand<T> (&q)[RB][D / 16], f32x16 (&acc)[RB]) {
-    constexpr int BATCH = D / 16 < 8 ? D / 16 : 8;
+template <class T, int D, int BATCH>
+__device__ __forceinline__ void tree_read_keys(uint32_t lds_k, int s0, typename Values<T, 8>::vec (&k)[BATCH]) {
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) k[s] = AttentionWave<T, D, D>::template read<typename Values<T, 8>::vec>(lds_k ^ (32 * (s0 + s)), 0);
+}
+
+// S^T of 32 keys and 32 rows; between(s): what else goes on behind product s
+template <class T, int D, int RB, int BATCH, class F>
+__device__ __forceinline__ void tree_scores(uint32_t lds_k, typename Values<T, 8>::vec (&k)[BATCH], const Operand<T> (&q)[RB][D / 16], f32x16 (&acc)[RB], F&& between) {
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f32x16{};
 #pragma unroll
     for (int s0 = 0; s0 < D / 16; s0 += BATCH) {
-        typename Values<T, 8>::vec k[BATCH];
+        if (s0) tree_read_keys<T, D, BATCH>(lds_k, s0, k);
 #pragma unroll
-        for (int s = 0; s < BATCH; ++s) k[s] = AttentionWave<T, D, D>::template read<typename Values<T, 8>::vec>(lds_k ^ (32 * (s0 + s)), 0);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s)
+        for (int s = 0; s < BATCH; ++s) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) Operand<T>::product({{k[s]}}, q[b][s0 + s], acc[b]);
+            between(s0 + s);
+        }
     }
 }
 
@@ -204,23 +210,31 @@ __device__ __forceinline__ void tree_read_values(uint32_t lds_v, typename Values
         }
 }
 
-template <class T, int VT, int RB>
-__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * VT], const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB]) {
+// between(n): behind product n of 2 VT
+template <class T, int VT, int RB, class F>
+__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * VT], const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB], F&& between) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         Operand<T> pr[RB];
+        T x[RB][8];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            T x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (T)prob[b][8 * t + e];
-            pr[b].set(x);
-            pr[b].add_to(sum[b], x);
+            for (int e = 0; e < 8; ++e) x[b][e] = (T)prob[b][8 * t + e];
+            pr[b].set(x[b]);
         }
 #pragma unroll
-        for (int c = 0; c < VT; ++c)
+        for (int c = 0; c < VT; ++c) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) Operand<T>::product({{v[t * VT + c]}}, pr[b], out[b][c]);
+            if (c == 0)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    pr[b].add_to(sum[b], x[b]);
+                    asm volatile("" : "+v"(sum[b]));   // (taken here, not behind all products)
+                }
+            between(t * VT + c);
+        }
     }
 }
 
@@ -431,31 +445,46 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
             odd = odd_keys[turn % 2];
         }
         if (stage * KT + key_wave * SUB * 32 >= wave_end) continue;   // (the same for the wave)
-        // Scores of the next 32 keys are on the matrix unit while the vector unit is at the probabilities of these.
+        // The scores of the next 32 keys are taken between the powers of these, their maxima between the products with the values of these.
         f32x16 scores[SUB][RB];
         const uint32_t keys0 = lds0 + (uint32_t)(buffer * STAGE + key_wave * SUB * 32 * Tile::ROW);
-        auto score = [&](int u) __attribute__((always_inline)) {
+        constexpr int QP = Wave::QP, BATCH = QP < 8 ? QP : 8;
+        typename Values<T, 8>::vec kh[AHEAD ? BATCH : 1];
+        auto key_place = [&](int u) __attribute__((always_inline)) {
             uint32_t lds_k = keys0 + (uint32_t)(u * 32 * Tile::ROW) + key_at;
             asm volatile("" : "+v"(lds_k));   // (nothing made of it is kept from one pass to the next)
-            if constexpr (AHEAD) tree_scores<T, D>(lds_k, q, scores[u]);
-            else Wave::scores(lds_k, q, scores[u]);
+            return lds_k;
         };
-        __builtin_amdgcn_s_setprio(1);
-        score(SUB - 1);
+        if constexpr (AHEAD) {
+            const uint32_t at = key_place(SUB - 1);
+            tree_read_keys<T, D, BATCH>(at, 0, kh);
+            __builtin_amdgcn_sched_barrier(0);
+            tree_scores<T, D, RB, BATCH>(at, kh, q, scores[SUB - 1], [](int) {});
+        } else Wave::scores(key_place(SUB - 1), q, scores[SUB - 1]);
+        float largest[RB];   // of the lane's scores of 32 keys
+        auto look = [&](int u, int r0, int r1) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i)
+#pragma unroll
+                for (int r = r0; r < r1; ++r) largest[i] = r ? fmaxf(largest[i], scores[u][i][r]) : scores[u][i][0];
+        };
+        look(SUB - 1, 0, 16);
 #pragma unroll
         for (int u = SUB - 1; u >= 0; --u) {
             const int local = (key_wave * SUB + u) * 32, key0 = stage * KT + local;
             uint32_t lds_v = keys0 + (uint32_t)(u * 32 * Tile::ROW) + HALF + value_at;
             asm volatile("" : "+v"(lds_v));
+            uint32_t next_k = 0;
             typename Values<T, 8>::vec held[AHEAD ? 2 * VT : 1];
             f32x16 (&s)[RB] = scores[u];
-            __builtin_amdgcn_s_setprio(1);
             if constexpr (AHEAD) {
+                if (u > 0) {
+                    next_k = key_place(u - 1);
+                    tree_read_keys<T, D, BATCH>(next_k, 0, kh);
+                }
                 tree_read_values<T, D, VT>(lds_v, held);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            if (u > 0) score(u - 1);
-            __builtin_amdgcn_s_setprio(0);
+            } else if (u > 0) Wave::scores(key_place(u - 1), q, scores[u - 1]);
             uint32_t seen[RB];   // of the 32 keys
 #pragma unroll
             for (int i = 0; i < RB; ++i) seen[i] = ~0u;
@@ -478,6 +507,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                     for (int r = 0; r < 16; ++r)
                         if (!(mine >> (8 * (r / 4) + r % 4) & 1)) s[i][r] = -__builtin_inff();
                 }
+                look(u, 0, 16);
             }
             // The base of a row's powers is the largest score so far, or up to 8 below it: P is at most 2^8, and outputs are rarely scaled. float16 has no
             // values below 2^-25 and few digits below 2^-14, where many keys of little weight may outweigh the rest: 10 to 15 below the largest score.
@@ -486,10 +516,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
             bool far = false;
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                m[i] = s[i][0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) m[i] = fmaxf(m[i], s[i][r]);
-                m[i] = across_halves(m[i], [](float x, float y) { return fmaxf(x, y); }) * p.scale_log2;
+                m[i] = across_halves(largest[i], [](float x, float y) { return fmaxf(x, y); }) * p.scale_log2;
                 far |= m[i] > base[i] + MOST;
             }
             if (__any(far)) {
@@ -502,16 +529,45 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                     for (int c = 0; c < VT; ++c) out[i][c] *= factor;
                 }
             }
+            float from[RB];
 #pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                const float from = base[i] == -__builtin_inff() ? 0.0f : base[i];   // no key so far: exp2(-inf)
+            for (int i = 0; i < RB; ++i) from[i] = base[i] == -__builtin_inff() ? 0.0f : base[i];   // no key so far: exp2(-inf)
+            auto powers = [&](int r0, int r1) __attribute__((always_inline)) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from));
+                for (int i = 0; i < RB; ++i)
+#pragma unroll
+                    for (int r = r0; r < r1; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from[i]));
+            };
+            if constexpr (AHEAD) {
+                // Vector instructions in between of the products, a few to each: a wave's own hide there almost whole (two powers with their multiply-adds behind a product of 32 cycles
+                // cost nothing, seven multiply-adds 7 %), those of the SIMD's other wave do not (as many multiply-adds 40 %).
+                constexpr int EACH = 16 / QP, LATER = 8 / VT;   // powers to a product, the maxima as many as LATER
+                __builtin_amdgcn_sched_barrier(0);
+                if (u > 0) {
+                    tree_scores<T, D, RB, BATCH>(next_k, kh, q, scores[u - 1], [&](int n) __attribute__((always_inline)) {
+                        powers(n * EACH, (n + 1) * EACH);
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                    tree_values<T, VT>(held, s, out, sum, [&](int n) __attribute__((always_inline)) {
+                        look(u - 1, n * LATER, (n + 1) * LATER);
+#pragma unroll
+                        for (int i = 0; i < RB; ++i) asm volatile("" : "+v"(largest[i]));   // (taken here, not where it is needed)
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                } else {
+                    powers(0, 8);
+                    tree_values<T, VT>(held, s, out, sum, [&](int n) __attribute__((always_inline)) {
+                        if (n < VT) {
+                            powers(8 + n * LATER, 8 + (n + 1) * LATER);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    });
+                }
+            } else {
+                powers(0, 16);
+                Wave::values(lds_v, s, out, sum);
+                if (u > 0) look(u - 1, 0, 16);
             }
-            __builtin_amdgcn_s_setprio(1);
-            if constexpr (AHEAD) tree_values<T, VT>(held, s, out, sum);
-            else Wave::values(lds_v, s, out, sum);
-            __builtin_amdgcn_s_setprio(0);
             if (!odd) continue;
             for (uint32_t left = __builtin_amdgcn_readfirstlane(odd[local / 32]); left; left &= left - 1) {
                 const int key = __builtin_ctz(left), at = key0 + key, column = tree_column(p, at);
