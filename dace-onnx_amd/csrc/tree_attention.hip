@@ -14,13 +14,13 @@
 // the table's room, and a second kernel joins the parts' outputs by their bases and sums. What the first says about the cut stands in scratch memory. No atomics: results repeat.
 //
 // Bound, at heads of 128 in bfloat16 (a copy 5.1 TB/s, a product of 8192^3 1570 TFLOP/s):
-// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 68 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 57 us, 4.7 TB/s, the join 6 of them.
+// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 67 us, 5.3 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 55 us, 4.9 TB/s, the join 5 of them.
 // - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 228 us, 900 to 960 TFLOP/s. Of a wave's cycles 38 % issue, 38 % wait for a unit, 24 % for LDS and barriers;
 //   the matrix unit is busy for 45 %. The vector instructions of 32 keys (a power, a multiply-add, half a conversion and half a product of pairs for each score) take about as long as
 //   their products, and the products of a wave's own are where they hide best (below). With 256 rows to a workgroup, one to a CU, calls whose blocks are all as long take 5 % less, but causal
 //   ones 8 % more: no short block stands next to a long one.
-// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 29 us where bytes are 9. A workgroup has five stages: 2.7 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6 for the parts' sums, and the
-//   second kernel 5.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
+// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 28.5 us where bytes are 9. A workgroup has five stages: 1.9 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6 for the parts' sums, and the
+//   second kernel 4.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -61,6 +61,14 @@ __device__ __forceinline__ uint32_t wave_uint(uint32_t v, F&& f) {
     return f(f(row(0), row(16)), f(row(32), row(48)));
 }
 
+// v of a lane and those before it: by rows of sixteen lanes, then the rows' ends to the rows behind them
+__device__ __forceinline__ int wave_sums(int v) {
+    auto from = [&](auto control, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(control)::value, decltype(rows)::value, 0xf, false); };
+    from(Int<0x111>{}, Int<0xf>{}), from(Int<0x112>{}, Int<0xf>{}), from(Int<0x114>{}, Int<0xf>{}), from(Int<0x118>{}, Int<0xf>{});   // row_shr:1, 2, 4, 8
+    from(Int<0x142>{}, Int<0xa>{}), from(Int<0x143>{}, Int<0xc>{});                                                                   // row_bcast:15, 31
+    return v;
+}
+
 // The keys of every block of an entry, in stages of KT, cut into as many parts as it takes for none to have more than `most` stages, which is as few as leave enough workgroups for all
 // parts; an entry's `items` blocks count alike. Workgroups go by entry, block and part. A lane of each wave looks at entries lane, lane + 64, ...
 constexpr int DEAL_ENTRIES = 256;
@@ -93,9 +101,11 @@ struct TreeDeal {
             all += wave_uint(stages[i], [](uint32_t x, uint32_t y) { return x + y; });
             longest = std::max(longest, wave_uint(stages[i], [](uint32_t x, uint32_t y) { return x > y ? x : y; }));
         }
-        // (enough are all stages of a block: there are no more blocks than workgroups)
-        uint32_t low = (uint32_t)((all * items + p.dealt - 1) / p.dealt);
-        most = longest;
+        // Between what even parts without a remainder would take and where a part more for every block cannot be too many, both a little wide as they are taken in float32; the longest is
+        // always enough: there are no more blocks than workgroups.
+        const float work = (float)all * (float)items, spare = (float)(p.dealt - (int)(p.batch * items));
+        uint32_t low = std::max(1u, (uint32_t)(work / (float)p.dealt * (1.0f - 0x1p-20f)));
+        most = spare > 0.0f ? std::min(longest, (uint32_t)std::min(0x1p31f, work / spare * (1.0f + 0x1p-20f) + 1.0f)) : longest;
         while (low < most) {
             const uint32_t enough = most;
             most = low + (enough - low) / 2;
@@ -111,12 +121,7 @@ struct TreeDeal {
         for (int i = 0; i < EACH; ++i) {
             if (i * WAVE >= p.batch) break;
             const int mine = (int)parts(stages[i]);
-            int with = mine;
-#pragma unroll
-            for (int d = 1; d < WAVE; d *= 2) {
-                const int other = __shfl_up(with, d);
-                with += (int)(threadIdx.x % WAVE) >= d ? other : 0;
-            }
+            const int with = wave_sums(mine);
             const uint64_t beyond = __ballot((passed + with) * items > w);
             if (beyond) {
                 const int lane = __builtin_ctzll(beyond);
@@ -677,9 +682,9 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
 
 // The parts of a row joined: WAVES waves to a row share its parts, the lanes of each are the D values. A block of one part is done.
 template <class T, int D, int WAVES>
-__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs p) {
-    constexpr int PER_LANE = D / WAVE, ROWS = 4 / WAVES, BATCH = 8;
-    __shared__ float sums[4][D + 2];
+__global__ __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) void tree_join_kernel(TreeArgs p) {
+    constexpr int PER_LANE = D / WAVE, ROWS = WAVES < 4 ? 4 / WAVES : 1, BATCH = 8;
+    __shared__ float sums[ROWS * WAVES][D + 2];
     const int64_t rows = p.tokens * p.share;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), share = wave % WAVES;
     const int64_t at = (int64_t)blockIdx.x * ROWS + wave / WAVES;   // of a slice's row
@@ -812,15 +817,18 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
         constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, CW = decltype(cw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
         constexpr int PER_SIMD = decltype(per_simd)::value;
         const int64_t grid = p.dealt ? p.dealt : p.row_blocks * slices;
-        const bool many_parts = p.dealt > 16 * p.row_blocks * slices;
-        const int64_t joins = p.dealt ? ceil_div(slices * rows, (int64_t)(many_parts ? 1 : 4)) : 0;
-        fits = grid_fits(grid, 64 * RW * CW * KW) && grid_fits(joins, 256);
+        // A wave has eight parts of a row on their way at once: four and sixteen waves to a row of more. us by four / sixteen: 16 rows of 128 parts 5.8 / 5.0, 32 of 64 3.9 / 4.5.
+        const int64_t parts = p.dealt / (p.row_blocks * slices);
+        const int join_waves = parts > 64 ? 16 : parts > 16 ? 4 : 1;
+        const int64_t joins = p.dealt ? join_waves > 1 ? slices * rows : ceil_div(slices * rows, (int64_t)4) : 0;
+        fits = grid_fits(grid, 64 * RW * CW * KW) && grid_fits(joins, 1024);
         if (!fits) return;
         const dim3 g((unsigned)grid), threads(64 * RW * CW * KW);
         if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, CW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
         else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, CW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
         if (!joins) return;
-        if (many_parts) hipLaunchKernelGGL((tree_join_kernel<T, D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
+        if (join_waves == 16) hipLaunchKernelGGL((tree_join_kernel<T, D, 16>), dim3((unsigned)joins), dim3(1024), 0, st, p);
+        else if (join_waves == 4) hipLaunchKernelGGL((tree_join_kernel<T, D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
         else hipLaunchKernelGGL((tree_join_kernel<T, D, 1>), dim3((unsigned)joins), dim3(256), 0, st, p);
     };
     // Heads of 256: a wave with all of their columns has no room for its sums beside the queries (they move between two register files for every 32 keys), two with half of them each have it,
