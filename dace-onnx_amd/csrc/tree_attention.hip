@@ -14,13 +14,13 @@
 // the table's room, and a second kernel joins the parts' outputs by their bases and sums. What the first says about the cut stands in scratch memory. No atomics: results repeat.
 //
 // Bound, at heads of 128 in bfloat16 (a copy 5.1 TB/s, a product of 8192^3 1570 TFLOP/s):
-// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 67 us, 5.3 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 55 us, 4.9 TB/s, the join 5 of them.
-// - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 228 us, 900 to 960 TFLOP/s. Of a wave's cycles 38 % issue, 38 % wait for a unit, 24 % for LDS and barriers;
-//   the matrix unit is busy for 45 %. The vector instructions of 32 keys (a power, a multiply-add, half a conversion and half a product of pairs for each score) take about as long as
-//   their products, and the products of a wave's own are where they hide best (below). With 256 rows to a workgroup, one to a CU, calls whose blocks are all as long take 5 % less, but causal
-//   ones 8 % more: no short block stands next to a long one.
-// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 28.5 us where bytes are 9. A workgroup has five stages: 1.9 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6 for the parts' sums, and the
-//   second kernel 4.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
+// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 69 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 55 us, 4.9 TB/s, the join 5 of them.
+// - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 228 us, 900 to 960 TFLOP/s. Of a wave's cycles 42 % issue, 34 % wait for a unit, 25 % for LDS and barriers;
+//   the matrix unit is busy for 48 % of the time in which its CU has work, which is 87 %: the longest block ends last, the second half of it with its CU to itself. The vector instructions of 32
+//   keys (a power, a multiply-add, half a conversion and half a product of pairs for each score) take about as long as their products, and the products of a wave's own are where they hide
+//   best (below). With 256 rows to a workgroup, one to a CU, calls whose blocks are all as long take 5 % less, but causal ones 11 % more: no short block stands next to a long one.
+// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 28.5 us where bytes are 9. A workgroup has five stages: 1.9 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6
+//   for the parts' sums, and the second kernel 4.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -771,9 +771,10 @@ static TreeForm tree_form(int form, int bytes, bool f32) {
 }
 
 // How a call is cut: which form, and how many workgroups the parts of its blocks are dealt to (0: one to a block), by what the forms take if the longest of the entries fills its table and they do
-// by two thirds. Measured, us, at heads of 128 in 16 bits (PAIR / DEEP / TALL, one workgroup to a block; the best in parts): 16 x 1 token of up to 8192, 32 heads in 8 groups 146 / 118 / 185, 73;
-// 32 x 1 159 / 140 / 180, 128; 8 trees of 64 behind 4000 69 / 54 / 97, 55; 2 of 256 57 / 45 / 80, 51; 4 of 32 67 / 51 / 98, 29; a prompt of 512 17.4 / 17.5 / 22, 22; of 1024 28 / 39 / 35, 38; of 2048
-// 65 / 84 / 63, 92; 4096 behind 4096, 16 heads in 4 groups 259 / 292 / 241, 300.
+// by two thirds. Measured, us, at heads of 128 in 16 bits, 32 heads in 8 groups (PAIR / DEEP / TALL, one workgroup to a block; the same in parts): 16 x 1 token of up to 8192 143 / 118 / 170,
+// 71 / 80 / 89; 32 x 1 of 8000 158 / 141 / 169, 129 / 144 / 173; 8 trees of 64 behind up to 4000 65 / 55 / 90, 72 / 70 / 61; 2 of 256 58 / 44 / 81, 58 / 51 / 63; 4 of 32 62 / 49 / 89,
+// 28 / 28 / 27; a prompt of 512 14.5 / 14.3 / 18, 30 / 21 / 30; of 1024 23 / 32 / 30, 36 / 23 / 38; of 2048 55 / 75 / 54, the same in parts; 4096 behind up to 4096, 16 heads in 4 groups,
+// 177 / 209 / 167, 177. The rule's choices take 28 where 27 is least, and at most 0.3 more elsewhere.
 struct TreeCut { int form, block_rows, dealt; int64_t row_blocks; };
 static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, int64_t size, int type) {
     const bool f32 = type == MI355X_TYPE_FLOAT;
