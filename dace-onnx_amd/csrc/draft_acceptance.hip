@@ -3,8 +3,8 @@
 // Every row is looked at, also those that the walk does not come to: which they are is known only once the largest of the rows before are, and reading all at once is one pass over memory. A
 // row's largest is that of its parts' keys, in 64 bits: the value's order, then how far its place is from the row's end, so the first of equal ones wins in any order of the parts, and nothing
 // has to be cleared or added to by atomics. Values are compared as they are; nothing is rounded.
-// Bound by the bytes of the logits: 16 trees of 32 over 131072 in bfloat16 25.4 us, 5.3 TB/s, and 4.6 for the walk. 8 rows of 32000: 3.4 and 2.5 us, less than the host takes for
-// the call (11).
+// Bound by the bytes of the logits: 16 trees of 32 over 131072 in bfloat16 25 to 26 us, 5.3 TB/s, and 3.9 for the walk. 8 rows of 32000: 3.4 and 2.2 us, less than the host
+// takes for the call (10.3).
 #include "mixed.h"
 
 #include <algorithm>
@@ -35,7 +35,7 @@ __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
     return v;
 }
 
-// A part of a row to a workgroup. A thread keeps the largest of its vectors and which it was, the first of equal ones, and looks for the place in it at the end.
+// A part of a row to a workgroup. A thread keeps the vector that has the largest of its values, the first of equal ones, and looks for the place in it at the end.
 template <class T>
 __global__ __launch_bounds__(256) void accept_rows_kernel(AcceptArgs p) {
     constexpr int E = 16 / sizeof(T), AHEAD = 4;
@@ -54,25 +54,26 @@ __global__ __launch_bounds__(256) void accept_rows_kernel(AcceptArgs p) {
     const Vector* v = reinterpret_cast<const Vector*>(x + begin);
     uint32_t largest = 0;
     int64_t which = threadIdx.x;
+    Vector kept = {};
     for (int64_t i0 = threadIdx.x; i0 < vectors; i0 += 256 * AHEAD) {
         Vector held[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) held[u] = v[i0 + 256 * u < vectors ? i0 + 256 * u : i0];   // (again the first, where there is none: not larger than itself)
+        if (i0 == threadIdx.x) kept = held[0];   // (of NaN only: the first of them)
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             float m = (float)held[u][0];
 #pragma unroll
             for (int e = 1; e < E; ++e) m = fmaxf(m, (float)held[u][e]);
             const uint32_t order = order_of(m);
-            if (order > largest) largest = order, which = i0 + 256 * u;
+            if (order > largest) largest = order, which = i0 + 256 * u, kept = held[u];
         }
     }
     if ((int64_t)threadIdx.x < vectors) {
-        const Vector again = v[which];
         int place = 0;
 #pragma unroll
         for (int e = E - 1; e >= 0; --e)
-            if (order_of((float)again[e]) == largest) place = e;
+            if (order_of((float)kept[e]) == largest) place = e;
         best = larger(best, key(largest, begin + which * E + place));
     }
     best = wave_largest(best);
@@ -81,17 +82,47 @@ __global__ __launch_bounds__(256) void accept_rows_kernel(AcceptArgs p) {
     if (threadIdx.x == 0) p.best[blockIdx.x] = larger(larger(found[0], found[1]), larger(found[2], found[3]));
 }
 
-// A workgroup to an entry. A token's children stand behind it: each step looks at the tokens from its own 64 on.
+// What the logits of a row say
+__device__ __forceinline__ int32_t accept_said(const AcceptArgs& p, int64_t row) {
+    uint64_t best = 0;
+#pragma unroll 8
+    for (int c = 0; c < p.parts; ++c) best = larger(best, p.best[row * p.parts + c]);
+    return (int32_t)~(uint32_t)best;
+}
+
+// Trees of up to 64 tokens, a wave to an entry: a lane has a token, and a step looks at all of them without LDS: 2.2 us for one of 8 where the
+// kernel below takes 2.8; a call with 16 of 32 28.7 for 30.0 (the kept vectors of the first kernel included).
+__global__ __launch_bounds__(WAVE) void accept_walk_wave_kernel(AcceptArgs p) {
+    const int S = p.batch_tokens, i = threadIdx.x;
+    const int64_t row0 = (int64_t)blockIdx.x * S;
+    int32_t token = 0, parent = -1, said = 0, place = -1;
+    if (i < S) {
+        token = p.tokens[row0 + i];
+        parent = p.parents ? p.parents[row0 + i] : i - 1;
+        said = accept_said(p, row0 + i);
+    }
+    int node = 0, length = 0;
+    int32_t wanted;
+    while (true) {
+        place = i == length ? node : place;
+        ++length;
+        wanted = __builtin_amdgcn_readlane(said, node);
+        const uint64_t fits = __ballot(i < S && i > node && parent == node && token == wanted);
+        if (!fits) break;
+        node = __builtin_ctzll(fits);
+    }
+    if (i < S) p.path[row0 + i] = place;
+    if (i == 0) p.count[blockIdx.x] = length, p.next[blockIdx.x] = wanted;
+}
+
+// Larger ones, a workgroup to an entry. A token's children stand behind it: each step looks at the tokens from its own 64 on.
 __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptArgs p) {
     __shared__ int32_t said[ACCEPT_MOST], tokens[ACCEPT_MOST], parents[ACCEPT_MOST];
     const int S = p.batch_tokens;
     const int64_t row0 = (int64_t)blockIdx.x * S;
     for (int i = threadIdx.x; i < S; i += 256) {
         const int32_t token = p.tokens[row0 + i], parent = p.parents ? p.parents[row0 + i] : i - 1;
-        uint64_t best = 0;
-#pragma unroll 8
-        for (int c = 0; c < p.parts; ++c) best = larger(best, p.best[(row0 + i) * p.parts + c]);
-        said[i] = (int32_t)~(uint32_t)best;
+        said[i] = accept_said(p, row0 + i);
         tokens[i] = token;
         parents[i] = parent;
     }
@@ -149,6 +180,7 @@ extern "C" int mi355x_draft_acceptance(const void* logits, const int32_t* tokens
     AcceptArgs p = {logits, tokens, parents, path, count, next, static_cast<uint64_t*>(scratch), rows, vocabulary, ceil_div(vocabulary, parts), (int)token_count, (int)parts};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     with_type(type, [&](auto t) { hipLaunchKernelGGL((accept_rows_kernel<decltype(t)>), dim3((unsigned)(rows * parts)), dim3(256), 0, st, p); });
-    hipLaunchKernelGGL(accept_walk_kernel, dim3((unsigned)batch), dim3(256), 0, st, p);
+    if (token_count <= WAVE) hipLaunchKernelGGL(accept_walk_wave_kernel, dim3((unsigned)batch), dim3(WAVE), 0, st, p);
+    else hipLaunchKernelGGL(accept_walk_kernel, dim3((unsigned)batch), dim3(256), 0, st, p);
     return check_launch("draft_acceptance");
 }

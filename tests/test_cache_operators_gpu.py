@@ -445,6 +445,15 @@ def test_acceptance_in_any_number_of_parts(parts, dtype, vocabulary, tuning):
     check_acceptance(logits, drafts(3, logits, None, 0.8))
 
 
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("tokens", [32, 63, 64, 65, 128, 129])
+def test_acceptance_of_trees_that_a_wave_has_lanes_for_and_larger_ones(tokens, tree):
+    logits = normal(1, 3, tokens, 200, scale=2.0)
+    parents = trees(2, 3, tokens) if tree else None
+    for hit in (0.0, 0.9, 1.0):
+        check_acceptance(logits, drafts(3, logits, parents, hit), parents)
+
+
 @pytest.mark.parametrize("parts", [None, 5])
 @pytest.mark.parametrize("dtype", R.TYPES)
 def test_acceptance_of_equal_logits_and_of_none(dtype, parts, tuning):
