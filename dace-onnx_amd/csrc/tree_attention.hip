@@ -15,12 +15,13 @@
 //
 // Bound, at heads of 128 in bfloat16 (a copy 5.1 TB/s, a product of 8192^3 1570 TFLOP/s):
 // - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 69 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 55 us, 4.9 TB/s, the join 5 of them.
-// - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 228 us, 900 to 960 TFLOP/s. Of a wave's cycles 42 % issue, 34 % wait for a unit, 25 % for LDS and barriers;
+// - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 231 us, 890 to 960 TFLOP/s. Of a wave's cycles 42 % issue, 34 % wait for a unit, 25 % for LDS and barriers;
 //   the matrix unit is busy for 48 % of the time in which its CU has work, which is 87 %: the longest block ends last, the second half of it with its CU to itself. The vector instructions of 32
 //   keys (a power, a multiply-add, half a conversion and half a product of pairs for each score) take about as long as their products, and the products of a wave's own are where they hide
 //   best (below). With 256 rows to a workgroup, one to a CU, calls whose blocks are all as long take 5 % less, but causal ones 11 % more: no short block stands next to a long one.
-// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 28.5 us where bytes are 9. A workgroup has five stages: 1.9 us to find its part, 1.4 its page, 2 to the first stage, 10 for five, 1.6
-//   for the parts' sums, and the second kernel 4.5. A stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores, powers and values together (930).
+// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 26.6 us where bytes are 9. A workgroup has about six stages. By 64 rows and eight waves, 28.3: 1.9 us to find its part, 1.4 its page, 2
+//   to the first stage, 10 for five, 1.6 for the parts' sums, and the second kernel 4.5; a stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores,
+//   powers and values together (930). 128 rows read every key once.
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -755,26 +756,27 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) void tree_join_kernel
 // two waves are not enough to get the transfers out.)
 enum { TREE_PAIR, TREE_DEEP, TREE_TALL, TREE_FORMS };
 
-// us: of 64 keys where a workgroup has its CU alone, and where another shares it; of a round of workgroups besides
+// us: of 64 keys where a workgroup has its CU alone, and where another shares it; of a row of workgroups besides
 struct TreeForm { int rows, places; double alone, shared, start; };
 static TreeForm tree_form(int form, int bytes, bool f32) {
     const int size = bytes / (f32 ? 4 : 2);
-    // by 8 x 64 and 8 x 8 tokens behind 4096, 1 to 16 heads of 1 to 4 groups, and prompts of 512 to 4096 tokens
-    const double rates[6][TREE_FORMS][2] = {{{0.65, 1.0}, {0.57, 0.57}, {1.12, 1.45}},   // 16 bits, heads of 64
-                                            {{1.05, 1.75}, {0.82, 0.82}, {1.55, 2.2}},    // 128
-                                            {{1.8, 1.8}, {}, {2.6, 2.6}},                 // 256
-                                            {{2.2, 3.0}, {1.6, 1.6}, {3.7, 5.0}},         // float32, 64
-                                            {{3.9, 3.9}, {}, {6.7, 6.7}},
-                                            {{10.8, 10.8}, {}, {13.5, 13.5}}};
+    // as they fit the times of 70 calls in all forms: 1 to 128 entries of 1 to 4096 tokens behind 0 to 16000, 1 to 16 heads to a group
+    const double rates[6][TREE_FORMS][2] = {{{0.55, 0.8}, {0.4, 0.4}, {0.8, 2.0}},      // 16 bits, heads of 64
+                                            {{0.85, 1.4}, {0.7, 0.7}, {1.05, 1.65}},    // 128
+                                            {{1.45, 1.45}, {}, {1.95, 1.95}},           // 256
+                                            {{1.75, 1.95}, {1.45, 1.45}, {2.95, 4.0}},  // float32, 64
+                                            {{3.2, 3.2}, {}, {4.6, 4.6}},
+                                            {{7.6, 7.6}, {}, {8.2, 8.2}}};
     const double(&rate)[2] = rates[(f32 ? 3 : 0) + (size == 64 ? 0 : size == 128 ? 1 : 2)][form];
-    return {form == TREE_TALL ? 128 : 64, form == TREE_DEEP || bytes > 256 ? 256 : 512, rate[0], rate[1], form == TREE_DEEP ? 10.0 : 8.0};
+    return {form == TREE_TALL ? 128 : 64, form == TREE_DEEP || bytes > 256 ? 256 : 512, rate[0], rate[1], form == TREE_DEEP ? 9.0 : 8.0};
 }
 
 // How a call is cut: which form, and how many workgroups the parts of its blocks are dealt to (0: one to a block), by what the forms take if the longest of the entries fills its table and they do
 // by two thirds. Measured, us, at heads of 128 in 16 bits, 32 heads in 8 groups (PAIR / DEEP / TALL, one workgroup to a block; the same in parts): 16 x 1 token of up to 8192 143 / 118 / 170,
 // 71 / 80 / 89; 32 x 1 of 8000 158 / 141 / 169, 129 / 144 / 173; 8 trees of 64 behind up to 4000 65 / 55 / 90, 72 / 70 / 61; 2 of 256 58 / 44 / 81, 58 / 51 / 63; 4 of 32 62 / 49 / 89,
 // 28 / 28 / 27; a prompt of 512 14.5 / 14.3 / 18, 30 / 21 / 30; of 1024 23 / 32 / 30, 36 / 23 / 38; of 2048 55 / 75 / 54, the same in parts; 4096 behind up to 4096, 16 heads in 4 groups,
-// 177 / 209 / 167, 177. The rule's choices take 28 where 27 is least, and at most 0.3 more elsewhere.
+// 177 / 209 / 167, 177. Over 70 calls of all types and head sizes, measured in all
+// forms, the choices take 0.5 % more than the least on average, 8 % at most (2 chains of 512 behind up to 2048, 8 heads: 31.8, DEEP with one workgroup to a block 29.5).
 struct TreeCut { int form, block_rows, dealt; int64_t row_blocks; };
 static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, int64_t size, int type) {
     const bool f32 = type == MI355X_TYPE_FLOAT;
@@ -789,15 +791,16 @@ static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv
         const TreeForm f = tree_form(form, bytes, f32);
         const int64_t blocks = ceil_div(rows, (int64_t)f.rows), items = blocks * slices;
         const int block_rows = (int)std::min<int64_t>(f.rows, rows);
-        // what the bytes take goes by how many workgroups ask for them; with one to a block the longest entry's are the last
-        const double memory = least_memory * (form == TREE_PAIR ? 1.0 : form == TREE_DEEP ? 1.1 : 1.3), uneven = batch > 1 ? 1.25 : 1.0, rounds = (double)items / f.places;
+        // what the bytes take goes by how many workgroups ask for them, and a little by how often; with one to a block the longest entry's are the last
+        const double memory = least_memory * (form == TREE_DEEP ? 0.95 : 0.7) * (1 + 0.08 * (double)(blocks - 1)), uneven = batch > 1 ? 1.25 : 1.0, rounds = (double)items / f.places;
         const double whole = f.start + std::max(memory * uneven, items <= 256 ? most * f.alone : items <= f.places ? std::max(most * f.alone, full * mean * f.shared) :
                                                                   rounds * full * mean * (f.places > 256 ? f.shared : f.alone) + (rounds - 1) * f.start);
         if (wanted <= 0 && whole < least) least = whole, best = {form, block_rows, 0, blocks};
         const int64_t places = wanted > 0 ? wanted : form == TREE_TALL ? 256 : f.places;
         if (wanted == 0 || items > places || batch > DEAL_ENTRIES) continue;
-        const double used = std::min((double)places, (double)items * most);   // parts are whole stages, and no block has less than one: a quarter more than even ones
-        const double parts = 3 + f.start + std::max(memory, 1.25 * (double)items * full * most / used * (used > 256 ? f.shared : f.alone)) + 4.5 + used * block_rows * (double)size * 8 / 4.5e6;
+        // parts are whole stages, and no block has less than one; 5.5 for finding them and for the join, and 2e-6 for a value that goes through memory
+        const double used = std::min((double)places, (double)items * most);
+        const double parts = f.start + 5.5 + std::max(memory, 1.7 * (double)items * full * most / used * (used > 256 ? f.shared : f.alone)) + used * block_rows * (double)size * 2e-6;
         if (parts < least) least = parts, best = {form, block_rows, (int)places, blocks};
     }
     if (!best.row_blocks) {   // (forced, and not possible so)
