@@ -244,6 +244,47 @@ __device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v
     }
 }
 
+// Of float32: the products of 32 keys have sums of their own, which are added to the outputs. The matrix unit loses a little of every sum it adds to, towards zero: outputs of 10000 keys were
+// off by 4.7e-6 (2-norm) where all products went to one sum, of 60000 by 1.3e-5; so 2.4e-7 and 3.3e-7, for 1 to 5 % of the time. The sum of the probabilities keeps what its additions lose.
+template <int D, int VT, int RB>
+__device__ __forceinline__ void tree_values_f32(uint32_t lds_v, const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB], float (&lost)[RB]) {
+    constexpr int ROW = AttentionTile<float, D>::ROW;
+    Operand<float> pr[2][RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        float all = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = prob[b][8 * t + e];
+            pr[t][b].set(x);
+            pr[t][b].add_to(all, x);
+        }
+        const float before = sum[b], added = before + all - before;
+        sum[b] = before + all;
+        lost[b] += (before - (sum[b] - added)) + (all - added);
+    }
+    f32x16 acc[2][RB];
+    AttentionWave<float, D, D>::template each_operand<2 * VT, 6 * RB>(
+        [&](auto operand, auto& v) __attribute__((always_inline)) {
+            constexpr int c = decltype(operand)::value / 2, t = decltype(operand)::value % 2;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = AttentionWave<float, D, D>::template read<float>(lds_v ^ (16 * (8 * c ^ (e % 4) << 2 ^ 2 * (e / 4))), (16 * t + 8 * (e / 4) + e % 4) * ROW);
+        },
+        [&](auto operand, const Operand<float>& v) __attribute__((always_inline)) {
+            constexpr int c = decltype(operand)::value / 2, t = decltype(operand)::value % 2;
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                if constexpr (t == 0) acc[c % 2][b] = f32x16{};
+                Operand<float>::product(v, pr[t][b], acc[c % 2][b]);
+                if constexpr (t == 0 && c > 0) out[b][c - 1] += acc[(c + 1) % 2][b];   // (those of the columns before: nobody waits for these)
+                if constexpr (t == 1 && c == VT - 1) out[b][c] += acc[c % 2][b];
+            }
+        });
+}
+
 // Waves: RW blocks of 32 RB rows, CW shares of the value columns (each takes the scores for itself), KW shares of a stage's keys, 32 SUB each; NS stages. WHOLE: no transfer's keys lie in
 // two pages.
 template <class T, int D, int RB, int RW, int CW, int KW, int SUB, int NS, int PER_SIMD, bool WHOLE>
@@ -406,11 +447,11 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
         for (int s = 0; s < Wave::QP; ++s)
             if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(q[i][s].part[0]));
     f32x16 out[RB][VT];
-    float base[RB], sum[RB];   // of the scores times scale_log2; the lane's share of the sum
+    float base[RB], sum[RB], lost[RB];   // of the scores times scale_log2; the lane's share of the sum, and what it lost by rounding (float32)
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
         base[i] = -__builtin_inff();
-        sum[i] = 0.0f;
+        sum[i] = lost[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < VT; ++c) out[i][c] = f32x16{};
     }
@@ -531,6 +572,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                     const float now = fmaxf(base[i], m[i] - BELOW), factor = base[i] == now ? 1.0f : __builtin_amdgcn_exp2f(base[i] - now);
                     base[i] = now;
                     sum[i] *= factor;
+                    lost[i] *= factor;
 #pragma unroll
                     for (int c = 0; c < VT; ++c) out[i][c] *= factor;
                 }
@@ -571,7 +613,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                 }
             } else {
                 powers(0, 16);
-                Wave::values(lds_v, s, out, sum);
+                tree_values_f32<D, VT>(lds_v, s, out, sum, lost);
                 if (u > 0) look(u - 1, 0, 16);
             }
             if (!odd) continue;
@@ -597,7 +639,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
         }
     }
 #pragma unroll
-    for (int i = 0; i < RB; ++i) sum[i] = across_halves(sum[i], [](float x, float y) { return x + y; });
+    for (int i = 0; i < RB; ++i) sum[i] = across_halves(sum[i] + lost[i], [](float x, float y) { return x + y; });
 
     // ---- the shares of the keys meet, in pairs ------------------------------------------------------------
     if constexpr (KW > 1) {

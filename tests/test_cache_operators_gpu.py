@@ -685,3 +685,23 @@ def test_another_stream_and_recordings_of_the_caller():
         graph.replay()
         check(outputs)
         check(run())   # and the program's own calls in between
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 512)])
+def test_attention_in_float32_over_many_keys(form, dealt, d, tuning):
+    """Sums of 20000 products in float32, which one sum for all of them would not keep (7e-6). Each 32 keys have sums of their own, of twelve products that may lose half of 2^-23 of the sum so
+    far each, towards zero: 12 2^-24 / 2 = 3.6e-7 of weights that add up to one, and products left out 4e-8: 5e-7 on average. The additions of 625 such sums are off by 2^-24 of the sum so
+    far, at random: 2^-24 sqrt(625) / 3 = 5e-7 where it grows evenly, three times that for the farthest of 4096 outputs: 2e-6. Outputs of random values are 1 / sqrt(N) of their weights' sum of
+    magnitudes, as are what they lose at random: 1e-6 in 2-norm with scores off by 1.4e-7 of 8."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    table, pages = shuffled_table(1, 1, 1252)
+    q, kp, vp = normal(2, 1, 8, 4, d), normal(3, pages, 1, 16, d), normal(4, pages, 1, 16, d)
+    lengths = whole([20000])
+    m, inputs = C.attention_model(q, kp, vp, table, lengths, None)
+    o = m(*inputs).double()
+    expected, _ = C.attention(q, kp, vp, table, lengths, None, None)
+    assert (o - expected).norm() <= 1e-6 * expected.norm()
+    inputs = [torch.ones_like(t) if t is vp else t for t in inputs]   # weights add up to one: a loss of all products shows whole
+    o = m(*inputs).double()
+    assert (o - 1).abs().max() <= 2e-6 and abs(float((o - 1).mean())) <= 5e-7
