@@ -53,6 +53,18 @@ __device__ __forceinline__ TreeEntry tree_entry(const TreeArgs& p, int64_t b) {
     return {length, (int)std::min<int64_t>(length + p.tokens, p.capacity)};
 }
 
+// What a row whose weights add up to 0 is scaled by: one without keys is 0, one whose scores are all minus infinity is not a number. Without keys in front of the call a row has one if the token
+// that its line begins with has a column; a line falls, whatever parent(token) says.
+template <class Parent>
+__device__ __forceinline__ float tree_no_weights(const TreeArgs& p, const TreeEntry& entry, int token, Parent&& parent) {
+    int first = 0;
+    if (p.parents && entry.length == 0 && entry.total > 0) {
+        first = token;
+        for (int up = parent(first); up >= 0 && up < first; up = parent(first)) first = up;
+    }
+    return entry.length > 0 || first < entry.total ? __builtin_nanf("") : 0.0f;
+}
+
 // f over the lanes of a wave, four of a row at a time, then the rows; every lane gets it
 template <class F>
 __device__ __forceinline__ uint32_t wave_uint(uint32_t v, F&& f) {
@@ -709,7 +721,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                         f32x4{out[i][c][4 * g], out[i][c][4 * g + 1], out[i][c][4 * g + 2], out[i][c][4 * g + 3]};
             continue;
         }
-        const float factor = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];   // a row without keys: 0
+        const float factor = sum[i] == 0.0f ? tree_no_weights(p, entry, token[i], [&](int at) { return (int)parents[at]; }) : 1.0f / sum[i];
         T* to = static_cast<T*>(p.o) + ((b * p.tokens + token[i]) * p.heads + group * p.share + (int)(row % p.share)) * D;
 #pragma unroll
         for (int c = 0; c < VT; ++c)
@@ -788,8 +800,9 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) void tree_join_kernel
             for (int e = 0; e < PER_LANE; ++e) o[e] = fmaf(sums[wave + w][lane * PER_LANE + e], f, o[e]);
         }
     }
+    const float scale = sum == 0.0f ? tree_no_weights(p, tree_entry(p, b), (int)(row / p.share), [&](int at) { return p.parents[b * p.tokens + at]; }) : 1.0f / sum;
 #pragma unroll
-    for (int e = 0; e < PER_LANE; ++e) o[e] *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int e = 0; e < PER_LANE; ++e) o[e] *= scale;
     store_values(to, o, PER_LANE);
 }
 

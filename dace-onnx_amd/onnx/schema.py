@@ -205,7 +205,7 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "O = softmax(scale Q K^T) V for the S tokens of each entry that PagedCacheAppend has written behind its first lengths[b]; Q, O [B, S, H, D], pages and "
                "table as there, H / G heads share keys and values. Token i sees the lengths[b] before the call, itself and its ancestors: parents[b, i] is the token "
                "whose child it is, a lower number, anything else makes it a child of what is before the call. Without `parents` it sees the tokens up to itself. A table "
-               "value that is no page counts as the nearest one, keys for which the table has no column do not exist, a row without keys is 0. `scale` is 1 / sqrt(D) if "
+               "value that is no page counts as the nearest one, keys for which the table has no column do not exist, a row without keys is 0, one whose scores are all minus infinity not a number. `scale` is 1 / sqrt(D) if "
                "it is left out. In float16 and bfloat16 the probabilities are rounded to that type for their product with the values. What a row does not see does not reach "
                "it, whatever it holds; an infinite value that it sees makes it infinite or not a number, in float32 not a number, as an infinite query or key does."),
     ONNXSchema("DraftAcceptance", 1,

@@ -531,8 +531,8 @@ int mi355x_paged_cache_append(const void* K, const void* V, const void* Q, void*
  * their entries: token i sees the numbers before lengths[b], itself and its ancestors. parents [batch, tokens] holds each token's
  * parent, a lower place; anything else is none. Without (NULL) a token's parent is the one before it. size is 64, 128 or 256,
  * heads / kv_heads heads share keys and values, tokens is 1024 at most with parents. Table values that are no page count as the
- * nearest one, numbers without a column do not exist, a length below 0 counts as 0; a row without keys is 0. The pages stand at
- * 16-byte boundaries. `scratch` has room for scratch_floats floats, 16-byte aligned (mi355x_tree_attention_scratch says how many,
+ * nearest one, numbers without a column do not exist, a length below 0 counts as 0; a row without keys is 0, one whose scores are
+ * all minus infinity not a number. The pages stand at 16-byte boundaries. `scratch` has room for scratch_floats floats, 16-byte aligned (mi355x_tree_attention_scratch says how many,
  * 0 with NULL: none needed), and belongs to the call until it is done.
  * With arrays of 16 bits the probabilities are rounded to `type` for their product with V, and their sum is that of the rounded
  * ones; scores, maxima, sums and results stay in float32. In float32 an infinite query, key or value that a row sees makes it not a

@@ -705,3 +705,52 @@ def test_attention_in_float32_over_many_keys(form, dealt, d, tuning):
     inputs = [torch.ones_like(t) if t is vp else t for t in inputs]   # weights add up to one: a loss of all products shows whole
     o = m(*inputs).double()
     assert (o - 1).abs().max() <= 2e-6 and abs(float((o - 1).mean())) <= 5e-7
+
+
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 40), (2, 40)])
+@pytest.mark.parametrize("dtype", [F16, BF])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_rows_whose_scores_are_all_minus_infinity(form, dealt, dtype, tree, tuning):
+    """Softmax of such a row is not a number: 0 is the result of a row without keys alone. A key whose score is minus infinity next to others has no weight."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    tokens, heads, d, page, columns = 70, 4, 64, 8, 30
+    table, pages = shuffled_table(1, 4, columns)
+    q, kp, vp = normal(2, 4, tokens, heads, d, dtype=dtype), normal(3, pages, 2, page, d, dtype=dtype), normal(4, pages, 2, page, d, dtype=dtype)
+    kp[..., 0] = kp[..., 0].abs() + 0.25
+    kp[int(table[0, 0]), :, 0, 1] = float("-inf")   # a key in front of the first entry's call
+    q[..., 1] = q[..., 1].abs() + 0.25
+    none = torch.zeros(4, tokens, heads, dtype=torch.bool, device="cuda")
+    none[0, 5, 1] = none[0, 69, 3] = none[1, 0, 0] = none[1, 40, 2] = none[2, 3, 3] = none[3, 1, 1] = True
+    q[..., 0] = torch.where(none, float("-inf"), q[..., 0].abs())
+    parents = trees(5, 4, tokens) if tree else None
+    capacity = columns * page
+    lengths = whole([100, 0, 17, capacity])   # rows of the last see keys, but not their own
+    finite = q.clone()
+    finite[..., 0] = torch.where(none, 0.0, q[..., 0])
+    expected, size = C.attention(finite, kp, vp, table, lengths, parents)
+    bound = attention_bound(finite, torch.nan_to_num(kp, neginf=0.0), capacity, size, expected, d ** -0.5)
+    m, inputs = C.attention_model(q, kp, vp, table, lengths, parents)
+    o = m(*inputs)
+    assert torch.isnan(o[none]).all()
+    within(o[~none], expected[~none], bound[~none])
+    # no column, and no key: a row of minus infinity among them as well
+    m, inputs = C.attention_model(q, kp, vp, table[:, :0].contiguous(), lengths, parents)
+    assert (m(*inputs) == 0).all()
+
+
+@pytest.mark.parametrize("form, dealt", [(0, 0), (2, 0), (0, 40)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_empty_entries_that_the_table_has_little_room_for(form, dealt, tree, tuning):
+    """No key before the call and a table of one page: a token whose line begins behind it sees nothing, the others of it what the page has."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    tokens, d, page = 9, 64, 4
+    q, kp, vp = normal(2, 1, tokens, 2, d, dtype=BF), normal(3, 3, 1, page, d, dtype=BF).abs(), normal(4, 3, 1, page, d, dtype=BF)
+    q[0, :, 1, 0] = float("-inf")
+    kp[..., 0] += 0.25
+    parents = whole([[-1, 0, 1, -1, 2, -1, 5, 3, -1]]) if tree else None
+    m, inputs = C.attention_model(q, kp, vp, whole([[2]]), whole([0]), parents)
+    o = m(*inputs)
+    sees = [True] * 5 + [False, False, True, False] if tree else [True] * tokens
+    for i in range(tokens):
+        assert torch.isnan(o[0, i, 1]).all() if sees[i] else (o[0, i] == 0).all()
+        assert not sees[i] or (o[0, i, 0] != 0).any()
