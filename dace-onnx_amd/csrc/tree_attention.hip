@@ -644,7 +644,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const float v = (float)value[32 * (column_wave * VT + c) + 8 * (r / 4) + 4 * h + r % 4];
-                            if (!(__builtin_fabsf(v) < __builtin_inff())) out[i][c][r] += weight * v;
+                            if (!(__builtin_fabsf(v) < __builtin_inff())) out[i][c][r] += sizeof(T) == 4 ? __builtin_nanf("") : weight * v;   // (float32: as its three parts have it)
                         }
                 }
             }

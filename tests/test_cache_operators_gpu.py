@@ -754,3 +754,26 @@ def test_attention_of_empty_entries_that_the_table_has_little_room_for(form, dea
     for i in range(tokens):
         assert torch.isnan(o[0, i, 1]).all() if sees[i] else (o[0, i] == 0).all()
         assert not sees[i] or (o[0, i, 0] != 0).any()
+
+
+INFINITE = [float("inf"), float("-inf"), float("nan")]
+
+
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 40), (2, 40)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_in_float32_of_infinite_values_is_not_a_number_whatever_the_form(form, dealt, d, tuning):
+    """Of a context that all rows see, and of tokens that only later ones see, wherever the blocks of a form end."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    tokens, context, page = 150, 90, 6 if d == 64 else 16
+    columns = -(-(context + tokens) // page)
+    table, pages = shuffled_table(1, 1, columns)
+    q, kp, vp = normal(2, 1, tokens, 2, d, scale=0.1), normal(3, pages, 1, page, d), normal(4, pages, 1, page, d)
+    bad = {-7: 3, 0: d - 1, 31: 5, 63: d // 2, 64: 9, 100: 40, 127: 17, 128: 33, 149: 62}   # number after the context -> column
+    for i, (n, column) in enumerate(bad.items()):
+        vp[int(table[0, (context + n) // page]), :, (context + n) % page, column] = INFINITE[i % 3]
+    m, inputs = C.attention_model(q, kp, vp, table, whole([context]))
+    o = m(*inputs)
+    expected = torch.zeros_like(o, dtype=torch.bool)
+    for n, column in bad.items():
+        expected[0, max(n, 0):, :, column] = True
+    assert torch.equal(torch.isnan(o), expected) and torch.isfinite(o[~expected]).all()
