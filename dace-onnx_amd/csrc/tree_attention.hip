@@ -195,20 +195,24 @@ __device__ __forceinline__ void tree_read_keys(uint32_t lds_k, int s0, typename 
 }
 
 // S^T of 32 keys and 32 rows; between(s): what else goes on behind product s
-template <class T, int D, int RB, int BATCH, class F>
-__device__ __forceinline__ void tree_scores(uint32_t lds_k, typename Values<T, 8>::vec (&k)[BATCH], const Operand<T> (&q)[RB][D / 16], f32x16 (&acc)[RB], F&& between) {
-#pragma unroll
-    for (int b = 0; b < RB; ++b) acc[b] = f32x16{};
+template <class T, int D, int BATCH, class F>
+__device__ __forceinline__ void tree_scores(uint32_t lds_k, typename Values<T, 8>::vec (&k)[BATCH], const Operand<T> (&q)[D / 16], f32x16& acc, F&& between) {
+    acc = f32x16{};
 #pragma unroll
     for (int s0 = 0; s0 < D / 16; s0 += BATCH) {
         if (s0) tree_read_keys<T, D, BATCH>(lds_k, s0, k);
 #pragma unroll
         for (int s = 0; s < BATCH; ++s) {
-#pragma unroll
-            for (int b = 0; b < RB; ++b) Operand<T>::product({{k[s]}}, q[b][s0 + s], acc[b]);
+            Operand<T>::product({{k[s]}}, q[s0 + s], acc);
             between(s0 + s);
         }
     }
+}
+
+// (the wave's for blocks of rows, of which it has one)
+template <int D>
+__device__ __forceinline__ void tree_scores_f32(uint32_t lds_k, const Operand<float> (&q)[D / 16], f32x16& acc) {
+    AttentionWave<float, D, D>::scores(lds_k, reinterpret_cast<const Operand<float>(&)[1][D / 16]>(q), reinterpret_cast<f32x16(&)[1]>(acc));
 }
 
 // The values' operands of 32 keys: in registers by the time the probabilities are
@@ -229,28 +233,22 @@ __device__ __forceinline__ void tree_read_values(uint32_t lds_v, typename Values
 }
 
 // between(n): behind product n of 2 VT
-template <class T, int VT, int RB, class F>
-__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * VT], const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB], F&& between) {
+template <class T, int VT, class F>
+__device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v)[2 * VT], const f32x16& prob, f32x16 (&out)[VT], float& sum, F&& between) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        Operand<T> pr[RB];
-        T x[RB][8];
+        Operand<T> pr;
+        T x[8];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][e] = (T)prob[b][8 * t + e];
-            pr[b].set(x[b]);
-        }
+        for (int e = 0; e < 8; ++e) x[e] = (T)prob[8 * t + e];
+        pr.set(x);
 #pragma unroll
         for (int c = 0; c < VT; ++c) {
-#pragma unroll
-            for (int b = 0; b < RB; ++b) Operand<T>::product({{v[t * VT + c]}}, pr[b], out[b][c]);
-            if (c == 0)
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    pr[b].add_to(sum[b], x[b]);
-                    asm volatile("" : "+v"(sum[b]));   // (taken here, not behind all products)
-                }
+            Operand<T>::product({{v[t * VT + c]}}, pr, out[c]);
+            if (c == 0) {
+                pr.add_to(sum, x);
+                asm volatile("" : "+v"(sum));   // (taken here, not behind all products)
+            }
             between(t * VT + c);
         }
     }
@@ -258,27 +256,24 @@ __device__ __forceinline__ void tree_values(const typename Values<T, 8>::vec (&v
 
 // Of float32: the products of 32 keys have sums of their own, which are added to the outputs. The matrix unit loses a little of every sum it adds to, towards zero: outputs of 10000 keys were
 // off by 4.7e-6 (2-norm) where all products went to one sum, of 60000 by 1.3e-5; so 2.4e-7 and 3.3e-7, for 1 to 5 % of the time. The sum of the probabilities keeps what its additions lose.
-template <int D, int VT, int RB>
-__device__ __forceinline__ void tree_values_f32(uint32_t lds_v, const f32x16 (&prob)[RB], f32x16 (&out)[RB][VT], float (&sum)[RB], float (&lost)[RB]) {
+template <int D, int VT>
+__device__ __forceinline__ void tree_values_f32(uint32_t lds_v, const f32x16& prob, f32x16 (&out)[VT], float& sum, float& lost) {
     constexpr int ROW = AttentionTile<float, D>::ROW;
-    Operand<float> pr[2][RB];
+    Operand<float> pr[2];
+    float all = 0.0f;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        float all = 0.0f;
+    for (int t = 0; t < 2; ++t) {
+        float x[8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = prob[b][8 * t + e];
-            pr[t][b].set(x);
-            pr[t][b].add_to(all, x);
-        }
-        const float before = sum[b], added = before + all - before;
-        sum[b] = before + all;
-        lost[b] += (before - (sum[b] - added)) + (all - added);
+        for (int e = 0; e < 8; ++e) x[e] = prob[8 * t + e];
+        pr[t].set(x);
+        pr[t].add_to(all, x);
     }
-    f32x16 acc[2][RB];
-    AttentionWave<float, D, D>::template each_operand<2 * VT, 6 * RB>(
+    const float before = sum, added = before + all - before;
+    sum = before + all;
+    lost += (before - (sum - added)) + (all - added);
+    f32x16 acc[2];
+    AttentionWave<float, D, D>::template each_operand<2 * VT, 6>(
         [&](auto operand, auto& v) __attribute__((always_inline)) {
             constexpr int c = decltype(operand)::value / 2, t = decltype(operand)::value % 2;
 #pragma unroll
@@ -287,31 +282,28 @@ __device__ __forceinline__ void tree_values_f32(uint32_t lds_v, const f32x16 (&p
         },
         [&](auto operand, const Operand<float>& v) __attribute__((always_inline)) {
             constexpr int c = decltype(operand)::value / 2, t = decltype(operand)::value % 2;
-#pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                if constexpr (t == 0) acc[c % 2][b] = f32x16{};
-                Operand<float>::product(v, pr[t][b], acc[c % 2][b]);
-                if constexpr (t == 0 && c > 0) out[b][c - 1] += acc[(c + 1) % 2][b];   // (those of the columns before: nobody waits for these)
-                if constexpr (t == 1 && c == VT - 1) out[b][c] += acc[c % 2][b];
-            }
+            if constexpr (t == 0) acc[c % 2] = f32x16{};
+            Operand<float>::product(v, pr[t], acc[c % 2]);
+            if constexpr (t == 0 && c > 0) out[c - 1] += acc[(c + 1) % 2];   // (those of the columns before: nobody waits for these)
+            if constexpr (t == 1 && c == VT - 1) out[c] += acc[c % 2];
         });
 }
 
-// Waves: RW blocks of 32 RB rows, CW shares of the value columns (each takes the scores for itself), KW shares of a stage's keys, 32 SUB each; NS stages. WHOLE: no transfer's keys lie in
+// Waves: RW blocks of 32 rows, CW shares of the value columns (each takes the scores for itself), KW shares of a stage's keys, 32 SUB each; NS stages. WHOLE: no transfer's keys lie in
 // two pages.
-template <class T, int D, int RB, int RW, int CW, int KW, int SUB, int NS, int PER_SIMD, bool WHOLE>
+template <class T, int D, int RW, int CW, int KW, int SUB, int NS, int PER_SIMD, bool WHOLE>
 __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_kernel(TreeArgs p) {
     using Tile = AttentionTile<T, D>;
     using Wave = AttentionWave<T, D, D, D / CW>;
     using Piece = typename Wave::Piece;
     using UnalignedPiece = typename Wave::UnalignedPiece;
-    constexpr int KT = 32 * KW * SUB, E = Tile::E, NT = 64 * RW * CW * KW, VT = Wave::VT, ROWS = 32 * RB * RW;
+    constexpr int KT = 32 * KW * SUB, E = Tile::E, NT = 64 * RW * CW * KW, VT = Wave::VT, ROWS = 32 * RW;
     constexpr int HALF = KT * Tile::ROW, STAGE = 2 * HALF;            // keys, then values
     constexpr int PER_T = KT * Tile::PIECES / NT, KPT = WAVE / Tile::PIECES;   // transfers of a wave's keys in a stage, keys to a transfer
     static_assert(KT * Tile::PIECES % NT == 0 && Tile::PIECES <= WAVE && NS >= 2 && (NS - 2) * 2 * PER_T < 64, "whole pieces to a thread, whole keys to a transfer");
     constexpr int EXCHANGE = 32 * D / CW;   // floats of a wave's output
     constexpr bool AHEAD = sizeof(T) == 2;   // operands are read from LDS all at once, before they are needed
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[std::max(NS * STAGE, KW == 1 ? 0 : 4 * EXCHANGE * (KW / 2) * RW * CW * RB)];
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[std::max(NS * STAGE, KW == 1 ? 0 : 4 * EXCHANGE * (KW / 2) * RW * CW)];
     __shared__ int16_t parents[TREE_MOST];
     __shared__ uint32_t odd_keys[2][KT / 32];   // of the stage and the one before
 
@@ -356,9 +348,9 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
         }
     }
     // keys that any row of the workgroup sees, and that all of them see; the same of the wave
-    const int64_t row0 = block * ROWS + row_wave * RB * 32;   // of the wave
+    const int64_t row0 = block * ROWS + row_wave * 32;   // of the wave
     const int end = up_to(std::min(rows, (block + 1) * ROWS) - 1), all = p.parents ? length : up_to(block * ROWS);
-    const int wave_end = row0 < rows ? __builtin_amdgcn_readfirstlane(up_to(std::min(rows, row0 + 32 * RB) - 1)) : 0;
+    const int wave_end = row0 < rows ? __builtin_amdgcn_readfirstlane(up_to(std::min(rows, row0 + 32) - 1)) : 0;
     const int wave_all = p.parents ? length : __builtin_amdgcn_readfirstlane(up_to(std::min(rows - 1, row0)));
     const int stages = (end + KT - 1) / KT, first = (int)((int64_t)part * stages / parts), last = (int)((int64_t)(part + 1) * stages / parts), count = last - first;
 
@@ -432,41 +424,30 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
         }
 
     // ---- queries: row r of a slice is head r % share of token r / share --------------------------------
-    int token[RB], ancestor[RB];
-    Operand<T> q[RB][Wave::QP];
+    const int64_t row = row0 + n, known_row = row < rows ? row : rows - 1;
+    const int token = (int)(known_row / p.share);
+    int ancestor = token;
+    Operand<T> q[Wave::QP];
+    const T* query = static_cast<const T*>(p.q) + ((b * p.tokens + token) * p.heads + group * p.share + (int)(known_row % p.share)) * D + 8 * h;
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        const int64_t row = row0 + 32 * i + n, r = row < rows ? row : rows - 1;
-        token[i] = ancestor[i] = (int)(r / p.share);
-        const int head = group * p.share + (int)(r % p.share);
-        const T* from = static_cast<const T*>(p.q) + ((b * p.tokens + token[i]) * p.heads + head) * D + 8 * h;
+    for (int s = 0; s < Wave::QP; ++s) {
+        T v[8];
 #pragma unroll
-        for (int s = 0; s < Wave::QP; ++s) {
-            T v[8];
+        for (int j = 0; j < 8 / E; ++j) {
+            const Piece piece = *reinterpret_cast<const UnalignedPiece*>(query + 16 * s + j * E);
 #pragma unroll
-            for (int j = 0; j < 8 / E; ++j) {
-                const Piece piece = *reinterpret_cast<const UnalignedPiece*>(from + 16 * s + j * E);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[j * E + e] = piece[e];
-            }
-            q[i][s].set(v);
+            for (int e = 0; e < E; ++e) v[j * E + e] = piece[e];
         }
+        q[s].set(v);
     }
     // The queries are here before the loop begins: the compiler would wait for them in it, each time, and so for all transfers, which count with them.
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
+    for (int s = 0; s < Wave::QP; ++s)
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(q[s].part[0]));
+    f32x16 out[VT];
+    float base = -__builtin_inff(), sum = 0.0f, lost = 0.0f;   // of the scores times scale_log2; the lane's share of the sum, and what it lost by rounding (float32)
 #pragma unroll
-        for (int s = 0; s < Wave::QP; ++s)
-            if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(q[i][s].part[0]));
-    f32x16 out[RB][VT];
-    float base[RB], sum[RB], lost[RB];   // of the scores times scale_log2; the lane's share of the sum, and what it lost by rounding (float32)
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        base[i] = -__builtin_inff();
-        sum[i] = lost[i] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < VT; ++c) out[i][c] = f32x16{};
-    }
+    for (int c = 0; c < VT; ++c) out[c] = f32x16{};
 
     int buffer = 0;
     for (int turn = 0; turn < count; ++turn, buffer = buffer + 1 == NS ? 0 : buffer + 1) {
@@ -505,7 +486,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
         }
         if (stage * KT + key_wave * SUB * 32 >= wave_end) continue;   // (the same for the wave)
         // The scores of the next 32 keys are taken between the powers of these, their maxima between the products with the values of these.
-        f32x16 scores[SUB][RB];
+        f32x16 scores[SUB];
         const uint32_t keys0 = lds0 + (uint32_t)(buffer * STAGE + key_wave * SUB * 32 * Tile::ROW);
         constexpr int QP = Wave::QP, BATCH = QP < 8 ? QP : 8;
         typename Values<T, 8>::vec kh[AHEAD ? BATCH : 1];
@@ -518,14 +499,12 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
             const uint32_t at = key_place(SUB - 1);
             tree_read_keys<T, D, BATCH>(at, 0, kh);
             __builtin_amdgcn_sched_barrier(0);
-            tree_scores<T, D, RB, BATCH>(at, kh, q, scores[SUB - 1], [](int) {});
-        } else Wave::scores(key_place(SUB - 1), q, scores[SUB - 1]);
-        float largest[RB];   // of the lane's scores of 32 keys
+            tree_scores<T, D, BATCH>(at, kh, q, scores[SUB - 1], [](int) {});
+        } else tree_scores_f32<D>(key_place(SUB - 1), q, scores[SUB - 1]);
+        float largest;   // of the lane's scores of 32 keys
         auto look = [&](int u, int r0, int r1) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < RB; ++i)
-#pragma unroll
-                for (int r = r0; r < r1; ++r) largest[i] = r ? fmaxf(largest[i], scores[u][i][r]) : scores[u][i][0];
+            for (int r = r0; r < r1; ++r) largest = r ? fmaxf(largest, scores[u][r]) : scores[u][0];
         };
         look(SUB - 1, 0, 16);
 #pragma unroll
@@ -535,7 +514,7 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
             asm volatile("" : "+v"(lds_v));
             uint32_t next_k = 0;
             typename Values<T, 8>::vec held[AHEAD ? 2 * VT : 1];
-            f32x16 (&s)[RB] = scores[u];
+            f32x16& s = scores[u];
             if constexpr (AHEAD) {
                 if (u > 0) {
                     next_k = key_place(u - 1);
@@ -543,60 +522,42 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                 }
                 tree_read_values<T, D, VT>(lds_v, held);
                 __builtin_amdgcn_sched_barrier(0);
-            } else if (u > 0) Wave::scores(key_place(u - 1), q, scores[u - 1]);
-            uint32_t seen[RB];   // of the 32 keys
-#pragma unroll
-            for (int i = 0; i < RB; ++i) seen[i] = ~0u;
+            } else if (u > 0) tree_scores_f32<D>(key_place(u - 1), q, scores[u - 1]);
+            uint32_t seen = ~0u;   // of the 32 keys
             if (key0 + 32 > wave_all) {
-#pragma unroll
-                for (int i = 0; i < RB; ++i) {
-                    if (p.parents) {
-                        seen[i] = lowest_bits(length - key0);
-                        while (length + ancestor[i] >= key0 && ancestor[i] >= 0) {
-                            const int bit = length + ancestor[i] - key0;
-                            if (bit < 32) seen[i] |= 1u << bit;
-                            ancestor[i] = parents[ancestor[i]];
-                        }
-                    } else {
-                        seen[i] = lowest_bits(length + token[i] + 1 - key0);
+                if (p.parents) {
+                    seen = lowest_bits(length - key0);
+                    while (length + ancestor >= key0 && ancestor >= 0) {
+                        const int bit = length + ancestor - key0;
+                        if (bit < 32) seen |= 1u << bit;
+                        ancestor = parents[ancestor];
                     }
-                    seen[i] &= lowest_bits(total - key0);
-                    const uint32_t mine = seen[i] >> (4 * h);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!(mine >> (8 * (r / 4) + r % 4) & 1)) s[i][r] = -__builtin_inff();
+                } else {
+                    seen = lowest_bits(length - key0 + token + 1);   // (in this order no sum leaves 32 bits)
                 }
+                seen &= lowest_bits(total - key0);
+                const uint32_t mine = seen >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(mine >> (8 * (r / 4) + r % 4) & 1)) s[r] = -__builtin_inff();
                 look(u, 0, 16);
             }
             // The base of a row's powers is the largest score so far, or up to 8 below it: P is at most 2^8, and outputs are rarely scaled. float16 has no
             // values below 2^-25 and few digits below 2^-14, where many keys of little weight may outweigh the rest: 10 to 15 below the largest score.
             constexpr float BELOW = std::is_same_v<T, f16> ? 10.0f : 0.0f, MOST = std::is_same_v<T, f16> ? 15.0f : 8.0f;
-            float m[RB];
-            bool far = false;
+            const float m = across_halves(largest, [](float x, float y) { return fmaxf(x, y); }) * p.scale_log2;
+            if (__any(m > base + MOST)) {
+                const float now = fmaxf(base, m - BELOW), factor = base == now ? 1.0f : __builtin_amdgcn_exp2f(base - now);
+                base = now;
+                sum *= factor;
+                lost *= factor;
 #pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                m[i] = across_halves(largest[i], [](float x, float y) { return fmaxf(x, y); }) * p.scale_log2;
-                far |= m[i] > base[i] + MOST;
+                for (int c = 0; c < VT; ++c) out[c] *= factor;
             }
-            if (__any(far)) {
-#pragma unroll
-                for (int i = 0; i < RB; ++i) {
-                    const float now = fmaxf(base[i], m[i] - BELOW), factor = base[i] == now ? 1.0f : __builtin_amdgcn_exp2f(base[i] - now);
-                    base[i] = now;
-                    sum[i] *= factor;
-                    lost[i] *= factor;
-#pragma unroll
-                    for (int c = 0; c < VT; ++c) out[i][c] *= factor;
-                }
-            }
-            float from[RB];
-#pragma unroll
-            for (int i = 0; i < RB; ++i) from[i] = base[i] == -__builtin_inff() ? 0.0f : base[i];   // no key so far: exp2(-inf)
+            const float from = base == -__builtin_inff() ? 0.0f : base;   // no key so far: exp2(-inf)
             auto powers = [&](int r0, int r1) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < RB; ++i)
-#pragma unroll
-                    for (int r = r0; r < r1; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -from[i]));
+                for (int r = r0; r < r1; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, -from));
             };
             if constexpr (AHEAD) {
                 // Vector instructions in between of the products, a few to each: a wave's own hide there almost whole (two powers with their multiply-adds behind a product of 32 cycles
@@ -604,14 +565,13 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                 constexpr int EACH = 16 / QP, LATER = 8 / VT;   // powers to a product, the maxima as many as LATER
                 __builtin_amdgcn_sched_barrier(0);
                 if (u > 0) {
-                    tree_scores<T, D, RB, BATCH>(next_k, kh, q, scores[u - 1], [&](int n) __attribute__((always_inline)) {
+                    tree_scores<T, D, BATCH>(next_k, kh, q, scores[u - 1], [&](int n) __attribute__((always_inline)) {
                         powers(n * EACH, (n + 1) * EACH);
                         __builtin_amdgcn_sched_barrier(0);
                     });
                     tree_values<T, VT>(held, s, out, sum, [&](int n) __attribute__((always_inline)) {
                         look(u - 1, n * LATER, (n + 1) * LATER);
-#pragma unroll
-                        for (int i = 0; i < RB; ++i) asm volatile("" : "+v"(largest[i]));   // (taken here, not where it is needed)
+                        asm volatile("" : "+v"(largest));   // (taken here, not where it is needed)
                         __builtin_amdgcn_sched_barrier(0);
                     });
                 } else {
@@ -632,107 +592,89 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
             for (uint32_t left = __builtin_amdgcn_readfirstlane(odd[local / 32]); left; left &= left - 1) {
                 const int key = __builtin_ctz(left), at = key0 + key, column = tree_column(p, at);
                 const T* value = reinterpret_cast<const T*>(V + from_page(columns[column], at - column * p.page_size));
+                float weight = 0.0f;
 #pragma unroll
-                for (int i = 0; i < RB; ++i) {
-                    float weight = 0.0f;
+                for (int r = 0; r < 16; ++r) weight = r == key / 8 * 4 + key % 4 ? s[r] : weight;
+                weight = __shfl(weight, n + key / 4 % 2 * 32);
+                if (!(seen >> key & 1)) continue;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) weight = r == key / 8 * 4 + key % 4 ? s[i][r] : weight;
-                    weight = __shfl(weight, n + key / 4 % 2 * 32);
-                    if (!(seen[i] >> key & 1)) continue;
+                for (int c = 0; c < VT; ++c)
 #pragma unroll
-                    for (int c = 0; c < VT; ++c)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float v = (float)value[32 * (column_wave * VT + c) + 8 * (r / 4) + 4 * h + r % 4];
-                            if (!(__builtin_fabsf(v) < __builtin_inff())) out[i][c][r] += sizeof(T) == 4 ? __builtin_nanf("") : weight * v;   // (float32: as its three parts have it)
-                        }
-                }
+                    for (int r = 0; r < 16; ++r) {
+                        const float v = (float)value[32 * (column_wave * VT + c) + 8 * (r / 4) + 4 * h + r % 4];
+                        if (!(__builtin_fabsf(v) < __builtin_inff())) out[c][r] += sizeof(T) == 4 ? __builtin_nanf("") : weight * v;   // (float32: as its three parts have it)
+                    }
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < RB; ++i) sum[i] = across_halves(sum[i] + lost[i], [](float x, float y) { return x + y; });
+    sum = across_halves(sum + lost, [](float x, float y) { return x + y; });
 
     // ---- the shares of the keys meet, in pairs ------------------------------------------------------------
     if constexpr (KW > 1) {
         float* exchange = reinterpret_cast<float*>(lds);
-        __shared__ float base_sum[KW][RW][RB][2][32];
+        __shared__ float base_sum[KW][RW][2][32];
         __syncthreads();   // nobody reads the stages any more
         if (h == 0 && column_wave == 0) {   // (the others have the same)
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                base_sum[key_wave][row_wave][i][0][n] = base[i];
-                base_sum[key_wave][row_wave][i][1][n] = sum[i];
-            }
+            base_sum[key_wave][row_wave][0][n] = base;
+            base_sum[key_wave][row_wave][1][n] = sum;
         }
         __syncthreads();
+        float top = -__builtin_inff(), whole_sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < RB; ++i) {
-            float top = -__builtin_inff(), whole_sum = 0.0f;
+        for (int w = 0; w < KW; ++w) top = fmaxf(top, base_sum[w][row_wave][0][n]);
+        const float from = top == -__builtin_inff() ? 0.0f : top, factor = __builtin_amdgcn_exp2f(base - from);
 #pragma unroll
-            for (int w = 0; w < KW; ++w) top = fmaxf(top, base_sum[w][row_wave][i][0][n]);
-            const float from = top == -__builtin_inff() ? 0.0f : top, factor = __builtin_amdgcn_exp2f(base[i] - from);
+        for (int w = 0; w < KW; ++w) whole_sum = fmaf(base_sum[w][row_wave][1][n], __builtin_amdgcn_exp2f(base_sum[w][row_wave][0][n] - from), whole_sum);
+        base = top;
+        sum = whole_sum;
 #pragma unroll
-            for (int w = 0; w < KW; ++w) whole_sum = fmaf(base_sum[w][row_wave][i][1][n], __builtin_amdgcn_exp2f(base_sum[w][row_wave][i][0][n] - from), whole_sum);
-            base[i] = top;
-            sum[i] = whole_sum;
-#pragma unroll
-            for (int c = 0; c < VT; ++c) out[i][c] *= factor;
-        }
+        for (int c = 0; c < VT; ++c) out[c] *= factor;
 #pragma unroll
         for (int step = KW / 2; step >= 1; step /= 2) {
-            const int slot = ((key_wave % step) * CW + column_wave) * RW + row_wave;
+            float* const slot = exchange + (((key_wave % step) * CW + column_wave) * RW + row_wave) * EXCHANGE;
             if (key_wave >= step && key_wave < 2 * step) {
 #pragma unroll
-                for (int i = 0; i < RB; ++i)
+                for (int c = 0; c < VT; ++c)
 #pragma unroll
-                    for (int c = 0; c < VT; ++c)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) exchange[(slot * RB + i) * EXCHANGE + (16 * c + r) * WAVE + lane] = out[i][c][r];
+                    for (int r = 0; r < 16; ++r) slot[(16 * c + r) * WAVE + lane] = out[c][r];
             }
             __syncthreads();
             if (key_wave < step) {
 #pragma unroll
-                for (int i = 0; i < RB; ++i)
+                for (int c = 0; c < VT; ++c)
 #pragma unroll
-                    for (int c = 0; c < VT; ++c)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) out[i][c][r] += exchange[(slot * RB + i) * EXCHANGE + (16 * c + r) * WAVE + lane];
+                    for (int r = 0; r < 16; ++r) out[c][r] += slot[(16 * c + r) * WAVE + lane];
             }
             __syncthreads();
         }
     }
 
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        const int64_t row = row0 + 32 * i + n;
-        if (key_wave || row >= rows) continue;
-        if (parts > 1) {
-            const int64_t at = (int64_t)blockIdx.x * p.block_rows + (row - block * ROWS);
-            if (h == 0 && column_wave == 0) {
-                p.partial_ml[2 * at] = base[i];
-                p.partial_ml[2 * at + 1] = sum[i];
-            }
-#pragma unroll
-            for (int c = 0; c < VT; ++c)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(p.partial_o + at * D + 32 * (column_wave * VT + c) + 8 * g + 4 * h) =
-                        f32x4{out[i][c][4 * g], out[i][c][4 * g + 1], out[i][c][4 * g + 2], out[i][c][4 * g + 3]};
-            continue;
+    if (key_wave || row >= rows) return;
+    if (parts > 1) {
+        const int64_t at = (int64_t)blockIdx.x * p.block_rows + (row - block * ROWS);
+        if (h == 0 && column_wave == 0) {
+            p.partial_ml[2 * at] = base;
+            p.partial_ml[2 * at + 1] = sum;
         }
-        const float factor = sum[i] == 0.0f ? tree_no_weights(p, entry, token[i], [&](int at) { return (int)parents[at]; }) : 1.0f / sum[i];
-        T* to = static_cast<T*>(p.o) + ((b * p.tokens + token[i]) * p.heads + group * p.share + (int)(row % p.share)) * D;
 #pragma unroll
         for (int c = 0; c < VT; ++c)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = out[i][c][4 * g + e] * factor;
-                store_values(to + 32 * (column_wave * VT + c) + 8 * g + 4 * h, o, 4);
-            }
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(p.partial_o + at * D + 32 * (column_wave * VT + c) + 8 * g + 4 * h) =
+                    f32x4{out[c][4 * g], out[c][4 * g + 1], out[c][4 * g + 2], out[c][4 * g + 3]};
+        return;
     }
+    const float factor = sum == 0.0f ? tree_no_weights(p, entry, token, [&](int at) { return (int)parents[at]; }) : 1.0f / sum;
+    T* to = static_cast<T*>(p.o) + ((b * p.tokens + token) * p.heads + group * p.share + (int)(row % p.share)) * D;
+#pragma unroll
+    for (int c = 0; c < VT; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = out[c][4 * g + e] * factor;
+            store_values(to + 32 * (column_wave * VT + c) + 8 * g + 4 * h, o, 4);
+        }
 }
 
 // The parts of a row joined: WAVES waves to a row share its parts, the lanes of each are the D values. A block of one part is done.
@@ -872,8 +814,8 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
     constexpr int BYTES = D * (int)sizeof(T);
     const int64_t rows = p.tokens * p.share, slices = p.batch * p.kv_heads;
     bool fits = true;
-    auto launch = [&](auto rb, auto rw, auto cw, auto kw, auto sub, auto ns, auto per_simd) {
-        constexpr int RB = decltype(rb)::value, RW = decltype(rw)::value, CW = decltype(cw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
+    auto launch = [&](auto rw, auto cw, auto kw, auto sub, auto ns, auto per_simd) {
+        constexpr int RW = decltype(rw)::value, CW = decltype(cw)::value, KW = decltype(kw)::value, SUB = decltype(sub)::value, NS = decltype(ns)::value;
         constexpr int PER_SIMD = decltype(per_simd)::value;
         const int64_t grid = p.dealt ? p.dealt : p.row_blocks * slices;
         // A wave has eight parts of a row on their way at once: four and sixteen waves to a row of more. us by four / sixteen: 16 rows of 128 parts 5.8 / 5.0, 32 of 64 3.9 / 4.5.
@@ -883,8 +825,8 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
         fits = grid_fits(grid, 64 * RW * CW * KW) && grid_fits(joins, 1024);
         if (!fits) return;
         const dim3 g((unsigned)grid), threads(64 * RW * CW * KW);
-        if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, CW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
-        else hipLaunchKernelGGL((tree_attention_kernel<T, D, RB, RW, CW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
+        if (p.page_size % (1024 / BYTES) == 0) hipLaunchKernelGGL((tree_attention_kernel<T, D, RW, CW, KW, SUB, NS, PER_SIMD, true>), g, threads, 0, st, p);
+        else hipLaunchKernelGGL((tree_attention_kernel<T, D, RW, CW, KW, SUB, NS, PER_SIMD, false>), g, threads, 0, st, p);
         if (!joins) return;
         if (join_waves == 16) hipLaunchKernelGGL((tree_join_kernel<T, D, 16>), dim3((unsigned)joins), dim3(1024), 0, st, p);
         else if (join_waves == 4) hipLaunchKernelGGL((tree_join_kernel<T, D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
@@ -894,9 +836,9 @@ static int launch_tree(TreeArgs p, const TreeCut& cut, hipStream_t st) {
     // and take the scores twice. us, 4 x 64 tokens behind 4096, 16 heads in 4 groups: bfloat16 128 -> 109, 128 rows a workgroup 214 -> 178, float32 939 -> 693; float32 heads of 128 are behind so.
     constexpr bool WIDE = BYTES > 256, WIDEST = BYTES > 512;
     constexpr int CW = D == 256 ? 2 : 1, PER_SIMD = WIDE && (D != 256 || WIDEST) ? 1 : 2;
-    if (cut.form == TREE_PAIR) launch(Int<1>{}, Int<2>{}, Int<CW>{}, Int<(WIDEST ? 1 : 2)>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<PER_SIMD>{});
-    else if (cut.form == TREE_TALL) launch(Int<1>{}, Int<4>{}, Int<(WIDEST ? 1 : CW)>{}, Int<1>{}, Int<(WIDE ? 1 : 2)>{}, Int<2>{}, Int<PER_SIMD>{});
-    else if constexpr (!WIDE) launch(Int<1>{}, Int<2>{}, Int<1>{}, Int<4>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
+    if (cut.form == TREE_PAIR) launch(Int<2>{}, Int<CW>{}, Int<(WIDEST ? 1 : 2)>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<PER_SIMD>{});
+    else if (cut.form == TREE_TALL) launch(Int<4>{}, Int<(WIDEST ? 1 : CW)>{}, Int<1>{}, Int<(WIDE ? 1 : 2)>{}, Int<2>{}, Int<PER_SIMD>{});
+    else if constexpr (!WIDE) launch(Int<2>{}, Int<1>{}, Int<4>{}, Int<1>{}, Int<(BYTES == 128 ? 4 : 2)>{}, Int<2>{});
     MI355X_REQUIRE(fits, "tree_attention: too large");
     return check_launch("tree_attention_kernel");
 }
