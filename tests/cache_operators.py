@@ -225,3 +225,94 @@ def greedy(weights, prompt, count):
         least = min(least, float(top.values[0] - top.values[1]))
         tokens.append(int(top.indices[0]))
     return tokens[len(prompt):], least
+
+
+# ---------------------------------------------------------------------------------------------- attention, row by row
+# Each row of D values has a bound of its own on its error's 2-norm, of what its own scores and weights are. U = 2^-24, P the row's weights, s its scores, w = scale sqrt(sum q^2 k^2), the size
+# of a random walk of a score's products.
+# Scores: n products of 16 terms go to one sum (D / 16, six times that in float32), each may lose up to 2^-23 of the sum so far, towards zero: U of it on average. A sum that walks from 0 to s is
+#   |s| / 2 + 0.4 w on the way. What float32 leaves out of a product is 2^-24.5 of it (one U more). The power's argument is rounded by U of itself, and the scale by 2 U: 3 U |s - largest|; the
+#   power by 2 U. A weight is off by A U of itself, A = n (|s| / 2 + 0.4 w) + |s| + 3 |s - largest| + 2. Such errors are of either sign for one key and another once the sum of the weights is
+#   divided by: sqrt(sum P^2 A^2 |v|^2) U, and sqrt(sum P^2 A^2) U of the result.
+# Values: 12 products for 32 keys, U of their sum each, and 2^-23.5 left out; the sums of N / 32 blocks are added at random; scaling, joining and dividing are a rounding each: (16 + sqrt(N / 32)) U
+#   of the result or of sqrt(sum P^2 |v|^2), whichever is larger (random values' results are as large as that).
+# 16 bits: weights and results are rounded, uniformly within half a step of their binade: sqrt(1 / 3) of it, of numbers of 1 to 2 in it whose root mean square is 1.47 to 1.53 (of even logarithms,
+#   of even values), so 0.4 of half a step relative to them as a mean over many, up to one half step for few: 0.4 (1 + 3 / sqrt(count)), count = D results, or as many keys as the weights are
+#   spread over. The two are independent.
+
+
+def attention_rows(q, k_pages, v_pages, table, lengths, parents=None, without=None, scores=None, weights=None):
+    """The result, and the bound of every row [B, S, H]. Every row sees a key, and what rows see is finite. ``without``: (entry, key) that is left out; ``scores`` and ``weights`` compute the two
+    products in another way."""
+    (B, S, H, D), (P, G, page, _) = q.shape, k_pages.shape
+    U, half, scale = 2.0 ** -24, R.HALF[q.dtype], D ** -0.5
+    products = D / 16 * (6 if q.dtype == torch.float32 else 1)
+    scores = scores or (lambda a, b: a @ b.t())
+    weights = weights or (lambda a, b: a @ b)
+    out = torch.zeros(B, S, H, D, dtype=torch.float64, device=q.device)
+    bound = torch.zeros(B, S, H, dtype=torch.float64, device=q.device)
+    spread = lambda count: (0.4 * (1 + 3 / count.sqrt())).clamp(max=1.0)   # noqa: E731
+    for b in range(B):
+        length = int(lengths[b])
+        numbers = torch.arange(min(length + S, page * table.shape[1]), device=q.device)
+        pages = table[b].long()[numbers // page]
+        seen = torch.ones(S, len(numbers), dtype=torch.bool, device=q.device)
+        own = lines(list(range(-1, S - 1)) if parents is None else parents[b].tolist()).to(q.device)
+        seen[:, length:] = own[:, :len(numbers) - length]
+        if without is not None and without[0] == b:
+            seen[:, without[1]] = False
+        for h in range(H):
+            x, k, v = q[b, :, h], k_pages[pages, h // (H // G), numbers % page], v_pages[pages, h // (H // G), numbers % page]
+            s = torch.where(seen, scale * scores(x.double(), k.double()), -torch.inf)
+            top = s.amax(-1, keepdim=True)
+            p = torch.exp(s - top)
+            total = p.sum(-1, keepdim=True)
+            out[b, :, h] = weights(p, v.double()) / total
+            p, s = p / total, torch.where(seen, s, 0.0)
+            walk = scale * (x.double().square() @ k.double().square().t()).sqrt()
+            off = torch.where(seen, products * (s.abs() / 2 + 0.4 * walk) + s.abs() + 3 * (top - s) + 2, 0.0)
+            values, size = v.double().square().sum(-1), out[b, :, h].norm(dim=-1)
+            each = (p.square() @ values).sqrt()
+            bound[b, :, h] = U * (((p * off).square() @ values).sqrt() + (p * off).norm(dim=-1) * size + (16 + (len(numbers) / 32) ** 0.5) * torch.maximum(each, size))
+            if q.dtype != torch.float32:
+                keys = (p.square() @ values).square() / (p.square().square() @ values.square())
+                bound[b, :, h] += half * ((spread(torch.tensor(float(D))) * size).square() + spread(keys).square() * (each.square() + p.square().sum(-1) * size.square())).sqrt()
+                bound[b, :, h] += D ** 0.5 * 2.0 ** -25 * (q.dtype == torch.float16)
+    return out, bound
+
+
+def attention_case(seed, batch, tokens, heads, groups, d, page, context, dtype, tree=False, device="cpu"):
+    """Entries of unequal lengths, pages in no order, what belongs to no token not a number."""
+    g = torch.Generator().manual_seed(seed)
+    normal = lambda *shape, scale=1.0: (torch.randn(*shape, generator=g) * scale).to(dtype)   # noqa: E731
+    lengths = [max(context - (7 * b + 1) * context // (4 * batch), 0) if b else context for b in range(batch)]
+    columns = -(-(context + tokens) // page)
+    pages = batch * columns + 2
+    table = torch.randperm(pages, generator=g)[:batch * columns].reshape(batch, columns).to(torch.int32)
+    q, k, v = normal(batch, tokens, heads, d, scale=2.0), normal(pages, groups, page, d), normal(pages, groups, page, d)
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    for b in range(batch):
+        numbers = torch.arange(lengths[b] + tokens)
+        used[table[b].long()[numbers // page], numbers % page] = True
+    hidden = ~used[:, None, :, None].expand(k.shape)
+    k[hidden] = v[hidden] = float("nan")
+    parents = (torch.rand(batch, tokens, generator=g) * torch.arange(tokens)).to(torch.int32).clamp(max=torch.arange(tokens, dtype=torch.int32) - 1) if tree else None
+    return [None if t is None else t.to(device) for t in (q, k, v, table, torch.tensor(lengths, dtype=torch.int32), parents)]
+
+
+def parts_of(x, count):
+    """x as `count` bfloat16 numbers, cut off one after the other, and what is left over dropped."""
+    x, result = x.float(), []
+    for _ in range(count):
+        part = (x.view(torch.int32) & -65536).view(torch.float32)
+        result.append(part.double())
+        x = x - part
+    return result
+
+
+def by_parts(count, least):
+    """A product of matrices by the partial products of `count` parts of each operand, the i-th with the j-th where i + j <= least."""
+    def product(a, b):
+        a, b = parts_of(a, count), parts_of(b, count)
+        return sum(a[i] @ b[j] for i in range(count) for j in range(count) if i + j <= least)
+    return {"scores": lambda x, k: product(x, k.t().contiguous()), "weights": product}

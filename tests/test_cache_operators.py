@@ -264,3 +264,43 @@ def test_keys_and_values_in_the_same_pages(apart):
 
 def test_a_scale_that_leaves_float32():
     assert "scale" in _refused("mi355x_tree_attention", *{**ATTENTION, "scale": 3e38}.values(), None)
+
+
+# ---------------------------------------------------------------------------------------------- the bound of a row
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_the_bound_of_a_row_takes_three_parts_and_no_two(d):
+    """What float32's operands become, in sums without an error of their own: of three parts the six largest products stay within the bound, of two parts the three largest do not."""
+    case = C.attention_case(1, 2, 5, 4, 2, d, 7, 300, F32, True)
+    expected, bound = C.attention_rows(*case)
+    three, two = (C.attention_rows(*case, **C.by_parts(count, least))[0] for count, least in ((3, 2), (2, 1)))
+    assert ((three - expected).norm(dim=-1) < bound / 3).all()
+    assert ((two - expected).norm(dim=-1) > bound).double().mean() > 0.5
+
+
+@pytest.mark.parametrize("dtype, share", [(F32, 0.99), (torch.float16, 0.9), (BF, 0.4)])
+@pytest.mark.parametrize("d", [64, 256])
+def test_the_bound_of_a_row_sees_a_key_that_is_missing(dtype, share, d):
+    """One of 5000 keys with scores of a deviation of 2 is worth e^(s - 4) / sqrt(5000) of a row's result. The bound is 2.8e-5 of that, 4.9e-4, 3.9e-3: s above -2.2, 0.6, 2.7, which 86, 38 and 9 % of keys
+    have for a row, and 100, 98 and 52 % for one of eight."""
+    case = C.attention_case(2, 1, 1, 8, 1, d, 16, 5000, dtype)
+    expected, bound = C.attention_rows(*case)
+    found = [bool(((C.attention_rows(*case, without=(0, n))[0] - expected).norm(dim=-1) > bound).any()) for n in range(1, 5000, 173)]
+    assert np.mean(found) >= share
+
+
+def test_the_bounds_of_rows_are_near_what_rounding_does():
+    """Results and weights rounded to 16 bits, nothing else: within the bound, and above a quarter of it on average."""
+    for dtype in (torch.float16, BF):
+        case = C.attention_case(3, 2, 9, 4, 2, 64, 16, 700, dtype)
+        expected, bound = C.attention_rows(*case)
+
+        def rounded(p, v):
+            r = p.to(dtype).double()
+            return r @ v * (p.sum(-1, keepdim=True) / r.sum(-1, keepdim=True))
+        got = C.attention_rows(*case, weights=rounded)[0].to(dtype)
+        error = (got.double() - expected).norm(dim=-1) / bound
+        assert error.max() < 1 and error.mean() > 0.25
+    out, _ = C.attention(*C.attention_case(4, 2, 9, 4, 2, 64, 16, 70, F32, True))
+    assert torch.allclose(out, C.attention_rows(*C.attention_case(4, 2, 9, 4, 2, 64, 16, 70, F32, True))[0], rtol=1e-12, atol=1e-12)

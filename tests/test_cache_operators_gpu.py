@@ -777,3 +777,41 @@ def test_attention_in_float32_of_infinite_values_is_not_a_number_whatever_the_fo
     for n, column in bad.items():
         expected[0, max(n, 0):, :, column] = True
     assert torch.equal(torch.isnan(o), expected) and torch.isfinite(o[~expected]).all()
+
+
+# ---------------------------------------------------------------------------------------------- row by row
+
+
+def check_rows(*sizes, **more):
+    """Every row's error within a bound of its own scores and weights (``cache_operators.attention_rows``)."""
+    case = C.attention_case(11, *sizes, **more, device="cuda")
+    m, inputs = C.attention_model(*case)
+    expected, bound = C.attention_rows(*case)
+    for _ in range(2):   # the general way, then the short one
+        error = (m(*inputs).double() - expected).norm(dim=-1)
+        worst = float((error / bound).max())
+        assert worst <= 1, f"{worst:.3g} of the bound in row {tuple(((error / bound) == worst).nonzero()[0].tolist())}"
+
+
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 60), (1, 60), (2, 60)])
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("batch, tokens, heads, groups, page, context, tree", [(3, 40, 4, 2, 23, 500, True), (2, 150, 2, 2, 16, 300, False)])
+def test_rows_of_every_form(form, dealt, dtype, d, batch, tokens, heads, groups, page, context, tree, tuning):
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    check_rows(batch, tokens, heads, groups, d, page, context, dtype, tree)
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("page", [1, 5, 7, 8, 11, 32, 64, 256])
+@pytest.mark.parametrize("tokens, tree", [(1, False), (9, True)])
+def test_rows_over_pages_of_any_size(dtype, page, tokens, tree):
+    check_rows(3, tokens, 6, 3, 64, page, 900, dtype, tree)
+
+
+@pytest.mark.parametrize("dtype", R.TYPES)
+@pytest.mark.parametrize("batch, tokens, heads, groups, d, page, context, tree", [
+    (1, 1, 8, 2, 128, 16, 9000, False), (70, 1, 2, 1, 64, 16, 700, False), (300, 1, 1, 1, 64, 8, 90, False), (1, 600, 2, 1, 64, 16, 0, False), (1, 200, 2, 1, 128, 16, 700, True), (4, 3, 40, 1, 64, 16, 2000, True)])
+def test_rows_of_calls_as_they_are(dtype, batch, tokens, heads, groups, d, page, context, tree):
+    """By the form that the sizes choose: few rows behind many keys, more entries than parts are dealt for, prompts, trees, many heads to a group."""
+    check_rows(batch, tokens, heads, groups, d, page, context, dtype, tree)
