@@ -815,3 +815,32 @@ def test_rows_over_pages_of_any_size(dtype, page, tokens, tree):
 def test_rows_of_calls_as_they_are(dtype, batch, tokens, heads, groups, d, page, context, tree):
     """By the form that the sizes choose: few rows behind many keys, more entries than parts are dealt for, prompts, trees, many heads to a group."""
     check_rows(batch, tokens, heads, groups, d, page, context, dtype, tree)
+
+
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 40)])
+@pytest.mark.parametrize("dtype", R.TYPES)
+def test_attention_of_scores_up_to_2_to_the_23rd(form, dealt, dtype, tuning):
+    """Scores that float32 holds, 2^13 or more apart but where they are equal: the mean of the values of a row's largest. Equal weights are rounded alike: what is left are sums of float32 and the
+    result's rounding."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    tokens, page, columns = 20, 8, 40
+    table, pages = shuffled_table(1, 2, columns)
+    q, kp, vp = torch.zeros(2, tokens, 4, 64, dtype=dtype, device="cuda"), torch.zeros(pages, 2, page, 64, dtype=dtype, device="cuda"), normal(4, pages, 2, page, 64, dtype=dtype)
+    q[..., 3] = torch.where(torch.arange(tokens, device="cuda") % 3 > 0, 8192.0, -8192.0)[None, :, None].to(dtype)
+    kp[..., 3] = (8192 - 64 * torch.randint(0, 60, (pages, 2, page), generator=torch.Generator().manual_seed(5))).to(dtype).cuda()   # (64 is a step of bfloat16 from 4096 on)
+    lengths = whole([290, 37])
+    expected, size = C.attention(q, kp, vp, table, lengths)
+    m, inputs = C.attention_model(q, kp, vp, table, lengths)
+    within(m(*inputs), expected, 64 * U * size + R.HALF[dtype] * expected.abs() * (1 + 2.0 ** -7) + TINY[dtype])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 40)])
+def test_attention_of_large_values(form, dealt, dtype, tuning):
+    """Of 2^103: 2^8 of them for each of 500 keys are below 2^128."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    q, kp, vp, *rest = C.attention_case(5, 2, 30, 4, 2, 64, 16, 450, dtype, True, device="cuda")
+    vp *= 2.0 ** 101
+    m, inputs = C.attention_model(q, kp, vp, *rest)
+    expected, bound = C.attention_rows(q, kp, vp, *rest)
+    assert ((m(*inputs).double() - expected).norm(dim=-1) <= bound).all()
