@@ -1031,9 +1031,13 @@ class MI355XDifferentialAttention(ONNXForward):
 
 
 def _updates_in_place(node, state):
-    """Whether each output that the node's schema says is an input's array is that array."""
-    data = {e.dst_conn: e.data.data for e in state.in_edges(node)}
-    return all(e.data.data == data.get(node.schema.updates[e.src_conn]) for e in state.out_edges(node) if e.src_conn in node.schema.updates)
+    """Whether each output that the node's schema says is an input's array is that array, and nobody else reads what the array was: which of the two came first would be open."""
+    read = {e.dst_conn: e for e in state.in_edges(node)}
+    for written in state.out_edges(node):
+        source = read.get(node.schema.updates.get(written.src_conn))
+        if written.src_conn in node.schema.updates and (source is None or source.data.data != written.data.data or state.out_degree(source.src) != 1):
+            return False
+    return True
 
 
 @op_implementation(op="PagedCacheAppend", name=IMPLEMENTATION_NAME)

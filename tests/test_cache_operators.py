@@ -152,6 +152,37 @@ def test_a_node_whose_output_is_another_array_is_refused():
         node.expand(sdfg, state)
 
 
+@pytest.mark.parametrize("shared", [True, False])
+def test_a_state_in_which_another_node_reads_what_the_array_was(shared):
+    """Nothing says which of the two comes first where both read one access node. A reader with a node of its own comes after the update."""
+    sdfg = dace.SDFG("s")
+    state = sdfg.add_state()
+    append, attend = donnx.ONNXPagedCacheAppend("append"), donnx.ONNXTreeAttention("attend")
+    shapes = {"K": SHAPES["k"], "V": SHAPES["v"], "k_pages": SHAPES["kp"], "v_pages": SHAPES["vp"], "table": (2, 4), "lengths": (2,), "Q": SHAPES["q"], "O": SHAPES["q"]}
+    for name, shape in shapes.items():
+        sdfg.add_array(name, shape, dace.int32 if name in ("table", "lengths") else dace.float32)
+    access = {}
+
+    def connect(node, reads, writes):
+        state.add_node(node)
+        for name in reads:
+            if name not in access or (name.endswith("_pages") and not shared):
+                access[name] = state.add_read(name)
+            node.add_in_connector(name)
+            state.add_edge(access[name], None, node, name, sdfg.make_array_memlet(name))
+        for conn, name in writes.items():
+            node.add_out_connector(conn)
+            state.add_edge(node, conn, state.add_write(name), None, sdfg.make_array_memlet(name))
+    connect(attend, ["Q", "k_pages", "v_pages", "table", "lengths"], {"O": "O"})
+    connect(append, ["K", "V", "k_pages", "v_pages", "table", "lengths"], {"k_pages_out": "k_pages", "v_pages_out": "v_pages"})
+    if shared:
+        with pytest.raises(donnx.ExpansionRefused):
+            sdfg.expand_library_nodes()
+    else:
+        sdfg.expand_library_nodes()
+        assert [n.function for _, n, *_ in dace.CompiledSDFG(sdfg)._plan] == ["mi355x_paged_cache_append", "mi355x_tree_attention"]
+
+
 def test_the_call_form_takes_one_array_for_both():
     values = {"K": _z(*SHAPES["k"]), "V": _z(*SHAPES["v"]), "table": _z(2, 4, dtype=I32), "lengths": _z(2, dtype=I32)}
     kp, vp = _z(*SHAPES["kp"]), _z(*SHAPES["vp"])
