@@ -1,27 +1,29 @@
 // TreeAttention: O = softmax(c Q K^T) V over a cache in pages, whose last tokens are a chain or a tree. The reference has no such node.
 //
 // Rows: a slice (an entry's group of keys and values) has tokens * share of them, the heads that share it side by side, so a page is read once for all of them. A workgroup has 64 or 128
-// rows and walks the keys in stages of 64 or 128, from the end on: S^T = K Q^T and O^T = V^T P^T by products of 32 x 32 x 16, in which a lane has a row of its own, its maximum and sum
+// rows and walks the keys in stages of 32, 64 or 128, from the end on: S^T = K Q^T and O^T = V^T P^T by products of 32 x 32 x 16, in which a lane has a row of its own, its maximum and sum
 // included; P goes from one product to the next in registers. Softmax runs in powers of two: a row has a base b, P = 2^(c' s - b) with c' = c log2 e, and sums and outputs take a factor where
 // the base moves. Scores, bases, sums and outputs are float32; with arrays of 16 bits P is rounded to their type for its product, by half a step of it, and its sum is taken of the rounded
-// values, so that weights add up to 1. float32 goes by three bfloat16 parts of each operand and the six products of them above 2^-24.
+// values, so that weights add up to 1. float32 goes by three bfloat16 parts of each operand and the six largest products of them; those left out are below 2^-21 of the product.
 // Whom a row sees: of the keys in front of the call all, of the call's its ancestors. Those fall, so a row walking back through the keys holds the next one and looks each up once in
 // a table of parents in LDS: a mask of 32 bits for 32 keys, taken where a block holds keys that some row does not see, nowhere else. Values that are not finite become 0 there, as 0 times
 // one is not a number, and the rows that do see them add them one by one.
 // Keys and values come from their pages into a ring of stages in LDS by transfers of 1 KB that no register waits for; a wave's transfer knows its page by a scalar load, and where pages are long
 // enough two to eight transfers share one. (Pages that are no whole number of transfers: through registers.)
 // Few rows and long caches leave CUs without work: the keys of all blocks are then cut into parts that are dealt to a fixed number of workgroups, by the lengths that the kernel finds, not by
-// the table's room, and a second kernel joins the parts' outputs by their bases and sums. What the first says about the cut stands in scratch memory. No atomics: results repeat.
+// the table's room, and a second kernel joins the parts' outputs by their bases and sums. What the first says about the cut stands in scratch memory. There are as many
+// workgroups as are resident, and keys are cut where no more blocks than that (and 256 entries) are: beyond, a block is one workgroup's, however long. That is behind where one entry is far longer than the
+// others: one token for each of 64 entries, 63 behind 1000 and one behind 131072, 32 heads in 8 groups of 128: 2150 us, where bytes take 156 (16 of them 114 and 117; 64 behind 1000 53 and 52).
+// No atomics but those that mark keys: results repeat.
 //
 // Bound, at heads of 128 in bfloat16 (a copy 5.1 TB/s, a product of 8192^3 1570 TFLOP/s):
-// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 69 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 55 us, 4.9 TB/s, the join 5 of them.
+// - one token, 16 entries of up to 8192, 32 heads in 8 groups: bytes. 69 to 71 us, 5.2 TB/s; one token of 16 heads in 4 groups behind 131072, in float16, 55 us, 4.9 TB/s, the join 5 of them.
 // - a prompt of 4096 behind 4096, 16 heads in 4 groups: products and powers, 214 to 231 us, 890 to 960 TFLOP/s. Of a wave's cycles 42 % issue, 34 % wait for a unit, 25 % for LDS and barriers;
 //   the matrix unit is busy for 48 % of the time in which its CU has work, which is 87 %: the longest block ends last, the second half of it with its CU to itself. The vector instructions of 32
 //   keys (a power, a multiply-add, half a conversion and half a product of pairs for each score) take about as long as their products, and the products of a wave's own are where they hide
 //   best (below). With 256 rows to a workgroup, one to a CU, calls whose blocks are all as long take 5 % less, but causal ones 11 % more: no short block stands next to a long one.
-// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 26.6 us where bytes are 9. A workgroup has about six stages. By 64 rows and eight waves, 28.3: 1.9 us to find its part, 1.4 its page, 2
-//   to the first stage, 10 for five, 1.6 for the parts' sums, and the second kernel 4.5; a stage of 64 keys takes as many cycles for its transfers' issue (64 bytes a cycle, 700) as for scores,
-//   powers and values together (930). 128 rows read every key once.
+// - 4 trees of 32 behind up to 4096, 32 heads in 8 groups: 26 us where bytes are 9, 21 of them in the first kernel and 5.4 in the second. A workgroup has about six stages, and what each waits for comes
+//   one after the other: its part, its pages, the first keys, the parts' sums. 128 rows read every key once.
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -560,8 +562,9 @@ __global__ __launch_bounds__(64 * RW * CW * KW, PER_SIMD) void tree_attention_ke
                 for (int r = r0; r < r1; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale_log2, -from));
             };
             if constexpr (AHEAD) {
-                // Vector instructions in between of the products, a few to each: a wave's own hide there almost whole (two powers with their multiply-adds behind a product of 32 cycles
-                // cost nothing, seven multiply-adds 7 %), those of the SIMD's other wave do not (as many multiply-adds 40 %).
+                // Vector instructions in between of the products, a few to each: a wave's own hide there almost whole, those of the SIMD's other wave do not. By two waves to a SIMD, in a kernel
+                // of nothing else: products with two powers and two multiply-adds behind each take 9 % longer than without, with seven multiply-adds 3 %; a wave's products beside another wave's
+                // multiply-adds, as many as take the same time alone, 35 %.
                 constexpr int EACH = 16 / QP, LATER = 8 / VT;   // powers to a product, the maxima as many as LATER
                 __builtin_amdgcn_sched_barrier(0);
                 if (u > 0) {
@@ -757,7 +760,7 @@ enum { TREE_PAIR, TREE_DEEP, TREE_TALL, TREE_FORMS };
 struct TreeForm { int rows, places; double alone, shared, start; };
 static TreeForm tree_form(int form, int bytes, bool f32) {
     const int size = bytes / (f32 ? 4 : 2);
-    // as they fit the times of 70 calls in all forms: 1 to 128 entries of 1 to 4096 tokens behind 0 to 16000, 1 to 16 heads to a group
+    // as they fit the times of calls in all forms: 1 to 128 entries of 1 to 4096 tokens behind 0 to 16000, 1 to 16 heads to a group
     const double rates[6][TREE_FORMS][2] = {{{0.55, 0.8}, {0.4, 0.4}, {0.8, 2.0}},      // 16 bits, heads of 64
                                             {{0.85, 1.4}, {0.7, 0.7}, {1.05, 1.65}},    // 128
                                             {{1.45, 1.45}, {}, {1.95, 1.95}},           // 256
@@ -769,11 +772,14 @@ static TreeForm tree_form(int form, int bytes, bool f32) {
 }
 
 // How a call is cut: which form, and how many workgroups the parts of its blocks are dealt to (0: one to a block), by what the forms take if the longest of the entries fills its table and they do
-// by two thirds. Measured, us, at heads of 128 in 16 bits, 32 heads in 8 groups (PAIR / DEEP / TALL, one workgroup to a block; the same in parts): 16 x 1 token of up to 8192 143 / 118 / 170,
-// 71 / 80 / 89; 32 x 1 of 8000 158 / 141 / 169, 129 / 144 / 173; 8 trees of 64 behind up to 4000 65 / 55 / 90, 72 / 70 / 61; 2 of 256 58 / 44 / 81, 58 / 51 / 63; 4 of 32 62 / 49 / 89,
-// 28 / 28 / 27; a prompt of 512 14.5 / 14.3 / 18, 30 / 21 / 30; of 1024 23 / 32 / 30, 36 / 23 / 38; of 2048 55 / 75 / 54, the same in parts; 4096 behind up to 4096, 16 heads in 4 groups,
-// 177 / 209 / 167, 177. Over 70 calls of all types and head sizes, measured in all
-// forms, the choices take 0.5 % more than the least on average, 8 % at most (2 chains of 512 behind up to 2048, 8 heads: 31.8, DEEP with one workgroup to a block 29.5).
+// by two thirds. Measured, us, at heads of 128 in 16 bits, 32 heads in 8 groups (PAIR / DEEP / TALL, one workgroup to a block; the same in parts): 16 x 1 token of up to 8192 147 / 120 / 174,
+// 73 / 80 / 91; 32 x 1 of 8000 156 / 139 / 168, 129 / 142 / 172; 8 trees of 64 behind 1400 to 3000 54 / 43 / 73, 67 / 60 / 59; 2 of 256 behind 1600 to 2700 54 / 42 / 75, 56 / 48 / 62; 4 of 32 behind
+// 1400 to 3800 61 / 48 / 87, 30 / 30 / 28; a prompt of 512 14.5 / 14.6 / 18, 30 / 21 / 30; of 1024 24 / 33 / 30, 36 / 24 / 38; of 2048 57 / 75 / 53, 54 / 54 / 53; 4096 behind 4096, 16 heads in 4 groups,
+// 235 / 269 / 214, 234. Over 70 calls of drawn sizes, all types and head sizes, in tables that fit, the choice takes 1 % more than the least of all forms for half of them, 5 % on average, and up to
+// 1.5 times as long (99 x 2162 tokens behind up to 2600, 2 heads of 64: PAIR 679, TALL 457).
+// A table with more columns than the lengths take is priced as if they were filled. With columns for 131072 keys the same 70 calls take 22 % more than the least on average, 30 of them 2 to 5 us for parts
+// that short caches do not need, 1.7 times as long at most; 8 trees of 64 57 for 42, 2 of 256 61 for 42, a prompt of 1024 30 for 24. One token for each of 16 to 300 entries and prompts from 2048 on are
+// as they were.
 struct TreeCut { int form, block_rows, dealt; int64_t row_blocks; };
 static TreeCut tree_cut(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t capacity, int64_t size, int type) {
     const bool f32 = type == MI355X_TYPE_FLOAT;

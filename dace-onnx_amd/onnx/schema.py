@@ -207,7 +207,8 @@ SCHEMAS: typing.List[ONNXSchema] = [
                "whose child it is, a lower number, anything else makes it a child of what is before the call. Without `parents` it sees the tokens up to itself. A table "
                "value that is no page counts as the nearest one, keys for which the table has no column do not exist, a row without keys is 0, one whose scores are all minus infinity not a number. `scale` is 1 / sqrt(D) if "
                "it is left out. In float16 and bfloat16 the probabilities are rounded to that type for their product with the values. What a row does not see does not reach "
-               "it, whatever it holds; an infinite value that it sees makes it infinite or not a number, in float32 not a number, as an infinite query or key does."),
+               "it, whatever it holds; an infinite value that it sees makes it infinite or not a number, in float32 not a number, as an infinite query or key does there; in 16 bits a key whose score is minus "
+               "infinity has no weight. Scores (with scale) are to be below 2^23, and 2^8 times a row's values added up has to be one of float32."),
     ONNXSchema("DraftAcceptance", 1,
                [ONNXParameter("logits", "T"), ONNXParameter("tokens", "I32"), ONNXParameter("parents", "I32", _O)],
                [ONNXParameter("path", "I32"), ONNXParameter("count", "I32"), ONNXParameter("next", "I32")], [],

@@ -537,7 +537,8 @@ int mi355x_paged_cache_append(const void* K, const void* V, const void* Q, void*
  * With arrays of 16 bits the probabilities are rounded to `type` for their product with V, and their sum is that of the rounded
  * ones; scores, maxima, sums and results stay in float32. In float32 an infinite query, key or value that a row sees makes it not a
  * number, and values below 2^-110 lose digits; with arrays of 16 bits an infinite value that it sees makes it infinite or not a
- * number. What a row does not see does not reach it, whatever it holds. */
+ * number. What a row does not see does not reach it, whatever it holds. Sums on the way are up to 2^8 times the row's values added
+ * up, and powers of two stand for scores (with scale) below 2^23: beyond, a row may be infinite or not a number. */
 int64_t mi355x_tree_attention_scratch(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t size,
                                       int64_t page_size, int64_t columns, int type);
 int mi355x_tree_attention(const void* Q, const void* k_pages, const void* v_pages, const int32_t* table,
