@@ -844,3 +844,12 @@ def test_attention_of_large_values(form, dealt, dtype, tuning):
     m, inputs = C.attention_model(q, kp, vp, *rest)
     expected, bound = C.attention_rows(q, kp, vp, *rest)
     assert ((m(*inputs).double() - expected).norm(dim=-1) <= bound).all()
+
+
+@pytest.mark.parametrize("form, dealt", [(0, 0), (1, 0), (2, 0), (0, 512), (1, 256), (2, 256)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [11, 16])
+def test_rows_in_float32_of_long_contexts(form, dealt, d, page, tuning):
+    """Trees behind 9000 keys, in every form, pages that go through registers and that do not."""
+    tuning(MI355X_TREE_FORM=form, MI355X_TREE_DEAL=dealt)
+    check_rows(2, 12, 4, 2, d, page, 9000, F32, True)
